@@ -322,7 +322,7 @@ def _plain_plan(s):
     need = torch.where(new >= 0, (cached + fresh + page - 1) // page - held, 0)
     upto = torch.cumsum(need, 0)
     served = (new >= 0) & ((need == 0) | (upto <= tail - head))
-    taken = torch.where(served, upto, 0).amax()
+    taken = torch.where(served & (need > 0), upto, 0).amax()
     col = torch.arange(width, device=DEV)[None]
     mine = served[:, None] & (col >= held[:, None]) & (col < (held + need)[:, None])
     at = (head + (upto - need)[:, None] + col - held[:, None]) % size
@@ -342,7 +342,7 @@ def _plain_plan(s):
     lens = torch.where(new < 0, 0, torch.where(served, cached + fresh, cached))
     counts = torch.stack([cu[-1], taken, back_upto[-1], ((new >= 0) & ~served).sum()])
     return {"table": table, "ring": ring, "ring_out": torch.stack([head + taken, tail + back_upto[-1]]),
-            "token_row": torch.where(live, row, -1).to(torch.int32), "positions": torch.where(live, pos, -1),
+            "token_row": torch.where(live, row, -1).to(torch.int32), "positions": torch.where(live & served[row], pos, -1),
             "slots": torch.where(live & served[row], slot, -1), "cu_new": cu.to(torch.int32),
             "lens": lens.to(torch.int32), "counts": counts.to(torch.int32)}
 
