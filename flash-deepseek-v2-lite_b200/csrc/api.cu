@@ -323,9 +323,10 @@ int dsv2_stream_check(void* stream) {
     return check_launch(e, "stream_check: read device error");
   if (code == 0) return DSV2_OK;
   static const char* what[] = {"none", "a bounded wait gave up", "an index was out of range",
-                               "tensor memory allocation failed"};
+                               "tensor memory allocation failed",
+                               "an infinity or NaN was written to the 4-bit cache"};
   return fail(DSV2_ERR_DEVICE, "device error word %d (%s); read and clear it with dsv2_get_device_error",
-              code, code >= 0 && code <= 3 ? what[code] : "unknown");
+              code, code >= 0 && code <= 4 ? what[code] : "unknown");
 }
 
 int dsv2_reset_progress(void* counters, int64_t count, void* stream) {
@@ -810,13 +811,17 @@ int dsv2_gather_rows(const void* x, int64_t x_row_stride, const int32_t* route_t
                       "gather_rows");
 }
 
-int dsv2_mla_prep(const dsv2_mla_prep_args* a, void* stream) {
-  if (!a || !a->qkva || !a->kv_norm_w || !a->cos_tab || !a->sin_tab || !a->positions || !a->cache ||
-      !a->q_pe_out)
+// cache4 != nullptr: into the slots of the 4-bit cache instead of a->cache
+static int mla_prep_impl(const dsv2_mla_prep_args* a, void* cache4, int64_t n_blocks, const int64_t* slots,
+                         void* stream) {
+  const bool q4 = cache4 != nullptr;
+  if (!a || !a->qkva || !a->kv_norm_w || !a->cos_tab || !a->sin_tab || !a->positions ||
+      (!q4 && !a->cache) || !a->q_pe_out)
     return fail(DSV2_ERR_INVALID, "mla_prep: null pointer");
   if (a->pos_numel != 1 && a->pos_numel != a->batch)
     return fail(DSV2_ERR_INVALID, "mla_prep: positions numel %d for batch %d", a->pos_numel, a->batch);
-  if (!aligned16(a->qkva) || a->qkva_row_stride % 8 || !aligned16(a->cache) || a->cache_b_stride % 8)
+  if (!aligned16(a->qkva) || a->qkva_row_stride % 8 || !aligned16(q4 ? cache4 : a->cache) ||
+      (!q4 && a->cache_b_stride % 8))
     return fail(DSV2_ERR_INVALID, "mla_prep: operands must be 16-byte aligned");
   if (a->rope_stride < 32) return fail(DSV2_ERR_INVALID, "mla_prep: rope table stride %lld < 32", (long long)a->rope_stride);
   if (a->batch <= 0) return DSV2_OK;
@@ -848,7 +853,22 @@ int dsv2_mla_prep(const dsv2_mla_prep_args* a, void* stream) {
   p.cache_b_stride = a->cache_b_stride;
   p.max_len = a->max_len;
   p.q_pe_out = reinterpret_cast<bf16*>(a->q_pe_out);
+  if (q4) {
+    p.cache4 = static_cast<unsigned char*>(cache4);
+    p.cache4_blocks = n_blocks;
+    p.slots = reinterpret_cast<const long long*>(slots);
+    return check_launch(launch_mla_prep_q4(p, a->batch, static_cast<cudaStream_t>(stream)), "mla_prep_q4");
+  }
   return check_launch(launch_mla_prep(p, a->batch, static_cast<cudaStream_t>(stream)), "mla_prep");
+}
+
+int dsv2_mla_prep(const dsv2_mla_prep_args* a, void* stream) { return mla_prep_impl(a, nullptr, 0, nullptr, stream); }
+
+int dsv2_mla_prep_q4(const dsv2_mla_prep_args* a, void* cache4, int64_t n_blocks, const int64_t* slots,
+                     void* stream) {
+  if (!cache4 || !slots) return fail(DSV2_ERR_INVALID, "mla_prep_q4: null pointer");
+  if (n_blocks <= 0) return fail(DSV2_ERR_INVALID, "mla_prep_q4: n_blocks %lld", (long long)n_blocks);
+  return mla_prep_impl(a, cache4, n_blocks, slots, stream);
 }
 
 int dsv2_mla_decode(const dsv2_mla_decode_args* a, void* stream) {

@@ -1,0 +1,179 @@
+// extern "C" entry points of the paged 4-bit serving operators (declared in include/dsv2.h).
+// Same rules as api.cu (which this file follows in the translation unit): arguments are
+// checked here, nothing allocates device memory or synchronises.
+
+namespace {
+
+// rows of a latent4 call: [n, 576] bf16 with 16-byte aligned rows
+int latent4_args(const char* what, const void* rows, int64_t row_stride, const int64_t* slots, int64_t n,
+                 const void* cache, int64_t n_blocks) {
+  if (n < 0) return fail(DSV2_ERR_INVALID, "%s: n %lld", what, (long long)n);
+  if (n > 0 && (!rows || !slots || !cache)) return fail(DSV2_ERR_INVALID, "%s: null pointer", what);
+  if (n > 0x7fffffffLL) return fail(DSV2_ERR_UNSUPPORTED, "%s: n %lld exceeds one launch", what, (long long)n);
+  if (n_blocks <= 0) return fail(DSV2_ERR_INVALID, "%s: n_blocks %lld", what, (long long)n_blocks);
+  if (!aligned16(rows) || !aligned16(cache) || row_stride % 8 || row_stride < 576)
+    return fail(DSV2_ERR_INVALID, "%s: rows of 576 elements and the cache must be 16-byte aligned", what);
+  return DSV2_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dsv2_page_plan(const dsv2_page_plan_args* a, void* stream) {
+  if (!a || !a->free_ring || !a->ring_in || !a->ring_out || !a->cu_new || !a->counts || !a->sync)
+    return fail(DSV2_ERR_INVALID, "page_plan: null pointer");
+  if (a->requests < 0 || a->width <= 0 || a->ring_size <= 0 || a->token_capacity < 0 || a->table_stride < a->width)
+    return fail(DSV2_ERR_INVALID, "page_plan: requests %d width %d ring %lld capacity %d", a->requests, a->width,
+                (long long)a->ring_size, a->token_capacity);
+  if (a->requests > 0 && (!a->cached || !a->fresh || !a->lens || !a->block_table))
+    return fail(DSV2_ERR_INVALID, "page_plan: null pointer");
+  if (a->token_capacity > 0 && (!a->token_row || !a->positions || !a->slots))
+    return fail(DSV2_ERR_INVALID, "page_plan: null pointer");
+  if (a->page_size <= 0 || a->page_size % DSV2_L4_BLOCK_TOKENS)
+    return fail(DSV2_ERR_INVALID, "page_plan: page_size %d (a positive multiple of %d)", a->page_size,
+                DSV2_L4_BLOCK_TOKENS);
+  if (static_cast<int64_t>(a->width) * a->page_size > 0x7fffffffLL)
+    return fail(DSV2_ERR_UNSUPPORTED, "page_plan: a table row of %d pages of %d tokens exceeds 2^31 tokens", a->width,
+                a->page_size);
+  const char* c = static_cast<const char*>(a->cached);
+  const char* l = reinterpret_cast<const char*>(a->lens);
+  const int64_t c_bytes = static_cast<int64_t>(a->requests) * (a->cached_is64 ? 8 : 4), l_bytes = static_cast<int64_t>(a->requests) * 4;
+  if (a->requests > 0 && c < l + l_bytes && l < c + c_bytes)
+    return fail(DSV2_ERR_INVALID, "page_plan: lens must not overlap cached");
+  int sms = 0;
+  if (int rc = ensure_init(&sms)) return rc;
+  PagePlanParams p = {};
+  p.cached = a->cached;
+  p.cached64 = a->cached_is64 != 0;
+  p.fresh = a->fresh;
+  p.requests = a->requests;
+  p.page = a->page_size;
+  p.table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.width = a->width;
+  p.ring = a->free_ring;
+  p.ring_size = a->ring_size;
+  p.ring_in = reinterpret_cast<const long long*>(a->ring_in);
+  p.ring_out = reinterpret_cast<long long*>(a->ring_out);
+  p.capacity = a->token_capacity;
+  p.token_row = a->token_row;
+  p.positions = reinterpret_cast<long long*>(a->positions);
+  p.slots = reinterpret_cast<long long*>(a->slots);
+  p.cu_new = a->cu_new;
+  p.lens = a->lens;
+  p.counts = a->counts;
+  p.sync = a->sync;
+  return check_launch(launch_page_plan(p, sms, static_cast<cudaStream_t>(stream)), "page_plan");
+}
+
+int dsv2_latent4_write(const void* rows, int64_t row_stride, const int64_t* slots, int64_t n, void* cache,
+                       int64_t n_blocks, void* stream) {
+  if (int rc = latent4_args("latent4_write", rows, row_stride, slots, n, cache, n_blocks)) return rc;
+  if (n == 0) return DSV2_OK;
+  Latent4Params p = {};
+  p.rows = static_cast<const bf16*>(rows);
+  p.row_stride = row_stride;
+  p.slots = reinterpret_cast<const long long*>(slots);
+  p.n = n;
+  p.cache = static_cast<unsigned char*>(cache);
+  p.n_blocks = n_blocks;
+  return check_launch(launch_latent4_write(p, static_cast<cudaStream_t>(stream)), "latent4_write");
+}
+
+int dsv2_latent4_read(const void* cache, int64_t n_blocks, const int64_t* slots, int64_t n, void* out,
+                      int64_t out_row_stride, void* stream) {
+  if (int rc = latent4_args("latent4_read", out, out_row_stride, slots, n, cache, n_blocks)) return rc;
+  if (n == 0) return DSV2_OK;
+  Latent4Params p = {};
+  p.out = static_cast<bf16*>(out);
+  p.row_stride = out_row_stride;
+  p.slots = reinterpret_cast<const long long*>(slots);
+  p.n = n;
+  p.cache = static_cast<unsigned char*>(const_cast<void*>(cache));
+  p.n_blocks = n_blocks;
+  return check_launch(launch_latent4_read(p, static_cast<cudaStream_t>(stream)), "latent4_read");
+}
+
+int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* a, void* stream) {
+  if (!a) return fail(DSV2_ERR_INVALID, "mla_decode_q4: null pointer");
+  if (a->rows < 0 || a->seqs <= 0 || a->width <= 0 || a->n_blocks <= 0 || a->table_stride < a->width)
+    return fail(DSV2_ERR_INVALID, "mla_decode_q4: rows %d seqs %d width %d blocks %lld", a->rows, a->seqs, a->width,
+                (long long)a->n_blocks);
+  if (a->rows == 0) return DSV2_OK;
+  if (!a->q_abs || !a->q_pe || !a->cache || !a->block_table || !a->positions || !a->o_lat)
+    return fail(DSV2_ERR_INVALID, "mla_decode_q4: null pointer");
+  if (a->page_size <= 0 || a->page_size % DSV2_L4_BLOCK_TOKENS)
+    return fail(DSV2_ERR_INVALID, "mla_decode_q4: page_size %d (a positive multiple of %d)", a->page_size,
+                DSV2_L4_BLOCK_TOKENS);
+  if (static_cast<int64_t>(a->width) * a->page_size > 0x7fffffffLL)
+    return fail(DSV2_ERR_UNSUPPORTED, "mla_decode_q4: a table row of %d pages of %d tokens exceeds 2^31 tokens",
+                a->width, a->page_size);
+  if (!aligned16(a->q_abs) || !aligned16(a->q_pe) || !aligned16(a->cache) || !aligned16(a->o_lat))
+    return fail(DSV2_ERR_INVALID, "mla_decode_q4: operands must be 16-byte aligned");
+  if (int rc = ensure_init(nullptr)) return rc;
+  MlaQ4Params p = {};
+  p.q_abs = static_cast<const bf16*>(a->q_abs);
+  p.q_pe = static_cast<const bf16*>(a->q_pe);
+  p.cache = static_cast<const unsigned char*>(a->cache);
+  p.n_blocks = a->n_blocks;
+  p.table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.width = a->width;
+  p.seqs = a->seqs;
+  p.page_blocks = a->page_size / DSV2_L4_BLOCK_TOKENS;
+  p.positions = reinterpret_cast<const long long*>(a->positions);
+  p.seq_rows = a->seq_rows;
+  p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  p.o_lat = static_cast<bf16*>(a->o_lat);
+  p.rows = a->rows;
+  if (!a->seq_rows && a->seqs < a->rows)
+    return fail(DSV2_ERR_INVALID, "mla_decode_q4: %d query rows, %d table rows (pass seq_rows)", a->rows, a->seqs);
+  return check_launch(launch_mla_q4(p, static_cast<cudaStream_t>(stream)), "mla_decode_q4");
+}
+
+int dsv2_lora(const dsv2_lora_args* a, void* stream) {
+  if (!a) return fail(DSV2_ERR_INVALID, "lora: null pointer");
+  if (a->tokens < 0 || a->adapters < 0 || a->n_base < 0 || a->ids_len < 0)
+    return fail(DSV2_ERR_INVALID, "lora: tokens %d adapters %d partials %d", a->tokens, a->adapters, a->n_base);
+  if (a->tokens == 0) return DSV2_OK;
+  if (!a->x || !a->ids || !a->y || !a->low || (a->adapters > 0 && (!a->a || !a->b || !a->ranks || !a->scales)) ||
+      (a->n_base > 0 && !a->base))
+    return fail(DSV2_ERR_INVALID, "lora: null pointer");
+  if (!a->token_row && a->ids_len < a->tokens)
+    return fail(DSV2_ERR_INVALID, "lora: %d ids for %d tokens (pass token_row)", a->ids_len, a->tokens);
+  if (a->k <= 0 || a->n <= 0 || a->rank <= 0 || a->k % 8 || a->n % 8 || a->rank % 8 || a->rank > 128)
+    return fail(DSV2_ERR_UNSUPPORTED, "lora: k %d, n %d, rank %d (multiples of 8, rank at most 128)", a->k, a->n, a->rank);
+  if (a->y_dtype != DSV2_BF16 && a->y_dtype != DSV2_F32) return fail(DSV2_ERR_UNSUPPORTED, "lora: y dtype %d", a->y_dtype);
+  if (!aligned16(a->x) || !aligned16(a->a) || !aligned16(a->b) || !aligned16(a->base) || !aligned16(a->low) ||
+      !aligned16(a->y) || a->x_row_stride % 8 || a->base_part_stride % 4 || a->base_row_stride % 4 ||
+      a->y_row_stride % (a->y_dtype == DSV2_F32 ? 4 : 8))
+    return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
+  if (int rc = ensure_init(nullptr)) return rc;
+  LoraParams p = {};
+  p.x = static_cast<const bf16*>(a->x);
+  p.x_row_stride = a->x_row_stride;
+  p.a = static_cast<const bf16*>(a->a);
+  p.b = static_cast<const bf16*>(a->b);
+  p.ids = a->ids;
+  p.token_row = a->token_row;
+  p.ranks = a->ranks;
+  p.scales = a->scales;
+  p.adapters = a->adapters;
+  p.rank = a->rank;
+  p.tokens = a->tokens;
+  p.k = a->k;
+  p.n = a->n;
+  p.ids_len = a->ids_len;
+  p.low = a->low;
+  p.base = a->base;
+  p.base_parts = a->n_base;
+  p.base_part_stride = a->base_part_stride;
+  p.base_row_stride = a->base_row_stride;
+  p.y = a->y;
+  p.y_f32 = a->y_dtype == DSV2_F32;
+  p.y_row_stride = a->y_row_stride;
+  return check_launch(launch_lora(p, static_cast<cudaStream_t>(stream)), "lora");
+}
+
+}  // extern "C"

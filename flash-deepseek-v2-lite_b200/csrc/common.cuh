@@ -28,6 +28,7 @@ enum DeviceError : int {
   kErrMbarTimeout = 1,
   kErrIndex = 2,
   kErrTmemAlloc = 3,
+  kErrNonFinite = 4,   // an infinity or NaN was given to the 4-bit cache, which cannot hold it
 };
 
 // Defined here: the library is one translation unit (dsv2_all.cu).

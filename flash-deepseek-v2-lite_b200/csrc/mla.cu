@@ -27,6 +27,7 @@
 // mla_combine_kernel merges the split partials of the tcgen05 kernel (mla_tc.cu).
 #include <algorithm>
 
+#include "latent4.cuh"
 #include "params.cuh"
 
 namespace dsv2 {
@@ -57,6 +58,9 @@ constexpr int kMlaMaxCtas = 160;                // merge scratch: 2 x 16 x CTAs 
 // mla_prep: latent RMSNorm + RoPE + cache write for the new token, RoPE of q_pe
 // ----------------------------------------------------------------------------
 
+// kQ4: the row goes into its slot of the paged 4-bit cache (latent4.cuh) instead of a bf16 row,
+// quantised from the same bf16-rounded values; a row with a negative position is padding.
+template <bool kQ4>
 __global__ __launch_bounds__(256) void mla_prep_kernel(const MlaPrepParams p) {
   const int t = threadIdx.x;
   // the latent norm weights are never written by earlier kernels: load them before the wait
@@ -72,8 +76,9 @@ __global__ __launch_bounds__(256) void mla_prep_kernel(const MlaPrepParams p) {
   // position, cache row and this thread's RoPE coefficients (every RoPE pair of thread t
   // has pair index t % 32) are fetched while the split-K partials are in flight
   const long long pos = p.positions[p.pos_numel == 1 ? 0 : b];
-  const bool pos_ok = (pos >= 0 && pos < p.max_len && pos < p.rope_rows);
-  const int cr = p.cache_rows ? p.cache_rows[b] : b;
+  const bool pos_ok = (pos >= 0 && (kQ4 || pos < p.max_len) && pos < p.rope_rows);
+  const int cr = kQ4 ? 0 : (p.cache_rows ? p.cache_rows[b] : b);
+  const long long slot = kQ4 ? p.slots[b] : 0;
   float rc = 0.f, rs = 0.f;
   if (pos_ok) {
     rc = p.cos_tab[pos * p.rope_stride + (t & 31)];
@@ -134,14 +139,21 @@ __global__ __launch_bounds__(256) void mla_prep_kernel(const MlaPrepParams p) {
     }
   }
   if (!pos_ok) {
+    if (kQ4 && pos < 0) return;   // padding
     if (threadIdx.x == 0) set_device_error(kErrIndex);
     return;
   }
-  if (cr < 0 || cr >= p.cache_batch) {
+  if (!kQ4 && (cr < 0 || cr >= p.cache_batch)) {
     if (threadIdx.x == 0) set_device_error(kErrIndex);
     return;
   }
-  bf16* crow = p.cache + static_cast<long long>(cr) * p.cache_b_stride + pos * kRow;
+  if (kQ4 && slot >= p.cache4_blocks * kL4Tokens) {
+    if (threadIdx.x == 0) set_device_error(kErrIndex);
+    return;
+  }
+  bf16* crow = kQ4 ? nullptr : p.cache + static_cast<long long>(cr) * p.cache_b_stride + pos * kRow;
+  unsigned char* blk = kQ4 && slot >= 0 ? p.cache4 + (slot >> 4) * kL4BlockBytes : nullptr;
+  const int tok = static_cast<int>(slot & (kL4Tokens - 1));
   // latent RMSNorm: threads 0..63 own 8 elements each
   float v[8];
   float ss = 0.f;
@@ -165,7 +177,29 @@ __global__ __launch_bounds__(256) void mla_prep_kernel(const MlaPrepParams p) {
     uint32_t* op = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
     for (int j = 0; j < 4; ++j) op[j] = pack_bf16x2(v[2 * j] * inv * kw[2 * j], v[2 * j + 1] * inv * kw[2 * j + 1]);
-    *reinterpret_cast<uint4*>(crow + t * 8) = o;
+    if constexpr (kQ4) {
+      // thread t owns word t & 3 of group t >> 2; the group's maximum is over 4 threads
+      float x[8];
+      float amax = 0.f;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[2 * j] = bf16lo(op[j]);
+        x[2 * j + 1] = bf16hi(op[j]);
+        amax = fmaxf(amax, fmaxf(fabsf(x[2 * j]), fabsf(x[2 * j + 1])));
+        bad |= l4_nonfinite(op[j]);
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int code = l4_code(amax);
+      if (blk) {
+        *reinterpret_cast<uint32_t*>(blk + l4_word_off(tok, t >> 2, t & 3)) = l4_pack(x, l4_scale(code));
+        if ((t & 3) == 0) blk[kL4ScaleOff + 16 * (t >> 2) + l4_scale_place(tok)] = static_cast<unsigned char>(code);
+        if (bad) set_device_error(kErrNonFinite);
+      }
+    } else {
+      *reinterpret_cast<uint4*>(crow + t * 8) = o;
+    }
   }
   // RoPE pairs: 16 heads x 32 pairs of q_pe, plus 32 pairs of k_pe
   for (int i = t; i < (kHeads + 1) * 32; i += 256) {
@@ -176,8 +210,12 @@ __global__ __launch_bounds__(256) void mla_prep_kernel(const MlaPrepParams p) {
     const uint32_t packed = pack_bf16x2(re, im);
     if (h < kHeads)
       *reinterpret_cast<uint32_t*>(p.q_pe_out + (static_cast<long long>(b) * kHeads + h) * kRope + 2 * j) = packed;
-    else
+    else if constexpr (kQ4) {
+      if (blk) *reinterpret_cast<uint32_t*>(blk + l4_rope_off(tok, j)) = packed;
+      if (blk && l4_nonfinite(packed)) set_device_error(kErrNonFinite);
+    } else {
       *reinterpret_cast<uint32_t*>(crow + kLatent + 2 * j) = packed;
+    }
   }
 }
 
@@ -882,7 +920,12 @@ static_assert(mla_decode_smem_bytes() <= 232448, "latent-attention shared memory
 static_assert(2 * kHeads * kMlaMaxCtas * sizeof(float) <= kStages * kTileBytes, "merge scratch exceeds the ring");
 
 cudaError_t launch_mla_prep(const MlaPrepParams& p, int batch, cudaStream_t st) {
-  launch_kernel(mla_prep_kernel, batch, 256, 0, st, p);
+  launch_kernel(mla_prep_kernel<false>, batch, 256, 0, st, p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_mla_prep_q4(const MlaPrepParams& p, int batch, cudaStream_t st) {
+  launch_kernel(mla_prep_kernel<true>, batch, 256, 0, st, p);
   return cudaGetLastError();
 }
 

@@ -96,6 +96,84 @@ struct MlaPrepParams {
   bf16* q_pe_out;              // [B, 16, 64]
   const int* cache_rows;       // optional [B]: cache row of input row b (else b)
   int cache_batch;             // rows of the cache
+  // 4-bit paged cache instead of `cache` (latent4.cuh)
+  unsigned char* cache4;
+  long long cache4_blocks;     // 16-token blocks of it
+  const long long* slots;      // [B] slot of the new token (negative: no cache write)
+};
+
+// Rows <-> slots of the 4-bit latent cache (latent4.cu)
+struct Latent4Params {
+  const bf16* rows;            // write: [n, 576] source rows
+  bf16* out;                   // read: [n, 576] destination rows
+  long long row_stride;
+  const long long* slots;      // [n], negative = padding
+  long long n;
+  unsigned char* cache;
+  long long n_blocks;
+};
+
+// Page tables, slots and positions of a serving step (page_plan.cu)
+struct PagePlanParams {
+  const void* cached;          // [requests] int32 or int64 (cached64)
+  int cached64;
+  const int* fresh;            // [requests] tokens to append; -1 = finished
+  int requests;
+  int page;
+  int* table;                  // [requests, width] at table_stride
+  long long table_stride;
+  int width;
+  int* ring;                   // [ring_size] free pages
+  long long ring_size;
+  const long long* ring_in;    // {taken, put} counters
+  long long* ring_out;
+  int capacity;                // token rows
+  int* token_row;
+  long long* positions;
+  long long* slots;
+  int* cu_new;                 // [requests + 1]
+  int* lens;                   // [requests]
+  int* counts;                 // {tokens, pages taken, pages returned, requests not served}
+  int* sync;                   // one ticket, left zero
+};
+
+// Latent attention over the paged 4-bit cache (mla_q4.cu)
+struct MlaQ4Params {
+  const bf16* q_abs;           // [rows, 16, 512]
+  const bf16* q_pe;            // [rows, 16, 64]
+  const unsigned char* cache;
+  long long n_blocks;          // 16-token blocks of the cache
+  const int* table;            // [seqs, width] pages at table_stride
+  long long table_stride;
+  int width;
+  int seqs;
+  int page_blocks;             // 16-token blocks per page
+  const long long* positions;  // [rows], attended length = position + 1
+  const int* seq_rows;         // optional [rows]: table row of each query row (negative: none)
+  float scale_log2;
+  bf16* o_lat;                 // [rows, 16, 512]
+  int rows;
+};
+
+// Low-rank adapters of many requests (lora.cu)
+struct LoraParams {
+  const bf16* x;               // [tokens, k]
+  long long x_row_stride;
+  const bf16* a;               // [adapters, rank, k]
+  const bf16* b;               // [adapters, n, rank]
+  const int* ids;              // [tokens] (or per request with token_row), negative = none
+  const int* token_row;        // optional [tokens]: request of each token (negative: none)
+  const int* ranks;            // [adapters] used rank
+  const float* scales;         // [adapters]
+  int adapters, rank, tokens, k, n;
+  int ids_len;
+  float* low;                  // [tokens, rank] work buffer
+  const float* base;           // optional fp32 partials of the shared projection, summed in order
+  int base_parts;
+  long long base_part_stride, base_row_stride;
+  void* y;                     // [tokens, n] bf16 or fp32
+  int y_f32;
+  long long y_row_stride;
 };
 
 struct MlaDecodeParams {
@@ -157,6 +235,13 @@ cudaError_t launch_gather_rows(const void*, long long, const int*, const int*, i
                                int, cudaStream_t);
 // mla.cu
 cudaError_t launch_mla_prep(const MlaPrepParams&, int, cudaStream_t);
+cudaError_t launch_mla_prep_q4(const MlaPrepParams&, int, cudaStream_t);
+// latent4.cu, page_plan.cu, mla_q4.cu, lora.cu
+cudaError_t launch_latent4_write(const Latent4Params&, cudaStream_t);
+cudaError_t launch_latent4_read(const Latent4Params&, cudaStream_t);
+cudaError_t launch_page_plan(const PagePlanParams&, int num_sms, cudaStream_t);
+cudaError_t launch_mla_q4(const MlaQ4Params&, cudaStream_t);
+cudaError_t launch_lora(const LoraParams&, cudaStream_t);
 cudaError_t mla_decode_init();
 int mla_decode_grid(const MlaDecodeParams&, int num_sms, long long part_slots);
 cudaError_t launch_mla_decode(const MlaDecodeParams&, const CUtensorMap& tm_kv, const CUtensorMap& tm_qa,

@@ -108,6 +108,35 @@ class MlaDecodeArgs(ctypes.Structure):
     ]
 
 
+class PagePlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("cached", c_vp), ("fresh", c_vp), ("block_table", c_vp), ("free_ring", c_vp), ("ring_in", c_vp),
+        ("ring_out", c_vp), ("token_row", c_vp), ("positions", c_vp), ("slots", c_vp), ("cu_new", c_vp),
+        ("lens", c_vp), ("counts", c_vp), ("sync", c_vp),
+        ("table_stride", c_i64), ("ring_size", c_i64),
+        ("requests", c_i32), ("width", c_i32), ("page_size", c_i32), ("token_capacity", c_i32),
+        ("cached_is64", c_i32),
+    ]
+
+
+class MlaDecodeQ4Args(ctypes.Structure):
+    _fields_ = [
+        ("q_abs", c_vp), ("q_pe", c_vp), ("cache", c_vp), ("n_blocks", c_i64), ("block_table", c_vp),
+        ("table_stride", c_i64), ("width", c_i32), ("seqs", c_i32), ("page_size", c_i32), ("rows", c_i32),
+        ("positions", c_vp), ("seq_rows", c_vp), ("softmax_scale", c_f32), ("o_lat", c_vp),
+    ]
+
+
+class LoraArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("x_row_stride", c_i64), ("a", c_vp), ("b", c_vp), ("ids", c_vp), ("token_row", c_vp),
+        ("ranks", c_vp), ("scales", c_vp), ("base", c_vp), ("base_part_stride", c_i64),
+        ("base_row_stride", c_i64), ("low", c_vp), ("y", c_vp), ("y_row_stride", c_i64),
+        ("y_dtype", c_i32), ("n_base", c_i32), ("ids_len", c_i32), ("adapters", c_i32), ("rank", c_i32),
+        ("tokens", c_i32), ("k", c_i32), ("n", c_i32),
+    ]
+
+
 _SIGNATURES = {
     "dsv2_version": ([], c_i32),
     "dsv2_last_error": ([], ctypes.c_char_p),
@@ -146,6 +175,12 @@ _SIGNATURES = {
     "dsv2_mla_decode": ([ctypes.POINTER(MlaDecodeArgs), c_vp], c_i32),
     "dsv2_mla_decode_noalloc": ([c_vp, c_vp, c_vp, c_i64, c_i32, c_vp, c_i32, c_f32, c_i32, c_vp, c_i32, c_vp],
                                 c_i32),
+    "dsv2_page_plan": ([ctypes.POINTER(PagePlanArgs), c_vp], c_i32),
+    "dsv2_latent4_write": ([c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp], c_i32),
+    "dsv2_latent4_read": ([c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp], c_i32),
+    "dsv2_mla_prep_q4": ([ctypes.POINTER(MlaPrepArgs), c_vp, c_i64, c_vp, c_vp], c_i32),
+    "dsv2_mla_decode_q4": ([ctypes.POINTER(MlaDecodeQ4Args), c_vp], c_i32),
+    "dsv2_lora": ([ctypes.POINTER(LoraArgs), c_vp], c_i32),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -15,13 +15,16 @@ import torch
 from . import _lib
 from ._lib import (
     DSV2_BF16, DSV2_F16, DSV2_F32, EPI_STORE_BF16, EPI_STORE_F32, EPI_SWIGLU, EPI_SCALE_F32,
-    FAMILY_SMALL, FAMILY_BATCH, LinearArgs, MlaDecodeArgs, MlaPrepArgs, MoeArgs, PeerTable, RouterArgs,
+    FAMILY_SMALL, FAMILY_BATCH, LinearArgs, LoraArgs, MlaDecodeArgs, MlaDecodeQ4Args, MlaPrepArgs, MoeArgs,
+    PagePlanArgs, PeerTable, RouterArgs,
 )
 
 __all__ = [
     "stream", "rmsnorm", "add_rmsnorm", "embed_rmsnorm", "residual_add", "silu_mul", "sum_partials",
     "prepare_decode_inputs", "copy_token_to_cache", "advance_positions", "linear",
     "router", "softmax_topk", "moe_bucket", "gather_rows", "moe", "mla_prep", "mla_decode", "mla_splits", "mla_workspace", "lm_head_argmax",
+    "latent4_cache", "page_plan", "page_plan_buffers", "latent4_write", "latent4_read", "mla_prep_q4", "mla_decode_q4",
+    "mla_q4_workspace", "lora", "lora_linear", "lora_workspace",
     "EPI_STORE_BF16", "EPI_STORE_F32", "EPI_SWIGLU", "EPI_SCALE_F32", "FAMILY_SMALL", "FAMILY_BATCH",
 ]
 
@@ -373,16 +376,8 @@ def _check_cache(cache: torch.Tensor) -> None:
         raise NotImplementedError("latent cache must be [B, max_len, 576] with contiguous 576-wide rows")
 
 
-def mla_prep(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos: torch.Tensor,
-             sin: torch.Tensor, positions: torch.Tensor, cache: torch.Tensor,
-             q_pe_out: torch.Tensor, q_nope_out: torch.Tensor | None = None,
-             cache_rows: torch.Tensor | None = None) -> None:
-    """New-token preparation for one layer.
-
-    qkva: bf16 [B, 3648], or fp32 split-K partial sums [S, B, 3648] (summed here);
-    cache: [rows, max_len, 576] (one layer); positions int64 [1] or [B];
-    q_nope_out (optional): bf16 [B, 16, 128] copy of the (summed) q_nope;
-    cache_rows (optional): int32 [B], the cache row of each input row (default: row b)."""
+def _mla_prep_args(qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos: torch.Tensor, sin: torch.Tensor,
+                   positions: torch.Tensor, q_pe_out: torch.Tensor, q_nope_out: torch.Tensor | None) -> MlaPrepArgs:
     _cuda(qkva, "qkva")
     if qkva.dim() == 2 and qkva.dtype == torch.bfloat16:
         dt, parts, pstride, rstride, batch = DSV2_BF16, 1, 0, qkva.stride(0), qkva.shape[0]
@@ -398,7 +393,6 @@ def mla_prep(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos: to
         raise NotImplementedError("q_nope_out must be a contiguous bf16 [B, 16, 128] tensor")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise NotImplementedError("rope tables must be fp32")
-    _check_cache(cache)
     a = MlaPrepArgs()
     a.qkva = qkva.data_ptr()
     a.qkva_row_stride = rstride
@@ -410,22 +404,37 @@ def mla_prep(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos: to
     a.rope_rows = cos.shape[0]
     a.positions = positions.data_ptr()
     a.pos_numel = positions.numel()
-    a.cache = cache.data_ptr()
-    a.cache_b_stride = cache.stride(0)
-    a.max_len = cache.shape[1]
     a.q_pe_out = q_pe_out.data_ptr()
     a.batch = batch
     a.qkva_dtype = dt
     a.qkva_parts = parts
     a.qkva_part_stride = pstride
     a.q_nope_out = _ptr(q_nope_out)
+    return a
+
+
+def mla_prep(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos: torch.Tensor,
+             sin: torch.Tensor, positions: torch.Tensor, cache: torch.Tensor,
+             q_pe_out: torch.Tensor, q_nope_out: torch.Tensor | None = None,
+             cache_rows: torch.Tensor | None = None) -> None:
+    """New-token preparation for one layer.
+
+    qkva: bf16 [B, 3648], or fp32 split-K partial sums [S, B, 3648] (summed here);
+    cache: [rows, max_len, 576] (one layer); positions int64 [1] or [B];
+    q_nope_out (optional): bf16 [B, 16, 128] copy of the (summed) q_nope;
+    cache_rows (optional): int32 [B], the cache row of each input row (default: row b)."""
+    a = _mla_prep_args(qkva, kv_norm_w, eps, cos, sin, positions, q_pe_out, q_nope_out)
+    _check_cache(cache)
+    a.cache = cache.data_ptr()
+    a.cache_b_stride = cache.stride(0)
+    a.max_len = cache.shape[1]
     a.cache_batch = cache.shape[0]
     if cache_rows is not None:
         _cuda(cache_rows, "cache_rows")
-        if cache_rows.dtype != torch.int32 or cache_rows.numel() < batch:
+        if cache_rows.dtype != torch.int32 or cache_rows.numel() < a.batch:
             raise ValueError("cache_rows must be int32 with one entry per input row")
         a.cache_rows = cache_rows.data_ptr()
-    elif cache.shape[0] < batch:
+    elif cache.shape[0] < a.batch:
         raise ValueError("the cache has fewer rows than the batch (pass cache_rows)")
     _lib.call("dsv2_mla_prep", ctypes.byref(a), stream())
 
@@ -516,3 +525,230 @@ def mla_decode(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tensor, 
             raise ValueError("part_count must be int32 [2]")
         a.part_count = part_count.data_ptr()
     _lib.call("dsv2_mla_decode", ctypes.byref(a), stream())
+
+
+# ---------------------------------------------------------------- paged 4-bit serving
+L4_BLOCK_TOKENS = 16     # tokens of a block of the 4-bit latent cache
+L4_BLOCK_BYTES = 6400    # its bytes (include/dsv2.h describes them)
+
+
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int | None = None) -> int:
+    """Address of a contiguous CUDA tensor of this dtype (and at least numel elements) on the
+    current device."""
+    if not t.is_cuda:
+        raise NotImplementedError(f"{name} must be a CUDA tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise NotImplementedError(f"{name} must be contiguous")
+    if numel is not None and t.numel() < numel:
+        raise ValueError(f"{name} holds {t.numel()} elements, {numel} needed")
+    return t.data_ptr()
+
+
+def _here(t: torch.Tensor) -> int:
+    """The current stream, of the device that t lives on."""
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def latent4_cache(pages: int, page_size: int, device, layers: int | None = None) -> torch.Tensor:
+    """An empty 4-bit latent cache: uint8 [pages, page_size / 16 * 6400] (one per layer with
+    `layers`).  Slots that were never written may hold anything: no value of the format is an
+    infinity or NaN but the roped dims can be, and attention never reads past a row's length."""
+    if page_size <= 0 or page_size % L4_BLOCK_TOKENS:
+        raise ValueError(f"page_size {page_size} (a positive multiple of {L4_BLOCK_TOKENS})")
+    shape = (pages, page_size // L4_BLOCK_TOKENS * L4_BLOCK_BYTES)
+    return torch.zeros(shape if layers is None else (layers, *shape), device=device, dtype=torch.uint8)
+
+
+def _l4_blocks(cache: torch.Tensor) -> tuple[int, int]:
+    """(address, 16-token blocks) of a 4-bit latent cache."""
+    ptr = _need(cache, "cache", torch.uint8)
+    n, rem = divmod(cache.numel(), L4_BLOCK_BYTES)
+    if rem or not n:
+        raise ValueError(f"the 4-bit cache must hold whole blocks of {L4_BLOCK_BYTES} bytes")
+    return ptr, n
+
+
+def page_plan_buffers(requests: int, token_capacity: int, device) -> dict:
+    """Outputs and the work counter of page_plan."""
+    def i32(n):
+        return torch.zeros(n, device=device, dtype=torch.int32)
+
+    def i64(n):
+        return torch.zeros(n, device=device, dtype=torch.int64)
+    return {"ring_out": i64(2), "token_row": i32(token_capacity), "positions": i64(token_capacity),
+            "slots": i64(token_capacity), "cu_new": i32(requests + 1), "lens": i32(requests), "counts": i32(4),
+            "sync": i32(1)}
+
+
+def page_plan(*, cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free_ring: torch.Tensor,
+              ring_in: torch.Tensor, page_size: int, ring_out: torch.Tensor, token_row: torch.Tensor,
+              positions: torch.Tensor, slots: torch.Tensor, cu_new: torch.Tensor, lens: torch.Tensor,
+              counts: torch.Tensor, sync: torch.Tensor) -> None:
+    """Page tables, slots and positions of a serving step from the requests' lengths
+    (dsv2_page_plan_args in include/dsv2.h): cached int32 / int64 [R], new int32 [R] (tokens to
+    append, -1 = finished), block_table int32 [R, width] and free_ring int32 [F] updated in
+    place, ring_in / ring_out int64 [2] (may be one tensor).  The token outputs have one row per
+    unit of capacity; see page_plan_buffers."""
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise NotImplementedError("block_table must be int32 [requests, width] with contiguous rows")
+    _cuda(block_table, "block_table")
+    R, width = block_table.shape
+    if cached.dtype not in (torch.int32, torch.int64):
+        raise ValueError("cached must be int32 or int64")
+    if cached.numel() != R or new.numel() != R:
+        raise ValueError(f"block_table has {R} rows, cached {cached.numel()} and new {new.numel()} entries")
+    cap = token_row.numel()
+    a = PagePlanArgs(
+        _need(cached, "cached", cached.dtype), _need(new, "new", torch.int32), block_table.data_ptr(),
+        _need(free_ring, "free_ring", torch.int32), _need(ring_in, "ring_in", torch.int64, 2),
+        _need(ring_out, "ring_out", torch.int64, 2), _need(token_row, "token_row", torch.int32),
+        _need(positions, "positions", torch.int64, cap), _need(slots, "slots", torch.int64, cap),
+        _need(cu_new, "cu_new", torch.int32, R + 1), _need(lens, "lens", torch.int32, R),
+        _need(counts, "counts", torch.int32, 4), _need(sync, "sync", torch.int32, 1),
+        block_table.stride(0) if R > 1 else max(width, 1), free_ring.numel(), R, width, page_size, cap,
+        cached.dtype == torch.int64)
+    _lib.call("dsv2_page_plan", ctypes.byref(a), _here(block_table))
+
+
+def _l4_rows(rows: torch.Tensor, slots: torch.Tensor, name: str) -> int:
+    _cuda(rows, name)
+    if rows.dim() != 2 or rows.shape[1] != 576 or rows.dtype != torch.bfloat16 or rows.stride(1) != 1:
+        raise NotImplementedError(f"{name} must be bf16 [n, 576] with a contiguous last dimension")
+    if slots.numel() != rows.shape[0]:
+        raise ValueError(f"{name} has {rows.shape[0]} rows, slots {slots.numel()} entries")
+    return rows.stride(0) if rows.shape[0] > 1 else 576
+
+
+def latent4_write(*, rows: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor) -> None:
+    """Quantise bf16 latent rows [n, 576] into their slots (int64 [n], negative = skipped) of a
+    4-bit latent cache."""
+    rs = _l4_rows(rows, slots, "rows")
+    ptr, blocks = _l4_blocks(cache)
+    _lib.call("dsv2_latent4_write", rows.data_ptr(), rs, _need(slots, "slots", torch.int64), rows.shape[0], ptr, blocks,
+              _here(rows))
+
+
+def latent4_read(*, cache: torch.Tensor, slots: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """The values that the slots hold (zeros for a negative slot) as bf16 rows [n, 576]."""
+    rs = _l4_rows(out, slots, "out")
+    ptr, blocks = _l4_blocks(cache)
+    _lib.call("dsv2_latent4_read", ptr, blocks, _need(slots, "slots", torch.int64), out.shape[0], out.data_ptr(), rs,
+              _here(out))
+    return out
+
+
+def mla_prep_q4(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos: torch.Tensor, sin: torch.Tensor,
+                positions: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor, q_pe_out: torch.Tensor,
+                q_nope_out: torch.Tensor | None = None) -> None:
+    """mla_prep into slots (int64 [B], negative = no cache write) of a 4-bit latent cache; a
+    negative position marks a padding row."""
+    a = _mla_prep_args(qkva, kv_norm_w, eps, cos, sin, positions, q_pe_out, q_nope_out)
+    ptr, blocks = _l4_blocks(cache)
+    _lib.call("dsv2_mla_prep_q4", ctypes.byref(a), ptr, blocks, _need(slots, "slots", torch.int64, a.batch), _here(cache))
+
+
+def mla_q4_workspace(rows: int, device) -> dict:
+    """Work buffers of mla_decode_q4 for up to `rows` query rows."""
+    return {}
+
+
+def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
+                  positions: torch.Tensor, page_size: int, softmax_scale: float, o_lat: torch.Tensor,
+                  seq_rows: torch.Tensor | None = None) -> torch.Tensor:
+    """Latent attention over the paged 4-bit cache (dsv2_mla_decode_q4_args in include/dsv2.h):
+    query row r attends positions 0 .. positions[r] of block-table row seq_rows[r] (default r);
+    position -1 or a negative seq_rows entry gives a row of zeros."""
+    rows = q_abs.shape[0]
+    if tuple(q_abs.shape) != (rows, 16, 512) or tuple(q_pe.shape) != (rows, 16, 64) or o_lat.shape != q_abs.shape:
+        raise ValueError("q_abs and o_lat must be [rows, 16, 512] and q_pe [rows, 16, 64]")
+    for name, t in (("q_abs", q_abs), ("q_pe", q_pe), ("o_lat", o_lat)):
+        if t.dtype != torch.bfloat16:
+            raise NotImplementedError(f"mla_decode_q4 supports bf16 only ({name} is {t.dtype})")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise NotImplementedError("block_table must be int32 [sequences, width] with contiguous rows")
+    _cuda(block_table, "block_table")
+    ptr, blocks = _l4_blocks(cache)
+    seqs, width = block_table.shape
+    a = MlaDecodeQ4Args(
+        _need(q_abs, "q_abs", torch.bfloat16), _need(q_pe, "q_pe", torch.bfloat16), ptr, blocks,
+        block_table.data_ptr(), block_table.stride(0) if seqs > 1 else max(width, 1), width, seqs, page_size, rows,
+        _need(positions, "positions", torch.int64, rows),
+        None if seq_rows is None else _need(seq_rows, "seq_rows", torch.int32, rows), softmax_scale,
+        _need(o_lat, "o_lat", torch.bfloat16))
+    _lib.call("dsv2_mla_decode_q4", ctypes.byref(a), _here(q_abs))
+    return o_lat
+
+
+def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, ranks: torch.Tensor,
+         scales: torch.Tensor, y: torch.Tensor, low: torch.Tensor, base: torch.Tensor | None = None,
+         token_row: torch.Tensor | None = None) -> torch.Tensor:
+    """y[t] = sum of base[:, t] + scales[i] * b[i] (a[i] x[t]) with i = ids[token_row[t]] (or
+    ids[t]); negative = no adapter.  x bf16 [T, K], a bf16 [adapters, rank, K], b bf16
+    [adapters, N, rank], ids int32, ranks int32 and scales fp32 [adapters], y bf16 or fp32
+    [T, N], low fp32 work buffer of T * rank elements, base (optional) fp32 [parts, T, N]."""
+    _cuda(x, "x")
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1:
+        raise NotImplementedError("x must be bf16 [tokens, k] with a contiguous last dimension")
+    T, K = x.shape
+    if a.dim() != 3 or b.dim() != 3 or a.shape[2] != K or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[1]:
+        raise ValueError(f"a must be [adapters, rank, {K}] and b [adapters, n, rank]")
+    n_ad, rank, N = a.shape[0], a.shape[1], b.shape[1]
+    if tuple(y.shape) != (T, N) or y.stride(1) != 1 or not y.is_cuda:
+        raise ValueError(f"y must be a CUDA tensor [{T}, {N}] with a contiguous last dimension")
+    if y.dtype not in (torch.bfloat16, torch.float32):
+        raise NotImplementedError(f"lora output dtype {y.dtype}")
+    args = LoraArgs(
+        x.data_ptr(), x.stride(0) if T > 1 else K, _need(a, "a", torch.bfloat16), _need(b, "b", torch.bfloat16),
+        _need(ids, "ids", torch.int32), None if token_row is None else _need(token_row, "token_row", torch.int32, T),
+        _need(ranks, "ranks", torch.int32, n_ad), _need(scales, "scales", torch.float32, n_ad), None, 0, 0,
+        _need(low, "low", torch.float32, T * rank), y.data_ptr(), y.stride(0) if T > 1 else N,
+        DSV2_F32 if y.dtype == torch.float32 else DSV2_BF16, 0, ids.numel(), n_ad, rank, T, K, N)
+    if base is not None:
+        if base.dim() != 3 or base.dtype != torch.float32 or base.shape[1:] != y.shape or base.stride(2) != 1:
+            raise ValueError(f"base must be fp32 [parts, {T}, {N}] with a contiguous last dimension")
+        _cuda(base, "base")
+        args.base, args.base_part_stride, args.base_row_stride = base.data_ptr(), base.stride(0), base.stride(1)
+        args.n_base = base.shape[0]
+    _lib.call("dsv2_lora", ctypes.byref(args), _here(x))
+    return y
+
+
+def lora_workspace(tokens: int, n: int, k: int, rank: int, device) -> dict:
+    """Work buffers of lora_linear: the shared projection's fp32 partials and the low-rank rows."""
+    sms = torch.cuda.get_device_properties(device).multi_processor_count
+    splits = 1
+    if LORA_GEMV_TOKENS < tokens <= 256:   # decode batches: K split over the SMs, as the engine's projections
+        splits = max(1, min(sms // ((n + 127) // 128), k // 64, 5))
+    return {"parts": torch.empty((splits, tokens, n), device=device, dtype=torch.float32),
+            "low": torch.empty((tokens, rank), device=device, dtype=torch.float32)}
+
+
+LORA_GEMV_TOKENS = 8   # up to here lora_linear's shared projection runs the small (GEMV) family
+
+
+def lora_linear(*, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
+                ranks: torch.Tensor, scales: torch.Tensor, y: torch.Tensor, parts: torch.Tensor, low: torch.Tensor,
+                token_row: torch.Tensor | None = None) -> torch.Tensor:
+    """The shared projection x @ w.T (w bf16 [N, K]) plus every token's low-rank adapter, rounded
+    once to y's dtype: y[t] = w x[t] + scales[i] * b[i] (a[i] x[t]); see lora and
+    lora_workspace."""
+    if w.dim() != 2 or w.dtype != torch.bfloat16 or w.stride(1) != 1 or not w.is_cuda or x.dtype != torch.bfloat16:
+        raise NotImplementedError("lora_linear supports bf16 x [T, K] and CUDA w [N, K] with contiguous rows")
+    T = x.shape[0]
+    if x.dim() != 2 or w.shape[1] != x.shape[1] or tuple(parts.shape[1:]) != (T, w.shape[0]) or b.shape[1] != w.shape[0]:
+        raise ValueError("lora_linear: inconsistent shapes of x, w, b and parts")
+    _need(parts, "parts", torch.float32)
+    if T == 0:
+        return y
+    if T <= LORA_GEMV_TOKENS:
+        linear(w=w, n_rows=w.shape[0], k=w.shape[1], x=x, y=parts[0], family=FAMILY_SMALL, epilogue=EPI_STORE_F32,
+               n_tokens=T, x_group_rows=T)
+        parts = parts[:1]
+    else:
+        linear(w=w, n_rows=w.shape[0], k=w.shape[1], x=x, y=parts[0], family=FAMILY_BATCH, epilogue=EPI_STORE_F32,
+               n_tokens=T, x_group_rows=T, k_splits=parts.shape[0], y_split_stride=parts.stride(0))
+    return lora(x=x, a=a, b=b, ids=ids, ranks=ranks, scales=scales, y=y, low=low, base=parts, token_row=token_row)

@@ -80,6 +80,7 @@ DSV2_API int64_t dsv2_kernel_launches(void);
 #define DSV2_DEVERR_TIMEOUT 1 /* a bounded wait (mbarrier, progress counter, peer) gave up */
 #define DSV2_DEVERR_INDEX 2   /* token id >= vocab, position >= max_len, cache row, tile bound */
 #define DSV2_DEVERR_TMEM 3    /* tensor-memory allocation failed */
+#define DSV2_DEVERR_NONFINITE 4 /* an infinity or NaN was written to the 4-bit latent cache */
 
 /* Reads (and optionally clears) the device error word of the current device.
  * Synchronous (cudaMemcpyFromSymbol); call outside the hot loop.  Clearing a nonzero
@@ -553,6 +554,147 @@ DSV2_API int dsv2_mla_decode_noalloc(const void* q_abs, const void* q_pe, const 
                                      int64_t cache_b_stride, int max_len, const int64_t* positions,
                                      int pos_numel, float softmax_scale, int split_len, void* o_lat,
                                      int batch, void* stream);
+
+/* ---- serving from a paged 4-bit latent cache ------------------------------------ */
+/* The 4-bit latent cache is an array of 16-token blocks of 6400 bytes (400 bytes a token
+ * against 1152): 512 latent dims as 4-bit integers with one 8-bit scale per 32 dims, and the
+ * 64 roped key dims in bf16.  Slot s is token s % 16 of block s / 16; a page of page_size
+ * tokens (a multiple of 16) is page_size / 16 consecutive blocks, so page g holds slots
+ * [g * page_size, (g + 1) * page_size).  An element is v * scale with v in -8 .. 7 and
+ * scale = max |x| of its 32 / 7 rounded to 3 mantissa bits (0, 2^-17 .. 60: larger groups
+ * saturate).  An infinity saturates and a NaN becomes 0; both set DSV2_DEVERR_NONFINITE.
+ * Byte layout of a block:
+ *   [0, 4096)     token p at 256 p, 16 bytes per group of 32 dims; group c at place
+ *                 c ^ (2 (p & 1) + 4 ((p >> 1 ^ p >> 2) & 1)); of its 32-bit word w, dim
+ *                 8 w + 2 i is nibble i and dim 8 w + 2 i + 1 nibble 4 + i, stored as v + 8
+ *   [4096, 4352)  scale of group c of token p at 4096 + 16 c + 4 (p & 3) + (p >> 2): bits
+ *                 14 .. 7 of the scale as an fp16 number
+ *   [4352, 6400)  roped dims of token p at 4352 + 128 p, 8 chunks of 8 dims, chunk j at j ^ (p & 4)
+ * No reference counterpart (its cache is the expanded bf16 one); block addresses are 16-byte
+ * aligned. */
+#define DSV2_L4_BLOCK_TOKENS 16
+#define DSV2_L4_BLOCK_BYTES 6400
+
+/* Page tables, slots and positions of a step, from the requests' lengths, in one launch.
+ * Request r holds cached[r] tokens in the pages block_table[r, 0 .. ceil(cached / page_size))
+ * and appends fresh[r] >= 0 tokens; fresh[r] = -1: it is finished.  Free pages sit in a ring:
+ * ring_in = {pages ever taken, pages ever put}, the free ones are free_ring[i % ring_size] for
+ * ring_in[0] <= i < ring_in[1].
+ *   - requests are served in order: r is served when the new pages of all requests up to and
+ *     including r are free and its tokens fit token_capacity; its new pages are appended to
+ *     its table row and lens[r] = cached + fresh.  A request that is not served takes nothing:
+ *     lens[r] = cached[r], its token rows have slot and position -1, counts[3] counts it;
+ *   - a finished request's pages are put into the ring, in order of its table row; lens[r] = 0
+ *     (its table row keeps its entries);
+ *   - token rows: requests laid end to end, cu_new[r] = first row of request r.  token_row =
+ *     request, positions = index in the request, slots = where its cache row goes (page *
+ *     page_size + position % page_size).  Rows past the last token hold -1 in all three, so
+ *     launches of a fixed token_capacity can follow (captured graphs);
+ *   - ring_out = the ring's counters after the step (may be ring_in); counts = {tokens asked
+ *     for, pages taken, pages put, requests not served}.
+ * lens must not overlap cached.  sync: one int32, zero before the first call and left zero;
+ * calls that share it must not overlap on the GPU.  A negative or too long request (more than
+ * width pages) is not served and sets DSV2_DEVERR_INDEX, as does a ring whose counters are
+ * impossible. */
+typedef struct dsv2_page_plan_args {
+  const void* cached;        /* [requests] int32, or int64 when cached_is64 */
+  const int32_t* fresh;      /* [requests] */
+  int32_t* block_table;      /* [requests, width] rows at table_stride, updated in place */
+  int32_t* free_ring;        /* [ring_size], updated in place */
+  const int64_t* ring_in;    /* [2] */
+  int64_t* ring_out;         /* [2] */
+  int32_t* token_row;        /* [token_capacity] */
+  int64_t* positions;        /* [token_capacity] */
+  int64_t* slots;            /* [token_capacity] */
+  int32_t* cu_new;           /* [requests + 1] */
+  int32_t* lens;             /* [requests] */
+  int32_t* counts;           /* [4] */
+  int32_t* sync;             /* [1] */
+  int64_t table_stride;
+  int64_t ring_size;
+  int32_t requests;
+  int32_t width;
+  int32_t page_size;
+  int32_t token_capacity;
+  int32_t cached_is64;
+} dsv2_page_plan_args;
+
+DSV2_API int dsv2_page_plan(const dsv2_page_plan_args* args, void* stream);
+
+/* Quantise bf16 latent rows [n, 576] (row stride in elements, 16-byte aligned rows) into their
+ * slots; a negative slot is skipped, one past the cache's n_blocks sets DSV2_DEVERR_INDEX and
+ * is skipped.  Two rows of one call must not name the same slot. */
+DSV2_API int dsv2_latent4_write(const void* rows, int64_t row_stride, const int64_t* slots, int64_t n,
+                                void* cache, int64_t n_blocks, void* stream);
+/* The values that the slots hold, as bf16 rows (exact); zeros for a negative slot. */
+DSV2_API int dsv2_latent4_read(const void* cache, int64_t n_blocks, const int64_t* slots, int64_t n,
+                               void* out, int64_t out_row_stride, void* stream);
+
+/* dsv2_mla_prep into the 4-bit cache: the row that dsv2_mla_prep would write (bf16) is
+ * quantised into slots[b]; positions[b] is the rope position.  A negative slot skips the cache
+ * write, a negative position the row's rope as well (padding).  Of args, cache, cache_b_stride,
+ * max_len, cache_rows and cache_batch are not used. */
+DSV2_API int dsv2_mla_prep_q4(const dsv2_mla_prep_args* args, void* cache4, int64_t n_blocks,
+                              const int64_t* slots, void* stream);
+
+/* dsv2_mla_decode over the paged 4-bit cache: query row r attends positions 0 .. positions[r]
+ * of table row seq_rows[r] (NULL: row r).  positions[r] = -1 or seq_rows[r] < 0: nothing to
+ * attend, o_lat[r] = 0.  Several rows may name one sequence (draft tokens, prompt chunks).  A
+ * length beyond the table's width, a table row >= seqs or a page outside the cache sets
+ * DSV2_DEVERR_INDEX. */
+typedef struct dsv2_mla_decode_q4_args {
+  const void* q_abs;           /* [rows, 16, 512] bf16 */
+  const void* q_pe;            /* [rows, 16, 64] bf16 */
+  const void* cache;
+  int64_t n_blocks;            /* 16-token blocks of the cache */
+  const int32_t* block_table;  /* [seqs, width] rows at table_stride */
+  int64_t table_stride;
+  int32_t width;
+  int32_t seqs;
+  int32_t page_size;           /* a multiple of 16 */
+  int32_t rows;
+  const int64_t* positions;    /* [rows] */
+  const int32_t* seq_rows;     /* optional [rows] */
+  float softmax_scale;
+  void* o_lat;                 /* [rows, 16, 512] bf16 */
+} dsv2_mla_decode_q4_args;
+
+DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   y[t, :] = sum_i base[i, t, :] + scales[a] * B_a (A_a x[t]),   a = ids[token_row ? token_row[t] : t]
+ * a: [adapters, rank, k], b: [adapters, n, rank] bf16 contiguous; of adapter a the first
+ * ranks[a] of its `rank` rows are used (the rest are not read into the result).  A negative id
+ * or token row: no adapter.  base: n_base fp32 partials of the shared projection (dsv2_linear
+ * with DSV2_EPI_STORE_F32), 0 = none.  y: y_dtype DSV2_BF16 (one rounding of the fp32 sum) or
+ * DSV2_F32 (with n_base = 0 the adapters' part alone, e.g. one more partial of the projection).
+ * low: fp32 work buffer [tokens, rank].  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128. */
+typedef struct dsv2_lora_args {
+  const void* x;
+  int64_t x_row_stride;
+  const void* a;
+  const void* b;
+  const int32_t* ids;
+  const int32_t* token_row;
+  const int32_t* ranks;
+  const float* scales;
+  const float* base;
+  int64_t base_part_stride;
+  int64_t base_row_stride;
+  float* low;
+  void* y;
+  int64_t y_row_stride;
+  int32_t y_dtype;
+  int32_t n_base;
+  int32_t ids_len;             /* entries of ids */
+  int32_t adapters;
+  int32_t rank;
+  int32_t tokens;
+  int32_t k;
+  int32_t n;
+} dsv2_lora_args;
+
+DSV2_API int dsv2_lora(const dsv2_lora_args* args, void* stream);
 
 #ifdef __cplusplus
 }
