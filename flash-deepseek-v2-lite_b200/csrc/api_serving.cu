@@ -4,6 +4,8 @@
 
 namespace {
 
+constexpr int kQ4MinUnits = 4;   // 64 positions: shorter pieces cost more in merges than they save
+
 // rows of a latent4 call: [n, 576] bf16 with 16-byte aligned rows
 int latent4_args(const char* what, const void* rows, int64_t row_stride, const int64_t* slots, int64_t n,
                  const void* cache, int64_t n_blocks) {
@@ -101,17 +103,21 @@ int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* a, void* stream) {
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: rows %d seqs %d width %d blocks %lld", a->rows, a->seqs, a->width,
                 (long long)a->n_blocks);
   if (a->rows == 0) return DSV2_OK;
-  if (!a->q_abs || !a->q_pe || !a->cache || !a->block_table || !a->positions || !a->o_lat)
+  if (!a->q_abs || !a->q_pe || !a->cache || !a->block_table || !a->positions || !a->o_lat || !a->o_part ||
+      !a->ml_part || !a->row_sync)
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: null pointer");
+  if (a->part_slots < 2) return fail(DSV2_ERR_INVALID, "mla_decode_q4: %d partial slots (at least 2)", a->part_slots);
   if (a->page_size <= 0 || a->page_size % DSV2_L4_BLOCK_TOKENS)
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: page_size %d (a positive multiple of %d)", a->page_size,
                 DSV2_L4_BLOCK_TOKENS);
   if (static_cast<int64_t>(a->width) * a->page_size > 0x7fffffffLL)
     return fail(DSV2_ERR_UNSUPPORTED, "mla_decode_q4: a table row of %d pages of %d tokens exceeds 2^31 tokens",
                 a->width, a->page_size);
-  if (!aligned16(a->q_abs) || !aligned16(a->q_pe) || !aligned16(a->cache) || !aligned16(a->o_lat))
+  if (!aligned16(a->q_abs) || !aligned16(a->q_pe) || !aligned16(a->cache) || !aligned16(a->o_lat) ||
+      !aligned16(a->o_part))
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: operands must be 16-byte aligned");
-  if (int rc = ensure_init(nullptr)) return rc;
+  int sms = 0;
+  if (int rc = ensure_init(&sms)) return rc;
   MlaQ4Params p = {};
   p.q_abs = static_cast<const bf16*>(a->q_abs);
   p.q_pe = static_cast<const bf16*>(a->q_pe);
@@ -127,9 +133,14 @@ int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* a, void* stream) {
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.o_lat = static_cast<bf16*>(a->o_lat);
   p.rows = a->rows;
+  p.min_units = kQ4MinUnits;
+  p.o_part = a->o_part;
+  p.ml_part = a->ml_part;
+  p.part_slots = a->part_slots;
+  p.row_sync = a->row_sync;
   if (!a->seq_rows && a->seqs < a->rows)
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: %d query rows, %d table rows (pass seq_rows)", a->rows, a->seqs);
-  return check_launch(launch_mla_q4(p, static_cast<cudaStream_t>(stream)), "mla_decode_q4");
+  return check_launch(launch_mla_q4(p, sms, static_cast<cudaStream_t>(stream)), "mla_decode_q4");
 }
 
 int dsv2_lora(const dsv2_lora_args* a, void* stream) {

@@ -12,8 +12,8 @@
 // Scale: max |x| of the group / 7, rounded to nearest even at 3 mantissa bits; the code is bits
 // 14..7 of the scale as a positive fp16 number (5 exponent bits, 3 mantissa bits), so decoding
 // is one shift.  v = round(x / scale).  A scale has 4 significant bits and v four, so every
-// value has at most 8: exact in bf16 and in fp16, and no decoded byte is an infinity or NaN
-// (code <= 167 is scale <= 60; groups beyond 60 * 7 saturate).
+// value has at most 8: exact in bf16 and in fp16.  Codes end at 167, scale 60 (groups beyond
+// 60 * 7 saturate); bytes of slots that were never written may decode to an infinity or NaN.
 //
 // The places are the shared-memory layout of the attention kernel (mla_q4.cu): a block is
 // copied as it lies, and the fragment loads of both products hit all 32 banks once.

@@ -2,74 +2,742 @@
 //   score[h, s] = scale * (q_abs[h] . latent[s] + q_pe[h] . rope[s]),  s = 0 .. position
 //   o_lat[h]    = sum_s softmax(score)[h, s] * latent[s]
 // for the 16 heads of every query row; the tokens of a row come from the pages of its
-// block-table row.  One CTA per query row, one warp per head, one 16-token block at a time.
+// block-table row.
 #include "latent4.cuh"
 #include "params.cuh"
 
 namespace dsv2 {
 
-__global__ __launch_bounds__(512) void mla_q4_simple_kernel(const MlaQ4Params p) {
-  pdl_enter();
-  __shared__ bf16 s_tok[kL4Tokens][578];   // every value is exact in bf16
-  __shared__ bf16 s_q[kHeads][578];
-  const int tid = threadIdx.x, lane = tid & 31, h = tid >> 5;
-  const int row = blockIdx.x;
-  const long long pos = p.positions[row];
-  const int seq = p.seq_rows ? p.seq_rows[row] : row;
-  long long len = (seq < 0 || pos < 0) ? 0 : pos + 1;
-  if (len > 0 && (seq >= p.seqs || len > static_cast<long long>(p.width) * p.page_blocks * kL4Tokens)) {
-    if (tid == 0) set_device_error(kErrIndex);
-    len = 0;
-  }
-  for (int i = tid; i < kHeads * 512; i += 512) s_q[i >> 9][i & 511] = p.q_abs[static_cast<long long>(row) * kHeads * 512 + i];
-  for (int i = tid; i < kHeads * 64; i += 512) s_q[i >> 6][512 + (i & 63)] = p.q_pe[static_cast<long long>(row) * kHeads * 64 + i];
-  float m = -INFINITY, l = 0.f, o[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = 0.f;
-  for (long long b = 0; b * kL4Tokens < len; ++b) {
-    long long blk = p.table[seq * p.table_stride + b / p.page_blocks] * static_cast<long long>(p.page_blocks) + b % p.page_blocks;
-    if (blk < 0 || blk >= p.n_blocks) {
-      if (tid == 0) set_device_error(kErrIndex);
-      blk = 0;
-    }
-    const unsigned char* src = p.cache + blk * kL4BlockBytes;
-    __syncthreads();
-    for (int i = tid; i < kL4Tokens * 64; i += 512) {
-      const int t = i >> 6, w = i & 63;
-      float x[8];
-      l4_unpack(*reinterpret_cast<const uint32_t*>(src + l4_word_off(t, w >> 2, w & 3)),
-                l4_scale(src[kL4ScaleOff + 16 * (w >> 2) + l4_scale_place(t)]), x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s_tok[t][8 * w + j] = __float2bfloat16_rn(x[j]);
-    }
-    {
-      const int t = tid >> 5, r = lane;
-      const uint32_t u = *reinterpret_cast<const uint32_t*>(src + l4_rope_off(t, r));
-      *reinterpret_cast<uint32_t*>(&s_tok[t][512 + 2 * r]) = u;
-    }
-    __syncthreads();
-    const int n = static_cast<int>(min(static_cast<long long>(kL4Tokens), len - b * kL4Tokens));
-    for (int t = 0; t < n; ++t) {
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < 18; ++j) s = fmaf(__bfloat162float(s_q[h][lane + 32 * j]), __bfloat162float(s_tok[t][lane + 32 * j]), s);
-      s = warp_sum(s) * p.scale_log2;
-      const float mn = fmaxf(m, s), u = mn == -INFINITY ? 0.f : mn;
-      const float a = exp2f(m - u), e = exp2f(s - u);
-      l = l * a + e;
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = o[i] * a + e * __bfloat162float(s_tok[t][lane + 32 * i]);
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  bf16* out = p.o_lat + (static_cast<long long>(row) * kHeads + h) * 512;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) out[lane + 32 * i] = __float2bfloat16_rn(o[i] * inv);
+constexpr int kQ4Pos = 64;                                   // positions of a tile: 4 blocks
+constexpr int kQ4TileBlocks = kQ4Pos / kL4Tokens;
+constexpr int kQ4Stages = 7;
+constexpr int kQ4StageBytes = kQ4TileBlocks * kL4BlockBytes; // 25600
+constexpr int kQ4SegUnits = 4;                               // per-row cost in blocks (work balance)
+constexpr int kQ4ScoreWarps = 8;                             // 4 blocks x 2 halves of the dims
+constexpr int kQ4PvWarps = 4;                                // 128 latent dims each
+constexpr int kQ4Compute = (kQ4ScoreWarps + kQ4PvWarps) * 32;
+constexpr int kQ4ProducerWarp = kQ4ScoreWarps + kQ4PvWarps;  // warp 12: copies, then tickets
+constexpr int kQ4Threads = kQ4Compute + 32;
+constexpr int kQ4QRow = 1024 + 16;                           // padded shared rows of q_abs / q_pe
+constexpr int kQ4PeRow = 128 + 16;
+constexpr int kQ4QBytes = kHeads * (kQ4QRow + kQ4PeRow);
+constexpr int kQ4PRow = kQ4Pos + 8;                          // row of P
+constexpr float kQ4Slack = 8.f;                              // log2 growth of a row's maximum left unscaled
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void q4_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+// barrier 1 over the score warps that also says whether any thread's predicate holds
+__device__ __forceinline__ bool q4_bar_any(bool pred) {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(r)
+               : "r"(static_cast<uint32_t>(pred)), "n"(kQ4ScoreWarps * 32)
+               : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t h2fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t h2mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t b2fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t b2mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
-cudaError_t launch_mla_q4(const MlaQ4Params& p, cudaStream_t st) {
-  launch_kernel(mla_q4_simple_kernel, p.rows, 512, 0, st, p);
+// Nibble pairs to the fp16 pairs of the score product (queries scaled into fp16's range).  A
+// nibble q at bits 3..0 of a half, under the bits of 1024, is the fp16 number 1024 + q; one at
+// bits 7..4, under the bits of 64, is 64 + q: one shift serves four nibbles.  (1024 + q) s - 1032 s
+// = (q - 8) s in one fma, exactly: s has 4 significant bits and is at most 60, so 1032 s (12 bits,
+// the last 0) and the result (8 bits) are fp16 numbers and the fma rounds once.
+struct Q4Scale {
+  uint32_t s, b0, b4;   // scale pair, -1032 s, -72 s
+};
+__device__ __forceinline__ Q4Scale q4_scale(uint32_t codes /* code of each half in its low byte */) {
+  Q4Scale r;
+  r.s = codes << 7;
+  r.b0 = h2mul(r.s, 0xe408e408u);   // -1032
+  r.b4 = h2mul(r.s, 0xd480d480u);   // -72
+  return r;
+}
+__device__ __forceinline__ uint32_t q4_lo(uint32_t w, const Q4Scale& c) { return h2fma((w & 0x000f000fu) | 0x64006400u, c.s, c.b0); }
+__device__ __forceinline__ uint32_t q4_hi(uint32_t w, const Q4Scale& c) { return h2fma((w & 0x00f000f0u) | 0x54005400u, c.s, c.b4); }
+
+// Nibble pairs to the bf16 pairs of the P V product: P spans more binades than fp16 has (a
+// probability far below the row's largest still decides a dim in which that token is 0).  bf16
+// holds 128 + q for a nibble at bits 3..0 only.  A code in bits 11..4 of a bf16 number is the
+// scale times 2^-112 (subnormals included), so the scale and -136 times it are one product each.
+struct Q4ScaleB {
+  uint32_t s, b;        // scale pair, -136 s
+};
+__device__ __forceinline__ Q4ScaleB q4_scale_b(uint32_t codes) {
+  Q4ScaleB r;
+  r.s = b2mul(codes << 4, 0x77807780u);   // 2^112
+  r.b = b2mul(codes << 4, 0xfb08fb08u);   // -136 * 2^112
+  return r;
+}
+__device__ __forceinline__ uint32_t q4_b(uint32_t w, const Q4ScaleB& c) { return b2fma((w & 0x000f000fu) | 0x43004300u, c.s, c.b); }
+
+// Attended length of query row r: 0 .. the positions its table row can hold.
+__device__ __forceinline__ int q4_len(const MlaQ4Params& p, int r) {
+  const long long pos = p.positions[r];
+  const int seq = p.seq_rows ? p.seq_rows[r] : r;
+  if (pos < 0 || seq < 0) return 0;
+  if (seq >= p.seqs || pos >= static_cast<long long>(p.width) * p.page_blocks * kL4Tokens) {
+    set_device_error(kErrIndex);
+    return 0;
+  }
+  return static_cast<int>(pos + 1);
+}
+// blocks of a row (a row with nothing to attend owns one, fully masked) and its units of work
+__device__ __forceinline__ int q4_blocks(int len) { return len > 0 ? (len + kL4Tokens - 1) / kL4Tokens : 1; }
+__device__ __forceinline__ int q4_units(int len) { return q4_blocks(len) + kQ4SegUnits; }
+
+struct Q4Smem {
+  unsigned char ring[kQ4Stages][kQ4StageBytes];
+  unsigned char q[2][kQ4QBytes];            // [16][1040] q_abs, [16][144] q_pe
+  bf16 p[2][kHeads][kQ4PRow];               // P, columns in the order the fragments want
+  float4 part[kQ4TileBlocks][2][32];        // scores of one half of the dims for the other half's warp
+  float smax[kHeads][kQ4ScoreWarps];
+  float alpha[2][kHeads];
+  float lsum[kQ4ScoreWarps][kHeads];
+  float fin[2][kHeads];
+  uint64_t full[kQ4Stages], empty[kQ4Stages];
+  uint64_t p_full[2], p_empty[2], q_full[2], q_empty[2], fin_full[2], fin_empty[2], tk_full[2], tk_done;
+  long long ll[4];                          // first row's stream position, two pending rows'
+  int wsum[32];
+  int rescale[2];
+  int first_row, abort, n_pend, pend_row[2], pend_blocks[2];
+};
+static_assert(sizeof(Q4Smem) <= 232448, "4-bit latent attention: shared memory exceeds 227 KB");
+
+// One launch, persistent: the rows form one stream of units (kQ4SegUnits of per-row cost, then
+// the row's 16-token blocks), cut into equal ranges, one CTA (13 warps) per SM.  A row inside
+// one range writes o_lat; a row cut by a boundary leaves (o, m, l) partials that the last of
+// its CTAs merges (row tickets).
+//  - warps 0-7, scores: warp w takes block w % 4 of a tile (16 positions) and half w / 4 of the
+//    dims (256 latent, 32 roped), its query slice in registers as fp16 scaled by a power of two
+//    per head; the halves exchange 8 positions each;
+//  - warps 8-11, P V: 128 latent dims each;
+//  - warp 12: copies blocks (looked up 32 at a time) and query rows, then publishes tickets.
+// The maximum that P is taken against is kept until a score exceeds it by 2^kQ4Slack: the score
+// warps then agree on a new one and the P V warps rescale.
+__global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  Q4Smem& sm = *reinterpret_cast<Q4Smem*>(smem_raw);
+  volatile int* s_abort = &sm.abort;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int R = p.rows;
+  if (tid == 0) {
+    for (int i = 0; i < kQ4Stages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], kQ4ScoreWarps + kQ4PvWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.p_full[i], kQ4ScoreWarps);
+      mbar_init(&sm.p_empty[i], kQ4PvWarps);
+      mbar_init(&sm.q_full[i], 1);
+      mbar_init(&sm.q_empty[i], kQ4ScoreWarps);
+      mbar_init(&sm.fin_full[i], 1);
+      mbar_init(&sm.fin_empty[i], kQ4PvWarps);
+      mbar_init(&sm.tk_full[i], 1 + kQ4PvWarps);
+    }
+    mbar_init(&sm.tk_done, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  pdl_enter();
+
+  // --- prefix sum of the rows' units; this CTA's range [start, end) and its first row
+  long long T = 0;
+  int mine0 = 0, incl0 = 0;
+  for (int base = 0; base < R; base += kQ4Threads) {
+    const int r = base + tid;
+    const int u = r < R ? q4_units(q4_len(p, r)) : 0;
+    int v = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int w = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += w;
+    }
+    if (lane == 31) sm.wsum[warp] = v;
+    if (base == 0) {
+      mine0 = u;
+      incl0 = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kQ4Threads / 32; ++w) T += sm.wsum[w];
+    if (base + kQ4Threads < R) __syncthreads();
+  }
+  const long long c = blockIdx.x;
+  const long long n_cta = min(static_cast<long long>(gridDim.x), (T + p.min_units - 1) / p.min_units);
+  if (c >= n_cta) return;
+  const long long start = mla_range_start(c, T, n_cta), end = mla_range_start(c + 1, T, n_cta);
+  if (R <= kQ4Threads) {
+    long long off = 0;
+#pragma unroll
+    for (int w = 0; w < kQ4Threads / 32; ++w)
+      if (w < warp) off += sm.wsum[w];
+    const long long S = off + incl0 - mine0;
+    if (tid < R && S <= start && start < S + mine0) {
+      sm.ll[0] = S;
+      sm.first_row = tid;
+    }
+  } else {
+    long long run = 0;
+    for (int base = 0; base < R && run <= start; base += kQ4Threads) {
+      __syncthreads();
+      const int r = base + tid;
+      const int u = r < R ? q4_units(q4_len(p, r)) : 0;
+      int v = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
+      }
+      if (lane == 31) sm.wsum[warp] = v;
+      __syncthreads();
+      long long off = run, total = 0;
+#pragma unroll
+      for (int w = 0; w < kQ4Threads / 32; ++w) {
+        if (w < warp) off += sm.wsum[w];
+        total += sm.wsum[w];
+      }
+      const long long S = off + v - u;
+      if (r < R && S <= start && start < S + u) {
+        sm.ll[0] = S;
+        sm.first_row = r;
+      }
+      run += total;
+    }
+  }
+  __syncthreads();
+  const long long S0 = sm.ll[0];
+  const int r0 = sm.first_row;
+
+  // the row at stream position S: its blocks [j0, j1) in this CTA's range
+  auto segment = [&](long long S, int nblk, int& j0, int& j1) {
+    const long long St = S + kQ4SegUnits;
+    j0 = static_cast<int>(max(0LL, start - St));
+    j1 = static_cast<int>(min(static_cast<long long>(nblk), end - St));
+    return St >= start && St + nblk <= end;   // wholly in the range
+  };
+
+  if (warp == kQ4ProducerWarp) {
+    // ================= producer warp
+    bool ok = true;
+    long long g = 0;
+    int seg = 0;
+    long long S = S0;
+    for (int r = r0; S + kQ4SegUnits < end && r < R; ++r, ++seg) {
+      const int len = q4_len(p, r), nblk = q4_blocks(len);
+      int j0, j1;
+      segment(S, nblk, j0, j1);
+      // query block into buffer seg & 1
+      if (seg >= 2 && ok) ok = mla_wait(&sm.q_empty[seg & 1], static_cast<uint32_t>(((seg >> 1) - 1) & 1), s_abort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        unsigned char* dq = sm.q[seg & 1];
+        uint64_t* bar = &sm.q_full[seg & 1];
+        if (lane == 0) mbar_arrive_expect_tx(bar, kHeads * (1024 + 128));
+        __syncwarp();
+        if (lane < kHeads)
+          bulk_load(smem_u32(dq + lane * kQ4QRow), p.q_abs + (static_cast<long long>(r) * kHeads + lane) * 512, 1024, bar);
+        else
+          bulk_load(smem_u32(dq + kHeads * kQ4QRow + (lane - kHeads) * kQ4PeRow),
+                    p.q_pe + (static_cast<long long>(r) * kHeads + lane - kHeads) * 64, 128, bar);
+      }
+      const int* table = len > 0 ? p.table + (p.seq_rows ? p.seq_rows[r] : r) * p.table_stride : nullptr;
+      for (int jb = j0; jb < j1; jb += 32) {
+        // 32 blocks' addresses, one per lane
+        long long blk = 0;
+        if (table && jb + lane < j1) {
+          const int j = jb + lane;
+          blk = static_cast<long long>(table[j / p.page_blocks]) * p.page_blocks + j % p.page_blocks;
+          if (blk < 0 || blk >= p.n_blocks) {
+            set_device_error(kErrIndex);
+            blk = 0;
+          }
+        }
+        for (int t = 0; t < 32 && jb + t < j1; t += kQ4TileBlocks, ++g) {
+          const int st = static_cast<int>(g % kQ4Stages);
+          if (g >= kQ4Stages && ok) ok = mla_wait(&sm.empty[st], static_cast<uint32_t>(((g / kQ4Stages) - 1) & 1), s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          const int nb = min(kQ4TileBlocks, j1 - jb - t);
+          if (ok && lane == 0) mbar_arrive_expect_tx(&sm.full[st], nb * kL4BlockBytes);
+          __syncwarp();
+          if (ok && lane >= t && lane < t + nb)
+            bulk_load(smem_u32(sm.ring[st] + (lane - t) * kL4BlockBytes), p.cache + blk * kL4BlockBytes, kL4BlockBytes, &sm.full[st]);
+        }
+      }
+      S += nblk + kQ4SegUnits;
+    }
+    // every copy has landed before the CTA may exit (consumed ones at once; after a failed wait,
+    // the ones nobody consumed)
+    for (int st = 0; st < kQ4Stages && st < g; ++st) {
+      const long long last = g - 1 - ((g - 1 - st) % kQ4Stages);
+      for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sm.full[st], static_cast<uint32_t>((last / kQ4Stages) & 1)); ++i) {
+      }
+    }
+    for (int k = max(0, seg - 2); k < seg; ++k)
+      for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sm.q_full[k & 1], static_cast<uint32_t>((k >> 1) & 1)); ++i) {
+      }
+    // publish the (at most two) rows this CTA holds a part of
+    if (lane == 0) {
+      int n_pend = 0;
+      S = S0;
+      for (int r = r0; S + kQ4SegUnits < end && r < R; ++r) {
+        const int nblk = q4_blocks(q4_len(p, r));
+        int j0, j1;
+        if (!segment(S, nblk, j0, j1)) {
+          const int slot = mla_slot(S, start);
+          if (mla_wait(&sm.tk_full[slot], 0, s_abort)) {
+            const long long St = S + kQ4SegUnits;
+            const int n_seg = static_cast<int>(mla_owner(St + nblk - 1, T, n_cta) - mla_owner(St, T, n_cta) + 1);
+            __threadfence();   // the partial (written by other warps, ordered by the mbarrier) first
+            if (atomicAdd(&p.row_sync[r], 1) == n_seg - 1) {
+              p.row_sync[r] = 0;
+              __threadfence();
+              sm.pend_row[n_pend] = r;
+              sm.pend_blocks[n_pend] = nblk;
+              sm.ll[2 + n_pend] = S;
+              ++n_pend;
+            }
+          }
+        }
+        S += nblk + kQ4SegUnits;
+      }
+      sm.n_pend = n_pend;
+      mbar_arrive(&sm.tk_done);
+    }
+    return;
+  }
+
+  const int gq = lane >> 2, tq = lane & 3;
+  long long g = 0;   // tiles of this CTA so far (ring slot, P buffer)
+  int seg = 0;
+  long long S = S0;
+
+  if (warp < kQ4ScoreWarps) {
+    // ================= score warps
+    const int pg = warp & 3, half = warp >> 2;
+    // B fragment column gq of 8 positions j: token 8 j + (gq >> 1) + 4 (gq & 1); its group xor
+    const int tok = (gq >> 1) + 4 * (gq & 1);
+    const int fx = l4_group_xor(tok);
+    const int off_a = pg * kL4BlockBytes + tok * 256 + (((8 * half + tq) ^ fx) << 4);       // group 8 half + tq
+    const int off_b = pg * kL4BlockBytes + tok * 256 + (((8 * half + 4 + tq) ^ fx) << 4);   // group 8 half + 4 + tq
+    const int off_s = pg * kL4BlockBytes + kL4ScaleOff + 16 * (8 * half + tq) + 4 * (gq >> 1);
+    const int off_r = pg * kL4BlockBytes + kL4RopeOff + tok * 128 + (((4 * half + tq) ^ (tok & 4)) << 4);
+    // bytes (gq & 1) and (gq & 1) + 2 of the scale word, into both halves
+    const uint32_t sel0 = (gq & 1) ? 0x4141u : 0x4040u, sel1 = (gq & 1) ? 0x4343u : 0x4242u;
+    for (int r = r0; S + kQ4SegUnits < end && r < R; ++r, ++seg) {
+      const int len = q4_len(p, r), nblk = q4_blocks(len);
+      int j0, j1;
+      const bool complete = segment(S, nblk, j0, j1);
+      // --- this warp's query slice: heads gq, gq + 8; groups 8 half + tq, 8 half + 4 + tq and 8
+      // roped dims, as A fragments in the order in which the nibbles come out of the words
+      mla_wait(&sm.q_full[seg & 1], static_cast<uint32_t>((seg >> 1) & 1), s_abort);
+      uint32_t qa[16][4], qr[2][4];
+      float inv0, inv1;   // softmax scale * 2^-k of the two heads
+      {
+        const unsigned char* sq = sm.q[seg & 1];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const unsigned char* row = sq + (gq + 8 * hh) * kQ4QRow;
+          uint32_t w[32];
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 u = *reinterpret_cast<const uint4*>(row + (8 * half + 4 * gi + tq) * 64 + 16 * i);
+              w[16 * gi + 4 * i] = u.x;
+              w[16 * gi + 4 * i + 1] = u.y;
+              w[16 * gi + 4 * i + 2] = u.z;
+              w[16 * gi + 4 * i + 3] = u.w;
+            }
+          const uint4 e = *reinterpret_cast<const uint4*>(sq + kHeads * kQ4QRow + (gq + 8 * hh) * kQ4PeRow + (4 * half + tq) * 16);
+          const uint32_t ev[4] = {e.x, e.y, e.z, e.w};
+          float amax = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fmaxf(fabsf(bf16lo(w[i])), fabsf(bf16hi(w[i]))));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(bf16lo(ev[i])), fabsf(bf16hi(ev[i]))));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          // 2^k brings the slice's largest element into [2^13, 2^14): bf16 elements down to 2^-27
+          // of it stay exact in fp16.  k is kept in -100 .. 100 so that 2^k and 2^-k are normal
+          int k = 13 - (static_cast<int>(__float_as_uint(amax) >> 23) - 127);
+          k = max(-100, min(100, k));
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+          const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23) * p.scale_log2;
+          if (hh == 0) inv0 = inv;
+          else inv1 = inv;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            // word i holds dims (2 i, 2 i + 1) of its group: k-step 2 (i / 4) + (i & 3) / 2, register i & 1
+            qa[2 * (i >> 2) + ((i & 3) >> 1)][2 * (i & 1) + hh] = pack_f16x2(bf16lo(w[i]) * up, bf16hi(w[i]) * up);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qr[i >> 1][2 * (i & 1) + hh] = pack_bf16x2(bf16lo(ev[i]) * up, bf16hi(ev[i]) * up);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_empty[seg & 1]);
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // heads gq, gq + 8
+
+      for (int jt = j0; jt < j1; jt += kQ4TileBlocks, ++g) {
+        const int st = static_cast<int>(g % kQ4Stages), buf = static_cast<int>(g & 1);
+        const bool active = jt + pg < j1;
+        mla_wait(&sm.full[st], static_cast<uint32_t>((g / kQ4Stages) & 1), s_abort);
+        float s[4];
+        if (active) {
+          const unsigned char* kv = sm.ring[st];
+          float acc[2][2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0.f;
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi) {
+            const uint32_t sw = *reinterpret_cast<const uint32_t*>(kv + off_s + 64 * gi);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint4 u = *reinterpret_cast<const uint4*>(kv + (gi ? off_b : off_a) + 2048 * j);
+              const Q4Scale sc = q4_scale(__byte_perm(sw, 0, j ? sel1 : sel0));
+              const uint32_t wv[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t w = wv[i], w8 = wv[i] >> 8;
+                mma_f16_16816(acc[j][0], qa[8 * gi + 2 * i], q4_lo(w, sc), q4_hi(w, sc));
+                mma_f16_16816(acc[j][1], qa[8 * gi + 2 * i + 1], q4_lo(w8, sc), q4_hi(w8, sc));
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 u = *reinterpret_cast<const uint4*>(kv + off_r + 1024 * j);
+            mma_bf16_16816(acc[j][0], qr[0], u.x, u.y);
+            mma_bf16_16816(acc[j][1], qr[1], u.z, u.w);
+          }
+          // this warp finishes positions 8 half .. + 8 of the block, its partner the others
+          const int o = 1 - half;
+          float own[4], oth[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float a = acc[0][0][i] + acc[0][1][i], b = acc[1][0][i] + acc[1][1][i];
+            own[i] = half ? b : a;
+            oth[i] = (half ? a : b) * (i < 2 ? inv0 : inv1);
+          }
+          sm.part[pg][o][lane] = make_float4(oth[0], oth[1], oth[2], oth[3]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.empty[st]);   // done with the tile
+          q4_bar(2 + pg, 64);
+          const float4 x = sm.part[pg][half][lane];
+          s[0] = fmaf(own[0], inv0, x.x);
+          s[1] = fmaf(own[1], inv0, x.y);
+          s[2] = fmaf(own[2], inv1, x.z);
+          s[3] = fmaf(own[3], inv1, x.w);
+          const int t0 = (jt + pg) * kL4Tokens + 8 * half + tq;   // columns 2 tq, 2 tq + 1: tokens t0, t0 + 4
+          if (t0 >= len) s[0] = s[2] = -INFINITY;
+          if (t0 + 4 >= len) s[1] = s[3] = -INFINITY;
+        } else {
+          s[0] = s[1] = s[2] = s[3] = -INFINITY;
+          if (lane == 0) mbar_arrive(&sm.empty[st]);
+        }
+        const float x0 = fmaxf(s[0], s[1]), x1 = fmaxf(s[2], s[3]);
+        const bool grow = q4_bar_any(x0 > m0 + kQ4Slack || x1 > m1 + kQ4Slack);
+        float a0 = 1.f, a1 = 1.f;
+        if (grow) {
+          float y0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1)), y1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+          y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 2));
+          y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 2));
+          if (tq == 0) {
+            sm.smax[gq][warp] = y0;
+            sm.smax[gq + 8][warp] = y1;
+          }
+          q4_bar(1, kQ4ScoreWarps * 32);
+          float n0 = m0, n1 = m1;
+#pragma unroll
+          for (int w = 0; w < kQ4ScoreWarps; ++w) {
+            n0 = fmaxf(n0, sm.smax[gq][w]);
+            n1 = fmaxf(n1, sm.smax[gq + 8][w]);
+          }
+          a0 = exp2f(m0 - (n0 == -INFINITY ? 0.f : n0));
+          a1 = exp2f(m1 - (n1 == -INFINITY ? 0.f : n1));
+          l0 *= a0;
+          l1 *= a1;
+          m0 = n0;
+          m1 = n1;
+        }
+        const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+        const float p0 = exp2f(s[0] - u0), p1 = exp2f(s[1] - u0), p2 = exp2f(s[2] - u1), p3 = exp2f(s[3] - u1);
+        l0 += p0 + p1;
+        l1 += p2 + p3;
+        if (g >= 2) mla_wait(&sm.p_empty[buf], static_cast<uint32_t>(((g >> 1) - 1) & 1), s_abort);
+        const int col = 16 * pg + 8 * half + 2 * tq;
+        *reinterpret_cast<uint32_t*>(&sm.p[buf][gq][col]) = pack_bf16x2(p0, p1);
+        *reinterpret_cast<uint32_t*>(&sm.p[buf][gq + 8][col]) = pack_bf16x2(p2, p3);
+        if (warp == 0) {
+          if (tq == 0) {
+            sm.alpha[buf][gq] = a0;
+            sm.alpha[buf][gq + 8] = a1;
+          }
+          if (lane == 0) sm.rescale[buf] = grow;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[buf]);
+      }
+
+      // --- row end: l over the quad and the 8 warps; warp 0 publishes 1 / l
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+      if (tq == 0) {
+        sm.lsum[warp][gq] = l0;
+        sm.lsum[warp][gq + 8] = l1;
+      }
+      q4_bar(1, kQ4ScoreWarps * 32);
+      if (warp == 0) {
+        const int fb = seg & 1;
+        if (seg >= 2) mla_wait(&sm.fin_empty[fb], static_cast<uint32_t>(((seg >> 1) - 1) & 1), s_abort);
+        if (tq == 0) {
+          float L0 = 0.f, L1 = 0.f;
+#pragma unroll
+          for (int w = 0; w < kQ4ScoreWarps; ++w) {
+            L0 += sm.lsum[w][gq];
+            L1 += sm.lsum[w][gq + 8];
+          }
+          sm.fin[fb][gq] = L0 > 0.f ? 1.f / L0 : (L0 == 0.f ? 0.f : L0);   // NaN stays NaN
+          sm.fin[fb][gq + 8] = L1 > 0.f ? 1.f / L1 : (L1 == 0.f ? 0.f : L1);
+          if (!complete) {
+            float* ml = p.ml_part + (c * 2 + mla_slot(S, start)) * kHeads * 2;
+            ml[gq * 2] = m0;
+            ml[gq * 2 + 1] = L0;
+            ml[(gq + 8) * 2] = m1;
+            ml[(gq + 8) * 2 + 1] = L1;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.fin_full[fb]);
+          if (!complete) mbar_arrive(&sm.tk_full[mla_slot(S, start)]);
+        }
+      }
+      // lsum is written again only after the next row's tile barriers
+      S += nblk + kQ4SegUnits;
+    }
+  } else {
+    // ================= P V warps: latent dims [128 pv, 128 pv + 128); lane gq owns dims 128 pv + 16 gq
+    // .. + 16, two words, whose dim t is column gq of n-tile t; lane tq takes tokens tq + 4 i
+    const int pv = warp - kQ4ScoreWarps;
+    const int grp = 4 * pv + (gq >> 1);
+    const int off0 = tq * 256 + ((grp ^ l4_group_xor(tq)) << 4) + 8 * (gq & 1);
+    const int off1 = (tq + 4) * 256 + ((grp ^ l4_group_xor(tq + 4)) << 4) + 8 * (gq & 1);
+    const int off_s = kL4ScaleOff + 16 * grp + 4 * tq;
+    const int mi = lane >> 3, ri = lane & 7;
+    for (int r = r0; S + kQ4SegUnits < end && r < R; ++r, ++seg) {
+      const int len = q4_len(p, r), nblk = q4_blocks(len);
+      int j0, j1;
+      const bool complete = segment(S, nblk, j0, j1);
+      float o[16][4];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+      for (int jt = j0; jt < j1; jt += kQ4TileBlocks, ++g) {
+        const int st = static_cast<int>(g % kQ4Stages), buf = static_cast<int>(g & 1);
+        mla_wait(&sm.p_full[buf], static_cast<uint32_t>((g >> 1) & 1), s_abort);
+        mla_wait(&sm.full[st], static_cast<uint32_t>((g / kQ4Stages) & 1), s_abort);
+        if (sm.rescale[buf]) {
+          const float a0 = sm.alpha[buf][gq], a1 = sm.alpha[buf][gq + 8];
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            o[t][0] *= a0;
+            o[t][1] *= a0;
+            o[t][2] *= a1;
+            o[t][3] *= a1;
+          }
+        }
+        const int nb = min(kQ4TileBlocks, j1 - jt);
+#pragma unroll
+        for (int b = 0; b < kQ4TileBlocks; ++b) {
+          if (b >= nb) break;
+          const unsigned char* kv = sm.ring[st] + b * kL4BlockBytes;
+          uint32_t pa[4];
+          ldmatrix_x4(smem_u32(&sm.p[buf][(mi & 1) * 8 + ri][16 * b + (mi >> 1) * 8]), pa[0], pa[1], pa[2], pa[3]);
+          const uint2 w0 = *reinterpret_cast<const uint2*>(kv + off0);
+          const uint2 w1 = *reinterpret_cast<const uint2*>(kv + off1);
+          const uint2 w2 = *reinterpret_cast<const uint2*>(kv + off0 + 2048);
+          const uint2 w3 = *reinterpret_cast<const uint2*>(kv + off1 + 2048);
+          uint32_t sw = *reinterpret_cast<const uint32_t*>(kv + off_s);
+          if (jt + b == nblk - 1) {
+            // tokens past the row's length may hold anything, and P = 0 does not cancel an infinity:
+            // give them a finite scale
+            const int rem = len - (jt + b) * kL4Tokens;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (tq + 4 * i >= rem) sw &= ~(0xffu << (8 * i));
+          }
+          const Q4ScaleB c01 = q4_scale_b(__byte_perm(sw, 0, 0x4140)), c23 = q4_scale_b(__byte_perm(sw, 0, 0x4342));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // even dims of the word are its low half's nibbles, odd ones the high half's
+            const uint32_t x0 = h ? w0.y : w0.x, x1 = h ? w1.y : w1.x, x2 = h ? w2.y : w2.x, x3 = h ? w3.y : w3.x;
+            const uint32_t e01 = __byte_perm(x0, x1, 0x5410), d01 = __byte_perm(x0, x1, 0x7632);
+            const uint32_t e23 = __byte_perm(x2, x3, 0x5410), d23 = __byte_perm(x2, x3, 0x7632);
+            float(*oo)[4] = o + 8 * h;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              mma_bf16_16816(oo[2 * i], pa, q4_b(e01 >> (4 * i), c01), q4_b(e23 >> (4 * i), c23));
+              mma_bf16_16816(oo[2 * i + 1], pa, q4_b(d01 >> (4 * i), c01), q4_b(d23 >> (4 * i), c23));
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.empty[st]);
+          mbar_arrive(&sm.p_empty[buf]);
+        }
+      }
+      const int fb = seg & 1;
+      mla_wait(&sm.fin_full[fb], static_cast<uint32_t>((seg >> 1) & 1), s_abort);
+      // columns 2 tq and 2 tq + 1 of the 16 n-tiles: 32 consecutive dims from 128 pv + 32 tq
+      if (complete) {
+        const float inv[2] = {sm.fin[fb][gq], sm.fin[fb][gq + 8]};
+        bf16* ob = p.o_lat + (static_cast<long long>(r) * kHeads + gq) * 512 + 128 * pv + 32 * tq;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float i = inv[cc >> 1];
+            uint4 v;
+            v.x = pack_bf16x2(o[8 * h][cc] * i, o[8 * h + 1][cc] * i);
+            v.y = pack_bf16x2(o[8 * h + 2][cc] * i, o[8 * h + 3][cc] * i);
+            v.z = pack_bf16x2(o[8 * h + 4][cc] * i, o[8 * h + 5][cc] * i);
+            v.w = pack_bf16x2(o[8 * h + 6][cc] * i, o[8 * h + 7][cc] * i);
+            *reinterpret_cast<uint4*>(ob + (cc >> 1) * 8 * 512 + 16 * (cc & 1) + 8 * h) = v;
+          }
+      } else {
+        float* op = p.o_part + ((c * 2 + mla_slot(S, start)) * kHeads + gq) * 512 + 128 * pv + 32 * tq;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            *reinterpret_cast<float4*>(op + (cc >> 1) * 8 * 512 + 16 * (cc & 1) + 4 * h) =
+                make_float4(o[4 * h][cc], o[4 * h + 1][cc], o[4 * h + 2][cc], o[4 * h + 3][cc]);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sm.fin_empty[fb]);
+        if (!complete) mbar_arrive(&sm.tk_full[mla_slot(S, start)]);
+      }
+      S += nblk + kQ4SegUnits;
+    }
+  }
+
+  // ================= merges of the rows this CTA published last (all compute warps)
+  mla_wait(&sm.tk_done, 0, s_abort);
+  const int n_pend = min(sm.n_pend, 2);
+  float* s_m = reinterpret_cast<float*>(sm.ring);   // the drained ring
+  for (int pi = 0; pi < n_pend; ++pi) {
+    const int r = sm.pend_row[pi], nblk = sm.pend_blocks[pi];
+    const long long Sb = sm.ll[2 + pi], St = Sb + kQ4SegUnits;
+    const long long c_first = mla_owner(St, T, n_cta), c_last = mla_owner(St + nblk - 1, T, n_cta);
+    const int n_seg = static_cast<int>(c_last - c_first + 1);
+    float* s_l = s_m + kHeads * n_seg;
+    auto part_index = [&](int k) -> long long {
+      const long long cc = c_first + k;
+      return cc * 2 + ((k == 0) ? mla_slot(Sb, mla_range_start(cc, T, n_cta)) : 0);
+    };
+    q4_bar(6, kQ4Compute);   // the ring is drained; the previous merge is done with it
+    for (int i = tid; i < kHeads * n_seg; i += kQ4Compute) {
+      const int h = i / n_seg, k = i % n_seg;
+      const long long pk = part_index(k);
+      s_m[i] = __ldcg(p.ml_part + (pk * kHeads + h) * 2);
+      s_l[i] = __ldcg(p.ml_part + (pk * kHeads + h) * 2 + 1);
+    }
+    q4_bar(6, kQ4Compute);
+    if (tid < kHeads) {
+      // w_k = 2^(m_k - M) / sum_k 2^(m_k - M) l_k
+      float M = -INFINITY;
+      for (int k = 0; k < n_seg; ++k)
+        if (s_l[tid * n_seg + k] != 0.f) M = fmaxf(M, s_m[tid * n_seg + k]);
+      float den = 0.f;
+      for (int k = 0; k < n_seg; ++k) {
+        const float l = s_l[tid * n_seg + k];
+        const float w = l != 0.f ? exp2f(s_m[tid * n_seg + k] - M) : 0.f;
+        s_m[tid * n_seg + k] = w;
+        den += w * l;
+      }
+      const float inv = den != 0.f ? 1.f / den : 0.f;
+      for (int k = 0; k < n_seg; ++k) s_m[tid * n_seg + k] *= inv;
+    }
+    q4_bar(6, kQ4Compute);
+    constexpr int kItems = kHeads * 512 / 4;
+    constexpr int kPer = (kItems + kQ4Compute - 1) / kQ4Compute;   // 6, the last third of one unused
+    float4 acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < n_seg; ++k) {
+      const float4* o = reinterpret_cast<const float4*>(p.o_part + part_index(k) * kHeads * 512);
+      float4 v[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[i] = __ldcg(o + min(tid + i * kQ4Compute, kItems - 1));
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float w = s_m[(min(tid + i * kQ4Compute, kItems - 1) / 128) * n_seg + k];
+        acc[i].x += w * v[i].x;
+        acc[i].y += w * v[i].y;
+        acc[i].z += w * v[i].z;
+        acc[i].w += w * v[i].w;
+      }
+    }
+    bf16* ob = p.o_lat + static_cast<long long>(r) * kHeads * 512;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      uint2 v;
+      v.x = pack_bf16x2(acc[i].x, acc[i].y);
+      v.y = pack_bf16x2(acc[i].z, acc[i].w);
+      if (tid + i * kQ4Compute < kItems) *reinterpret_cast<uint2*>(ob + 4 * (tid + i * kQ4Compute)) = v;
+    }
+  }
+}
+
+cudaError_t mla_q4_init() {
+  return cudaFuncSetAttribute(mla_q4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Q4Smem)));
+}
+
+// One CTA per SM, at most kMlaMaxCtas and at most one per two partial slots; the kernel itself
+// uses no more CTAs than the stream has min_units pieces.
+cudaError_t launch_mla_q4(const MlaQ4Params& p, int num_sms, cudaStream_t st) {
+  const int grid = std::min(std::min(num_sms, kMlaMaxCtas), p.part_slots / 2);
+  launch_kernel(mla_q4_kernel, grid, kQ4Threads, sizeof(Q4Smem), st, p);
   return cudaGetLastError();
 }
 

@@ -153,6 +153,11 @@ struct MlaQ4Params {
   float scale_log2;
   bf16* o_lat;                 // [rows, 16, 512]
   int rows;
+  int min_units;               // fewest units of work (16-token blocks) per CTA
+  float* o_part;               // [part_slots, 16, 512] partials, two slots per CTA
+  float* ml_part;              // [part_slots, 16, 2] (m in the log2 domain, l)
+  int part_slots;
+  int* row_sync;               // [rows] zero-initialised, left zero
 };
 
 // Low-rank adapters of many requests (lora.cu)
@@ -240,7 +245,8 @@ cudaError_t launch_mla_prep_q4(const MlaPrepParams&, int, cudaStream_t);
 cudaError_t launch_latent4_write(const Latent4Params&, cudaStream_t);
 cudaError_t launch_latent4_read(const Latent4Params&, cudaStream_t);
 cudaError_t launch_page_plan(const PagePlanParams&, int num_sms, cudaStream_t);
-cudaError_t launch_mla_q4(const MlaQ4Params&, cudaStream_t);
+cudaError_t mla_q4_init();
+cudaError_t launch_mla_q4(const MlaQ4Params&, int num_sms, cudaStream_t);
 cudaError_t launch_lora(const LoraParams&, cudaStream_t);
 cudaError_t mla_decode_init();
 int mla_decode_grid(const MlaDecodeParams&, int num_sms, long long part_slots);

@@ -555,8 +555,8 @@ def _here(t: torch.Tensor) -> int:
 
 def latent4_cache(pages: int, page_size: int, device, layers: int | None = None) -> torch.Tensor:
     """An empty 4-bit latent cache: uint8 [pages, page_size / 16 * 6400] (one per layer with
-    `layers`).  Slots that were never written may hold anything: no value of the format is an
-    infinity or NaN but the roped dims can be, and attention never reads past a row's length."""
+    `layers`).  Slots that were never written may hold anything: what lies past a row's length
+    does not reach its result."""
     if page_size <= 0 or page_size % L4_BLOCK_TOKENS:
         raise ValueError(f"page_size {page_size} (a positive multiple of {L4_BLOCK_TOKENS})")
     shape = (pages, page_size // L4_BLOCK_TOKENS * L4_BLOCK_BYTES)
@@ -652,16 +652,21 @@ def mla_prep_q4(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos:
 
 
 def mla_q4_workspace(rows: int, device) -> dict:
-    """Work buffers of mla_decode_q4 for up to `rows` query rows."""
-    return {}
+    """Work buffers of mla_decode_q4 for up to `rows` query rows: partials (two slots per CTA, one
+    CTA per SM) and the zeroed row tickets."""
+    slots = 2 * min(torch.cuda.get_device_properties(device).multi_processor_count, MLA_MAX_CTAS)
+    return {"o_part": torch.empty((slots, 16, 512), device=device, dtype=torch.float32),
+            "ml_part": torch.empty((slots, 16, 2), device=device, dtype=torch.float32),
+            "row_sync": torch.zeros(rows, device=device, dtype=torch.int32)}
 
 
 def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                   positions: torch.Tensor, page_size: int, softmax_scale: float, o_lat: torch.Tensor,
+                  o_part: torch.Tensor, ml_part: torch.Tensor, row_sync: torch.Tensor,
                   seq_rows: torch.Tensor | None = None) -> torch.Tensor:
     """Latent attention over the paged 4-bit cache (dsv2_mla_decode_q4_args in include/dsv2.h):
     query row r attends positions 0 .. positions[r] of block-table row seq_rows[r] (default r);
-    position -1 or a negative seq_rows entry gives a row of zeros."""
+    position -1 or a negative seq_rows entry gives a row of zeros.  Buffers: mla_q4_workspace."""
     rows = q_abs.shape[0]
     if tuple(q_abs.shape) != (rows, 16, 512) or tuple(q_pe.shape) != (rows, 16, 64) or o_lat.shape != q_abs.shape:
         raise ValueError("q_abs and o_lat must be [rows, 16, 512] and q_pe [rows, 16, 64]")
@@ -673,12 +678,14 @@ def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tenso
     _cuda(block_table, "block_table")
     ptr, blocks = _l4_blocks(cache)
     seqs, width = block_table.shape
+    slots = o_part.shape[0]
     a = MlaDecodeQ4Args(
         _need(q_abs, "q_abs", torch.bfloat16), _need(q_pe, "q_pe", torch.bfloat16), ptr, blocks,
         block_table.data_ptr(), block_table.stride(0) if seqs > 1 else max(width, 1), width, seqs, page_size, rows,
         _need(positions, "positions", torch.int64, rows),
         None if seq_rows is None else _need(seq_rows, "seq_rows", torch.int32, rows), softmax_scale,
-        _need(o_lat, "o_lat", torch.bfloat16))
+        _need(o_lat, "o_lat", torch.bfloat16), _need(o_part, "o_part", torch.float32, slots * 16 * 512),
+        _need(ml_part, "ml_part", torch.float32, slots * 16 * 2), _need(row_sync, "row_sync", torch.int32, rows), slots)
     _lib.call("dsv2_mla_decode_q4", ctypes.byref(a), _here(q_abs))
     return o_lat
 

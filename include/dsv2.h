@@ -641,7 +641,7 @@ DSV2_API int dsv2_mla_prep_q4(const dsv2_mla_prep_args* args, void* cache4, int6
  * of table row seq_rows[r] (NULL: row r).  positions[r] = -1 or seq_rows[r] < 0: nothing to
  * attend, o_lat[r] = 0.  Several rows may name one sequence (draft tokens, prompt chunks).  A
  * length beyond the table's width, a table row >= seqs or a page outside the cache sets
- * DSV2_DEVERR_INDEX. */
+ * DSV2_DEVERR_INDEX.  Calls that share the work buffers must not overlap on the GPU. */
 typedef struct dsv2_mla_decode_q4_args {
   const void* q_abs;           /* [rows, 16, 512] bf16 */
   const void* q_pe;            /* [rows, 16, 64] bf16 */
@@ -657,6 +657,10 @@ typedef struct dsv2_mla_decode_q4_args {
   const int32_t* seq_rows;     /* optional [rows] */
   float softmax_scale;
   void* o_lat;                 /* [rows, 16, 512] bf16 */
+  float* o_part;               /* work buffer [part_slots, 16, 512] */
+  float* ml_part;              /* work buffer [part_slots, 16, 2] */
+  int32_t* row_sync;           /* [rows], zero before the first call and left zero by every call */
+  int32_t part_slots;          /* two per CTA: 2 * SMs for the whole GPU, at least 2 */
 } dsv2_mla_decode_q4_args;
 
 DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* stream);
