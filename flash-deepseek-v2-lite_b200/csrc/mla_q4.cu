@@ -8,19 +8,18 @@
 
 namespace dsv2 {
 
-constexpr int kQ4Pos = 64;                                   // positions of a tile: 4 blocks
+constexpr int kQ4Pos = 128;                                  // positions of a tile: 8 blocks
 constexpr int kQ4TileBlocks = kQ4Pos / kL4Tokens;
-constexpr int kQ4Stages = 7;
-constexpr int kQ4StageBytes = kQ4TileBlocks * kL4BlockBytes; // 25600
+constexpr int kQ4Stages = 3;
+constexpr int kQ4StageBytes = kQ4TileBlocks * kL4BlockBytes; // 51200
 constexpr int kQ4SegUnits = 4;                               // per-row cost in blocks (work balance)
-constexpr int kQ4ScoreWarps = 8;                             // 4 blocks x 2 halves of the dims
-constexpr int kQ4PvWarps = 4;                                // 128 latent dims each
+constexpr int kQ4ScoreWarps = 8;                             // a block of a tile each
+constexpr int kQ4PvWarps = 8;                                // 64 latent dims each
 constexpr int kQ4Compute = (kQ4ScoreWarps + kQ4PvWarps) * 32;
-constexpr int kQ4ProducerWarp = kQ4ScoreWarps + kQ4PvWarps;  // warp 12: copies, then tickets
+constexpr int kQ4ProducerWarp = kQ4ScoreWarps + kQ4PvWarps;  // warp 16: copies, then tickets
 constexpr int kQ4Threads = kQ4Compute + 32;
-constexpr int kQ4QRow = 1024 + 16;                           // padded shared rows of q_abs / q_pe
-constexpr int kQ4PeRow = 128 + 16;
-constexpr int kQ4QBytes = kHeads * (kQ4QRow + kQ4PeRow);
+constexpr int kQ4QBytes = kHeads * (1024 + 128);             // a query row: q_abs, then q_pe
+constexpr int kQ4Steps = 32;                                 // k-steps of 16 latent dims; 4 roped ones follow
 constexpr int kQ4PRow = kQ4Pos + 8;                          // row of P
 constexpr float kQ4Slack = 8.f;                              // log2 growth of a row's maximum left unscaled
 
@@ -30,7 +29,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -65,6 +64,11 @@ __device__ __forceinline__ uint32_t b2mul(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+__device__ __forceinline__ float ex2(float x) {   // 2^x to 2 ulp, results below 2^-126 are 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -86,8 +90,21 @@ __device__ __forceinline__ Q4Scale q4_scale(uint32_t codes /* code of each half 
   r.b4 = h2mul(r.s, 0xd480d480u);   // -72
   return r;
 }
-__device__ __forceinline__ uint32_t q4_lo(uint32_t w, const Q4Scale& c) { return h2fma((w & 0x000f000fu) | 0x64006400u, c.s, c.b0); }
-__device__ __forceinline__ uint32_t q4_hi(uint32_t w, const Q4Scale& c) { return h2fma((w & 0x00f000f0u) | 0x54005400u, c.s, c.b4); }
+// (w & mask) | bits in one instruction: it takes one immediate, so the bits are kept in a register
+// that the compiler cannot see through (else it splits the two constants over two instructions)
+template <uint32_t kMask>
+__device__ __forceinline__ uint32_t q4_under(uint32_t w, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(kMask), "r"(bits));
+  return r;
+}
+__device__ __forceinline__ uint32_t q4_opaque(uint32_t bits) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(bits));
+  return r;
+}
+__device__ __forceinline__ uint32_t q4_lo(uint32_t w, const Q4Scale& c, uint32_t m1024) { return h2fma(q4_under<0x000f000fu>(w, m1024), c.s, c.b0); }
+__device__ __forceinline__ uint32_t q4_hi(uint32_t w, const Q4Scale& c, uint32_t m64) { return h2fma(q4_under<0x00f000f0u>(w, m64), c.s, c.b4); }
 
 // Nibble pairs to the bf16 pairs of the P V product: P spans more binades than fp16 has (a
 // probability far below the row's largest still decides a dim in which that token is 0).  bf16
@@ -102,7 +119,27 @@ __device__ __forceinline__ Q4ScaleB q4_scale_b(uint32_t codes) {
   r.b = b2mul(codes << 4, 0xfb08fb08u);   // -136 * 2^112
   return r;
 }
-__device__ __forceinline__ uint32_t q4_b(uint32_t w, const Q4ScaleB& c) { return b2fma((w & 0x000f000fu) | 0x43004300u, c.s, c.b); }
+__device__ __forceinline__ uint32_t q4_b(uint32_t w, const Q4ScaleB& c, uint32_t m128) { return b2fma(q4_under<0x000f000fu>(w, m128), c.s, c.b); }
+
+// Bounded mbarrier wait, a loop of four instructions: the waiting warps share the issue slots with
+// the working ones.  It gives up after 2^24 polls (seconds), and at once when this CTA already has.
+__device__ __forceinline__ bool q4_wait(uint64_t* bar, uint32_t parity, volatile int* s_abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  if (*s_abort != 0) return false;
+  uint32_t left;
+  asm volatile(
+      "{\n .reg .pred p;\n mov.u32 %0, 16777216;\n"
+      "POLL:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+      " sub.u32 %0, %0, 1;\n setp.ne.u32 p, %0, 0;\n @p bra POLL;\n"
+      "DONE:\n}\n"
+      : "=&r"(left)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (left != 0) return true;
+  *s_abort = 1;
+  set_device_error(kErrMbarTimeout);
+  return false;
+}
 
 // Attended length of query row r: 0 .. the positions its table row can hold.
 __device__ __forceinline__ int q4_len(const MlaQ4Params& p, int r) {
@@ -119,11 +156,15 @@ __device__ __forceinline__ int q4_len(const MlaQ4Params& p, int r) {
 __device__ __forceinline__ int q4_blocks(int len) { return len > 0 ? (len + kL4Tokens - 1) / kL4Tokens : 1; }
 __device__ __forceinline__ int q4_units(int len) { return q4_blocks(len) + kQ4SegUnits; }
 
+// place of a lane's fragment of a step in its row of 32
+__device__ __forceinline__ int q4_frag_slot(int step, int lane) { return lane ^ ((step & 6) >> 1); }
+
 struct Q4Smem {
   unsigned char ring[kQ4Stages][kQ4StageBytes];
-  unsigned char q[2][kQ4QBytes];            // [16][1040] q_abs, [16][144] q_pe
+  unsigned char q[2][kQ4QBytes];            // query rows as they lie in memory
+  uint4 qf[kQ4Steps + 4][32];               // the row's A fragments, one per lane: fp16 latent, bf16 roped steps
   bf16 p[2][kHeads][kQ4PRow];               // P, columns in the order the fragments want
-  float4 part[kQ4TileBlocks][2][32];        // scores of one half of the dims for the other half's warp
+  float qinv[kHeads];                       // softmax scale over the power of two that scaled the query
   float smax[kHeads][kQ4ScoreWarps];
   float alpha[2][kHeads];
   float lsum[kQ4ScoreWarps][kHeads];
@@ -138,14 +179,13 @@ struct Q4Smem {
 static_assert(sizeof(Q4Smem) <= 232448, "4-bit latent attention: shared memory exceeds 227 KB");
 
 // One launch, persistent: the rows form one stream of units (kQ4SegUnits of per-row cost, then
-// the row's 16-token blocks), cut into equal ranges, one CTA (13 warps) per SM.  A row inside
+// the row's 16-token blocks), cut into equal ranges, one CTA (17 warps) per SM.  A row inside
 // one range writes o_lat; a row cut by a boundary leaves (o, m, l) partials that the last of
 // its CTAs merges (row tickets).
-//  - warps 0-7, scores: warp w takes block w % 4 of a tile (16 positions) and half w / 4 of the
-//    dims (256 latent, 32 roped), its query slice in registers as fp16 scaled by a power of two
-//    per head; the halves exchange 8 positions each;
-//  - warps 8-11, P V: 128 latent dims each;
-//  - warp 12: copies blocks (looked up 32 at a time) and query rows, then publishes tickets.
+//  - warps 0-7, scores: one block (16 positions) of a tile each, all dims; the row's query
+//    fragments are made once per row, in shared memory, as fp16 scaled by a power of two per head;
+//  - warps 8-15, P V: 64 latent dims each;
+//  - warp 16: copies blocks (looked up 32 at a time) and query rows, then publishes tickets.
 // The maximum that P is taken against is kept until a score exceeds it by 2^kQ4Slack: the score
 // warps then agree on a new one and the P V warps rescale.
 __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params p) {
@@ -253,26 +293,25 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
   if (warp == kQ4ProducerWarp) {
     // ================= producer warp
     bool ok = true;
-    long long g = 0;
-    int seg = 0;
+    int seg = 0, st = 0;
+    uint32_t round = 0;   // times the ring has been filled
     long long S = S0;
     for (int r = r0; S + kQ4SegUnits < end && r < R; ++r, ++seg) {
       const int len = q4_len(p, r), nblk = q4_blocks(len);
       int j0, j1;
       segment(S, nblk, j0, j1);
       // query block into buffer seg & 1
-      if (seg >= 2 && ok) ok = mla_wait(&sm.q_empty[seg & 1], static_cast<uint32_t>(((seg >> 1) - 1) & 1), s_abort);
+      if (seg >= 2 && ok) ok = q4_wait(&sm.q_empty[seg & 1], static_cast<uint32_t>(((seg >> 1) - 1) & 1), s_abort);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         unsigned char* dq = sm.q[seg & 1];
         uint64_t* bar = &sm.q_full[seg & 1];
-        if (lane == 0) mbar_arrive_expect_tx(bar, kHeads * (1024 + 128));
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, kQ4QBytes);
+          bulk_load(smem_u32(dq), p.q_abs + static_cast<long long>(r) * kHeads * 512, kHeads * 1024, bar);
+          bulk_load(smem_u32(dq + kHeads * 1024), p.q_pe + static_cast<long long>(r) * kHeads * 64, kHeads * 128, bar);
+        }
         __syncwarp();
-        if (lane < kHeads)
-          bulk_load(smem_u32(dq + lane * kQ4QRow), p.q_abs + (static_cast<long long>(r) * kHeads + lane) * 512, 1024, bar);
-        else
-          bulk_load(smem_u32(dq + kHeads * kQ4QRow + (lane - kHeads) * kQ4PeRow),
-                    p.q_pe + (static_cast<long long>(r) * kHeads + lane - kHeads) * 64, 128, bar);
       }
       const int* table = len > 0 ? p.table + (p.seq_rows ? p.seq_rows[r] : r) * p.table_stride : nullptr;
       for (int jb = j0; jb < j1; jb += 32) {
@@ -286,24 +325,28 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
             blk = 0;
           }
         }
-        for (int t = 0; t < 32 && jb + t < j1; t += kQ4TileBlocks, ++g) {
-          const int st = static_cast<int>(g % kQ4Stages);
-          if (g >= kQ4Stages && ok) ok = mla_wait(&sm.empty[st], static_cast<uint32_t>(((g / kQ4Stages) - 1) & 1), s_abort);
+        for (int t = 0; t < 32 && jb + t < j1; t += kQ4TileBlocks) {
+          if (round > 0 && ok) ok = q4_wait(&sm.empty[st], (round - 1) & 1, s_abort);
           ok = __all_sync(0xffffffffu, ok);
           const int nb = min(kQ4TileBlocks, j1 - jb - t);
           if (ok && lane == 0) mbar_arrive_expect_tx(&sm.full[st], nb * kL4BlockBytes);
           __syncwarp();
           if (ok && lane >= t && lane < t + nb)
             bulk_load(smem_u32(sm.ring[st] + (lane - t) * kL4BlockBytes), p.cache + blk * kL4BlockBytes, kL4BlockBytes, &sm.full[st]);
+          if (++st == kQ4Stages) {
+            st = 0;
+            ++round;
+          }
         }
       }
       S += nblk + kQ4SegUnits;
     }
     // every copy has landed before the CTA may exit (consumed ones at once; after a failed wait,
     // the ones nobody consumed)
-    for (int st = 0; st < kQ4Stages && st < g; ++st) {
-      const long long last = g - 1 - ((g - 1 - st) % kQ4Stages);
-      for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sm.full[st], static_cast<uint32_t>((last / kQ4Stages) & 1)); ++i) {
+    for (int i = 0; i < kQ4Stages; ++i) {
+      if (i >= st && round == 0) break;   // never filled
+      const uint32_t last = i < st ? round : round - 1;
+      for (uint32_t n = 0; n < (1u << 20) && !mbar_try_wait(&sm.full[i], last & 1); ++n) {
       }
     }
     for (int k = max(0, seg - 2); k < seg; ++k)
@@ -318,7 +361,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
         int j0, j1;
         if (!segment(S, nblk, j0, j1)) {
           const int slot = mla_slot(S, start);
-          if (mla_wait(&sm.tk_full[slot], 0, s_abort)) {
+          if (q4_wait(&sm.tk_full[slot], 0, s_abort)) {
             const long long St = S + kQ4SegUnits;
             const int n_seg = static_cast<int>(mla_owner(St + nblk - 1, T, n_cta) - mla_owner(St, T, n_cta) + 1);
             __threadfence();   // the partial (written by other warps, ordered by the mbarrier) first
@@ -341,137 +384,147 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
   }
 
   const int gq = lane >> 2, tq = lane & 3;
-  long long g = 0;   // tiles of this CTA so far (ring slot, P buffer)
-  int seg = 0;
+  int seg = 0, st = 0;
+  uint32_t ring_phase = 0, g = 0;   // parity of the ring's round; tiles of this CTA so far
   long long S = S0;
+  auto next_tile = [&]() {
+    ++g;
+    if (++st == kQ4Stages) {
+      st = 0;
+      ring_phase ^= 1;
+    }
+  };
 
   if (warp < kQ4ScoreWarps) {
     // ================= score warps
-    const int pg = warp & 3, half = warp >> 2;
-    // B fragment column gq of 8 positions j: token 8 j + (gq >> 1) + 4 (gq & 1); its group xor
+    const uint32_t m1024 = q4_opaque(0x64006400u), m64 = q4_opaque(0x54005400u);
+    // B fragment column gq of the 8 positions of half i of a block: token 8 i + (gq >> 1) + 4 (gq & 1);
+    // lane tq takes groups 4 gi + tq
     const int tok = (gq >> 1) + 4 * (gq & 1);
     const int fx = l4_group_xor(tok);
-    const int off_a = pg * kL4BlockBytes + tok * 256 + (((8 * half + tq) ^ fx) << 4);       // group 8 half + tq
-    const int off_b = pg * kL4BlockBytes + tok * 256 + (((8 * half + 4 + tq) ^ fx) << 4);   // group 8 half + 4 + tq
-    const int off_s = pg * kL4BlockBytes + kL4ScaleOff + 16 * (8 * half + tq) + 4 * (gq >> 1);
-    const int off_r = pg * kL4BlockBytes + kL4RopeOff + tok * 128 + (((4 * half + tq) ^ (tok & 4)) << 4);
+    const int base = warp * kL4BlockBytes;
+    const int off_w = base + tok * 256 + ((tq ^ (fx & 3)) << 4);   // group gi: + 64 (gi ^ (fx >> 2))
+    const int off_s = base + kL4ScaleOff + 16 * tq + 4 * (gq >> 1);
+    const int off_r = base + kL4RopeOff + tok * 128 + (tq << 4);   // chunk 4 h + tq: + 64 (h ^ (tok >> 2))
     // bytes (gq & 1) and (gq & 1) + 2 of the scale word, into both halves
     const uint32_t sel0 = (gq & 1) ? 0x4141u : 0x4040u, sel1 = (gq & 1) ? 0x4343u : 0x4242u;
     for (int r = r0; S + kQ4SegUnits < end && r < R; ++r, ++seg) {
       const int len = q4_len(p, r), nblk = q4_blocks(len);
       int j0, j1;
       const bool complete = segment(S, nblk, j0, j1);
-      // --- this warp's query slice: heads gq, gq + 8; groups 8 half + tq, 8 half + 4 + tq and 8
-      // roped dims, as A fragments in the order in which the nibbles come out of the words
-      mla_wait(&sm.q_full[seg & 1], static_cast<uint32_t>((seg >> 1) & 1), s_abort);
-      uint32_t qa[16][4], qr[2][4];
-      float inv0, inv1;   // softmax scale * 2^-k of the two heads
-      {
+      // --- query fragments: thread (heads h and h + 8, part e) takes pieces e + 16 i of 8 dims (words
+      // 4 (e & 3) .. of group 4 i + e / 4), and parts 0 .. 7 a piece of 8 roped dims.  Every score warp is
+      // past the previous row's products (row-end barrier)
+      q4_wait(&sm.q_full[seg & 1], static_cast<uint32_t>((seg >> 1) & 1), s_abort);
+      if (warp < 4) {
+        const int h = tid >> 4, e = tid & 15;
         const unsigned char* sq = sm.q[seg & 1];
+        uint4 u[2][5];
+        float up[2];
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          const unsigned char* row = sq + (gq + 8 * hh) * kQ4QRow;
-          uint32_t w[32];
 #pragma unroll
-          for (int gi = 0; gi < 2; ++gi)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint4 u = *reinterpret_cast<const uint4*>(row + (8 * half + 4 * gi + tq) * 64 + 16 * i);
-              w[16 * gi + 4 * i] = u.x;
-              w[16 * gi + 4 * i + 1] = u.y;
-              w[16 * gi + 4 * i + 2] = u.z;
-              w[16 * gi + 4 * i + 3] = u.w;
-            }
-          const uint4 e = *reinterpret_cast<const uint4*>(sq + kHeads * kQ4QRow + (gq + 8 * hh) * kQ4PeRow + (4 * half + tq) * 16);
-          const uint32_t ev[4] = {e.x, e.y, e.z, e.w};
+          for (int i = 0; i < 4; ++i) u[hh][i] = *reinterpret_cast<const uint4*>(sq + (h + 8 * hh) * 1024 + e * 16 + 256 * i);
+          u[hh][4] = *reinterpret_cast<const uint4*>(sq + kHeads * 1024 + (h + 8 * hh) * 128 + (e & 7) * 16);
           float amax = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fmaxf(fabsf(bf16lo(w[i])), fabsf(bf16hi(w[i]))));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(bf16lo(ev[i])), fabsf(bf16hi(ev[i]))));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          // 2^k brings the slice's largest element into [2^13, 2^14): bf16 elements down to 2^-27
-          // of it stay exact in fp16.  k is kept in -100 .. 100 so that 2^k and 2^-k are normal
-          int k = 13 - (static_cast<int>(__float_as_uint(amax) >> 23) - 127);
-          k = max(-100, min(100, k));
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-          const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23) * p.scale_log2;
-          if (hh == 0) inv0 = inv;
-          else inv1 = inv;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            // word i holds dims (2 i, 2 i + 1) of its group: k-step 2 (i / 4) + (i & 3) / 2, register i & 1
-            qa[2 * (i >> 2) + ((i & 3) >> 1)][2 * (i & 1) + hh] = pack_f16x2(bf16lo(w[i]) * up, bf16hi(w[i]) * up);
+          for (int i = 0; i < 5; ++i) {
+            const uint4 v = u[hh][i];
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16lo(v.x)), fabsf(bf16hi(v.x))), fmaxf(fabsf(bf16lo(v.y)), fabsf(bf16hi(v.y)))));
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16lo(v.z)), fabsf(bf16hi(v.z))), fmaxf(fabsf(bf16lo(v.w)), fabsf(bf16hi(v.w)))));
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) qr[i >> 1][2 * (i & 1) + hh] = pack_bf16x2(bf16lo(ev[i]) * up, bf16hi(ev[i]) * up);
+          for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          // 2^k brings the head's largest element into [2^13, 2^14): bf16 elements down to 2^-27 of it
+          // stay exact in fp16.  k is kept in -100 .. 100 so that 2^k and 2^-k are normal
+          int k = 13 - (static_cast<int>(__float_as_uint(amax) >> 23) - 127);
+          k = max(-100, min(100, k));
+          up[hh] = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+          if (e == 0) sm.qinv[h + 8 * hh] = __uint_as_float(static_cast<uint32_t>(127 - k) << 23) * p.scale_log2;
+        }
+        // word j of group c holds its dims (2 j, 2 j + 1): step 8 (c / 4) + j / 2, registers 2 (j & 1) and
+        // 2 (j & 1) + 1 (the two heads) of lane (h, c & 3)
+        auto f16 = [&](int hh, uint32_t w) { return pack_f16x2(bf16lo(w) * up[hh], bf16hi(w) * up[hh]); };
+        auto b16 = [&](int hh, uint32_t w) { return pack_bf16x2(bf16lo(w) * up[hh], bf16hi(w) * up[hh]); };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int step = 8 * i + 2 * (e & 3), ln = h * 4 + (e >> 2);
+          const uint4 v0 = u[0][i], v1 = u[1][i];
+          sm.qf[step][q4_frag_slot(step, ln)] = make_uint4(f16(0, v0.x), f16(1, v1.x), f16(0, v0.y), f16(1, v1.y));
+          sm.qf[step + 1][q4_frag_slot(step + 1, ln)] = make_uint4(f16(0, v0.z), f16(1, v1.z), f16(0, v0.w), f16(1, v1.w));
+        }
+        if (e < 8) {
+          const int step = kQ4Steps + 2 * (e >> 2), ln = h * 4 + (e & 3);
+          const uint4 v0 = u[0][4], v1 = u[1][4];
+          sm.qf[step][q4_frag_slot(step, ln)] = make_uint4(b16(0, v0.x), b16(1, v1.x), b16(0, v0.y), b16(1, v1.y));
+          sm.qf[step + 1][q4_frag_slot(step + 1, ln)] = make_uint4(b16(0, v0.z), b16(1, v1.z), b16(0, v0.w), b16(1, v1.w));
         }
       }
-      __syncwarp();
+      q4_bar(1, kQ4ScoreWarps * 32);
       if (lane == 0) mbar_arrive(&sm.q_empty[seg & 1]);
+      const float inv0 = sm.qinv[gq], inv1 = sm.qinv[gq + 8];
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // heads gq, gq + 8
 
-      for (int jt = j0; jt < j1; jt += kQ4TileBlocks, ++g) {
-        const int st = static_cast<int>(g % kQ4Stages), buf = static_cast<int>(g & 1);
-        const bool active = jt + pg < j1;
-        mla_wait(&sm.full[st], static_cast<uint32_t>((g / kQ4Stages) & 1), s_abort);
-        float s[4];
-        if (active) {
+      for (int jt = j0; jt < j1; jt += kQ4TileBlocks, next_tile()) {
+        const int buf = static_cast<int>(g & 1);
+        q4_wait(&sm.full[st], ring_phase, s_abort);
+        float s[2][4];
+        if (jt + warp < j1) {
           const unsigned char* kv = sm.ring[st];
-          float acc[2][2][4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0.f;
-#pragma unroll
-          for (int gi = 0; gi < 2; ++gi) {
+          for (int gi = 0; gi < 4; ++gi) {
             const uint32_t sw = *reinterpret_cast<const uint32_t*>(kv + off_s + 64 * gi);
+            const Q4Scale sc[2] = {q4_scale(__byte_perm(sw, 0, sel0)), q4_scale(__byte_perm(sw, 0, sel1))};
+            const uint4 u[2] = {*reinterpret_cast<const uint4*>(kv + off_w + 64 * (gi ^ (fx >> 2))),
+                                *reinterpret_cast<const uint4*>(kv + off_w + 2048 + 64 * (gi ^ (fx >> 2)))};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint4 u = *reinterpret_cast<const uint4*>(kv + (gi ? off_b : off_a) + 2048 * j);
-              const Q4Scale sc = q4_scale(__byte_perm(sw, 0, j ? sel1 : sel0));
-              const uint32_t wv[4] = {u.x, u.y, u.z, u.w};
+            for (int i = 0; i < 4; ++i) {
+              const int ks = 8 * gi + 2 * i;
+              const uint4 q0 = sm.qf[ks][q4_frag_slot(ks, lane)], q1 = sm.qf[ks + 1][q4_frag_slot(ks + 1, lane)];
+              const uint32_t a0[4] = {q0.x, q0.y, q0.z, q0.w}, a1[4] = {q1.x, q1.y, q1.z, q1.w};
+              uint32_t w[2];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t w = wv[i], w8 = wv[i] >> 8;
-                mma_f16_16816(acc[j][0], qa[8 * gi + 2 * i], q4_lo(w, sc), q4_hi(w, sc));
-                mma_f16_16816(acc[j][1], qa[8 * gi + 2 * i + 1], q4_lo(w8, sc), q4_hi(w8, sc));
+              for (int j = 0; j < 2; ++j) {
+                w[j] = i == 0 ? u[j].x : i == 1 ? u[j].y : i == 2 ? u[j].z : u[j].w;
+                mma_f16_16816(s[j], a0, q4_lo(w[j], sc[j], m1024), q4_hi(w[j], sc[j], m64));
               }
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                mma_f16_16816(s[j], a1, q4_lo(w[j] >> 8, sc[j], m1024), q4_hi(w[j] >> 8, sc[j], m64));
             }
           }
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 u = *reinterpret_cast<const uint4*>(kv + off_r + 1024 * j);
-            mma_bf16_16816(acc[j][0], qr[0], u.x, u.y);
-            mma_bf16_16816(acc[j][1], qr[1], u.z, u.w);
-          }
-          // this warp finishes positions 8 half .. + 8 of the block, its partner the others
-          const int o = 1 - half;
-          float own[4], oth[4];
+          for (int h = 0; h < 2; ++h) {
+            const int ks = kQ4Steps + 2 * h;
+            const uint4 q0 = sm.qf[ks][q4_frag_slot(ks, lane)], q1 = sm.qf[ks + 1][q4_frag_slot(ks + 1, lane)];
+            const uint32_t a0[4] = {q0.x, q0.y, q0.z, q0.w}, a1[4] = {q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = acc[0][0][i] + acc[0][1][i], b = acc[1][0][i] + acc[1][1][i];
-            own[i] = half ? b : a;
-            oth[i] = (half ? a : b) * (i < 2 ? inv0 : inv1);
+            for (int j = 0; j < 2; ++j) {
+              const uint4 u = *reinterpret_cast<const uint4*>(kv + off_r + 1024 * j + 64 * (h ^ (tok >> 2)));
+              mma_bf16_16816(s[j], a0, u.x, u.y);
+              mma_bf16_16816(s[j], a1, u.z, u.w);
+            }
           }
-          sm.part[pg][o][lane] = make_float4(oth[0], oth[1], oth[2], oth[3]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.empty[st]);   // done with the tile
-          q4_bar(2 + pg, 64);
-          const float4 x = sm.part[pg][half][lane];
-          s[0] = fmaf(own[0], inv0, x.x);
-          s[1] = fmaf(own[1], inv0, x.y);
-          s[2] = fmaf(own[2], inv1, x.z);
-          s[3] = fmaf(own[3], inv1, x.w);
-          const int t0 = (jt + pg) * kL4Tokens + 8 * half + tq;   // columns 2 tq, 2 tq + 1: tokens t0, t0 + 4
-          if (t0 >= len) s[0] = s[2] = -INFINITY;
-          if (t0 + 4 >= len) s[1] = s[3] = -INFINITY;
+          const int t0 = (jt + warp) * kL4Tokens + tq;   // columns 2 tq, 2 tq + 1: tokens t0 + 8 j, + 4
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[j][0] *= inv0;
+            s[j][1] *= inv0;
+            s[j][2] *= inv1;
+            s[j][3] *= inv1;
+            if (t0 + 8 * j >= len) s[j][0] = s[j][2] = -INFINITY;
+            if (t0 + 8 * j + 4 >= len) s[j][1] = s[j][3] = -INFINITY;
+          }
         } else {
-          s[0] = s[1] = s[2] = s[3] = -INFINITY;
-          if (lane == 0) mbar_arrive(&sm.empty[st]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = -INFINITY;
         }
-        const float x0 = fmaxf(s[0], s[1]), x1 = fmaxf(s[2], s[3]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[st]);   // done with the tile
+        const float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        const float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
         const bool grow = q4_bar_any(x0 > m0 + kQ4Slack || x1 > m1 + kQ4Slack);
         float a0 = 1.f, a1 = 1.f;
         if (grow) {
@@ -489,21 +542,24 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
             n0 = fmaxf(n0, sm.smax[gq][w]);
             n1 = fmaxf(n1, sm.smax[gq + 8][w]);
           }
-          a0 = exp2f(m0 - (n0 == -INFINITY ? 0.f : n0));
-          a1 = exp2f(m1 - (n1 == -INFINITY ? 0.f : n1));
+          a0 = ex2(m0 - (n0 == -INFINITY ? 0.f : n0));
+          a1 = ex2(m1 - (n1 == -INFINITY ? 0.f : n1));
           l0 *= a0;
           l1 *= a1;
           m0 = n0;
           m1 = n1;
         }
         const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
-        const float p0 = exp2f(s[0] - u0), p1 = exp2f(s[1] - u0), p2 = exp2f(s[2] - u1), p3 = exp2f(s[3] - u1);
-        l0 += p0 + p1;
-        l1 += p2 + p3;
-        if (g >= 2) mla_wait(&sm.p_empty[buf], static_cast<uint32_t>(((g >> 1) - 1) & 1), s_abort);
-        const int col = 16 * pg + 8 * half + 2 * tq;
-        *reinterpret_cast<uint32_t*>(&sm.p[buf][gq][col]) = pack_bf16x2(p0, p1);
-        *reinterpret_cast<uint32_t*>(&sm.p[buf][gq + 8][col]) = pack_bf16x2(p2, p3);
+        if (g >= 2) q4_wait(&sm.p_empty[buf], ((g >> 1) - 1) & 1, s_abort);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float p0 = ex2(s[j][0] - u0), p1 = ex2(s[j][1] - u0), p2 = ex2(s[j][2] - u1), p3 = ex2(s[j][3] - u1);
+          l0 += p0 + p1;
+          l1 += p2 + p3;
+          const int col = 16 * warp + 8 * j + 2 * tq;
+          *reinterpret_cast<uint32_t*>(&sm.p[buf][gq][col]) = pack_bf16x2(p0, p1);
+          *reinterpret_cast<uint32_t*>(&sm.p[buf][gq + 8][col]) = pack_bf16x2(p2, p3);
+        }
         if (warp == 0) {
           if (tq == 0) {
             sm.alpha[buf][gq] = a0;
@@ -515,7 +571,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
         if (lane == 0) mbar_arrive(&sm.p_full[buf]);
       }
 
-      // --- row end: l over the quad and the 8 warps; warp 0 publishes 1 / l
+      // --- row end: l over the quad and the score warps; warp 0 publishes 1 / l
       l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
       l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
       l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
@@ -527,7 +583,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
       q4_bar(1, kQ4ScoreWarps * 32);
       if (warp == 0) {
         const int fb = seg & 1;
-        if (seg >= 2) mla_wait(&sm.fin_empty[fb], static_cast<uint32_t>(((seg >> 1) - 1) & 1), s_abort);
+        if (seg >= 2) q4_wait(&sm.fin_empty[fb], static_cast<uint32_t>(((seg >> 1) - 1) & 1), s_abort);
         if (tq == 0) {
           float L0 = 0.f, L1 = 0.f;
 #pragma unroll
@@ -555,29 +611,30 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
       S += nblk + kQ4SegUnits;
     }
   } else {
-    // ================= P V warps: latent dims [128 pv, 128 pv + 128); lane gq owns dims 128 pv + 16 gq
-    // .. + 16, two words, whose dim t is column gq of n-tile t; lane tq takes tokens tq + 4 i
+    // ================= P V warps: latent dims [64 pv, 64 pv + 64); lane gq owns dims 64 pv + 8 gq
+    // .. + 8, one word, whose dim t is column gq of n-tile t; lane tq takes tokens tq + 4 i
+    const uint32_t m128 = q4_opaque(0x43004300u);
     const int pv = warp - kQ4ScoreWarps;
-    const int grp = 4 * pv + (gq >> 1);
-    const int off0 = tq * 256 + ((grp ^ l4_group_xor(tq)) << 4) + 8 * (gq & 1);
-    const int off1 = (tq + 4) * 256 + ((grp ^ l4_group_xor(tq + 4)) << 4) + 8 * (gq & 1);
+    const int grp = 2 * pv + (gq >> 2);
+    const int off0 = tq * 256 + ((grp ^ l4_group_xor(tq)) << 4) + 4 * (gq & 3);
+    const int off1 = (tq + 4) * 256 + ((grp ^ l4_group_xor(tq + 4)) << 4) + 4 * (gq & 3);
     const int off_s = kL4ScaleOff + 16 * grp + 4 * tq;
     const int mi = lane >> 3, ri = lane & 7;
     for (int r = r0; S + kQ4SegUnits < end && r < R; ++r, ++seg) {
       const int len = q4_len(p, r), nblk = q4_blocks(len);
       int j0, j1;
       const bool complete = segment(S, nblk, j0, j1);
-      float o[16][4];
+      float o[8][4];
 #pragma unroll
-      for (int t = 0; t < 16; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-      for (int jt = j0; jt < j1; jt += kQ4TileBlocks, ++g) {
-        const int st = static_cast<int>(g % kQ4Stages), buf = static_cast<int>(g & 1);
-        mla_wait(&sm.p_full[buf], static_cast<uint32_t>((g >> 1) & 1), s_abort);
-        mla_wait(&sm.full[st], static_cast<uint32_t>((g / kQ4Stages) & 1), s_abort);
+      for (int t = 0; t < 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+      for (int jt = j0; jt < j1; jt += kQ4TileBlocks, next_tile()) {
+        const int buf = static_cast<int>(g & 1);
+        q4_wait(&sm.p_full[buf], (g >> 1) & 1, s_abort);
+        q4_wait(&sm.full[st], ring_phase, s_abort);
         if (sm.rescale[buf]) {
           const float a0 = sm.alpha[buf][gq], a1 = sm.alpha[buf][gq + 8];
 #pragma unroll
-          for (int t = 0; t < 16; ++t) {
+          for (int t = 0; t < 8; ++t) {
             o[t][0] *= a0;
             o[t][1] *= a0;
             o[t][2] *= a1;
@@ -585,18 +642,18 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
           }
         }
         const int nb = min(kQ4TileBlocks, j1 - jt);
-#pragma unroll
-        for (int b = 0; b < kQ4TileBlocks; ++b) {
-          if (b >= nb) break;
-          const unsigned char* kv = sm.ring[st] + b * kL4BlockBytes;
+        const unsigned char* tile = sm.ring[st];
+        const uint32_t p_row = smem_u32(&sm.p[buf][(mi & 1) * 8 + ri][(mi >> 1) * 8]);
+        auto block = [&](int b, bool tail) {
+          const unsigned char* kv = tile + b * kL4BlockBytes;
           uint32_t pa[4];
-          ldmatrix_x4(smem_u32(&sm.p[buf][(mi & 1) * 8 + ri][16 * b + (mi >> 1) * 8]), pa[0], pa[1], pa[2], pa[3]);
-          const uint2 w0 = *reinterpret_cast<const uint2*>(kv + off0);
-          const uint2 w1 = *reinterpret_cast<const uint2*>(kv + off1);
-          const uint2 w2 = *reinterpret_cast<const uint2*>(kv + off0 + 2048);
-          const uint2 w3 = *reinterpret_cast<const uint2*>(kv + off1 + 2048);
+          ldmatrix_x4(p_row + 32 * b, pa[0], pa[1], pa[2], pa[3]);
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kv + off0);
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kv + off1);
+          const uint32_t w2 = *reinterpret_cast<const uint32_t*>(kv + off0 + 2048);
+          const uint32_t w3 = *reinterpret_cast<const uint32_t*>(kv + off1 + 2048);
           uint32_t sw = *reinterpret_cast<const uint32_t*>(kv + off_s);
-          if (jt + b == nblk - 1) {
+          if (tail) {
             // tokens past the row's length may hold anything, and P = 0 does not cancel an infinity:
             // give them a finite scale
             const int rem = len - (jt + b) * kL4Tokens;
@@ -605,19 +662,21 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
               if (tq + 4 * i >= rem) sw &= ~(0xffu << (8 * i));
           }
           const Q4ScaleB c01 = q4_scale_b(__byte_perm(sw, 0, 0x4140)), c23 = q4_scale_b(__byte_perm(sw, 0, 0x4342));
+          // even dims of the word are its low half's nibbles, odd ones the high half's
+          const uint32_t e01 = __byte_perm(w0, w1, 0x5410), d01 = __byte_perm(w0, w1, 0x7632);
+          const uint32_t e23 = __byte_perm(w2, w3, 0x5410), d23 = __byte_perm(w2, w3, 0x7632);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // even dims of the word are its low half's nibbles, odd ones the high half's
-            const uint32_t x0 = h ? w0.y : w0.x, x1 = h ? w1.y : w1.x, x2 = h ? w2.y : w2.x, x3 = h ? w3.y : w3.x;
-            const uint32_t e01 = __byte_perm(x0, x1, 0x5410), d01 = __byte_perm(x0, x1, 0x7632);
-            const uint32_t e23 = __byte_perm(x2, x3, 0x5410), d23 = __byte_perm(x2, x3, 0x7632);
-            float(*oo)[4] = o + 8 * h;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              mma_bf16_16816(oo[2 * i], pa, q4_b(e01 >> (4 * i), c01), q4_b(e23 >> (4 * i), c23));
-              mma_bf16_16816(oo[2 * i + 1], pa, q4_b(d01 >> (4 * i), c01), q4_b(d23 >> (4 * i), c23));
-            }
+          for (int i = 0; i < 4; ++i) {
+            mma_bf16_16816(o[2 * i], pa, q4_b(e01 >> (4 * i), c01, m128), q4_b(e23 >> (4 * i), c23, m128));
+            mma_bf16_16816(o[2 * i + 1], pa, q4_b(d01 >> (4 * i), c01, m128), q4_b(d23 >> (4 * i), c23, m128));
           }
+        };
+        if (jt + kQ4TileBlocks < nblk && nb == kQ4TileBlocks) {   // whole blocks only: no branch between them
+#pragma unroll
+          for (int b = 0; b < kQ4TileBlocks; ++b) block(b, false);
+        } else {
+#pragma unroll 1
+          for (int b = 0; b < nb; ++b) block(b, jt + b == nblk - 1);
         }
         __syncwarp();
         if (lane == 0) {
@@ -626,31 +685,29 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
         }
       }
       const int fb = seg & 1;
-      mla_wait(&sm.fin_full[fb], static_cast<uint32_t>((seg >> 1) & 1), s_abort);
-      // columns 2 tq and 2 tq + 1 of the 16 n-tiles: 32 consecutive dims from 128 pv + 32 tq
+      q4_wait(&sm.fin_full[fb], static_cast<uint32_t>((seg >> 1) & 1), s_abort);
+      // columns 2 tq and 2 tq + 1 of the 8 n-tiles: 16 consecutive dims from 64 pv + 16 tq
       if (complete) {
         const float inv[2] = {sm.fin[fb][gq], sm.fin[fb][gq + 8]};
-        bf16* ob = p.o_lat + (static_cast<long long>(r) * kHeads + gq) * 512 + 128 * pv + 32 * tq;
+        bf16* ob = p.o_lat + (static_cast<long long>(r) * kHeads + gq) * 512 + 64 * pv + 16 * tq;
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float i = inv[cc >> 1];
-            uint4 v;
-            v.x = pack_bf16x2(o[8 * h][cc] * i, o[8 * h + 1][cc] * i);
-            v.y = pack_bf16x2(o[8 * h + 2][cc] * i, o[8 * h + 3][cc] * i);
-            v.z = pack_bf16x2(o[8 * h + 4][cc] * i, o[8 * h + 5][cc] * i);
-            v.w = pack_bf16x2(o[8 * h + 6][cc] * i, o[8 * h + 7][cc] * i);
-            *reinterpret_cast<uint4*>(ob + (cc >> 1) * 8 * 512 + 16 * (cc & 1) + 8 * h) = v;
-          }
+        for (int cc = 0; cc < 4; ++cc) {
+          const float i = inv[cc >> 1];
+          uint4 v;
+          v.x = pack_bf16x2(o[0][cc] * i, o[1][cc] * i);
+          v.y = pack_bf16x2(o[2][cc] * i, o[3][cc] * i);
+          v.z = pack_bf16x2(o[4][cc] * i, o[5][cc] * i);
+          v.w = pack_bf16x2(o[6][cc] * i, o[7][cc] * i);
+          *reinterpret_cast<uint4*>(ob + (cc >> 1) * 8 * 512 + 8 * (cc & 1)) = v;
+        }
       } else {
-        float* op = p.o_part + ((c * 2 + mla_slot(S, start)) * kHeads + gq) * 512 + 128 * pv + 32 * tq;
+        float* op = p.o_part + ((c * 2 + mla_slot(S, start)) * kHeads + gq) * 512 + 64 * pv + 16 * tq;
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-          for (int h = 0; h < 4; ++h)
-            *reinterpret_cast<float4*>(op + (cc >> 1) * 8 * 512 + 16 * (cc & 1) + 4 * h) =
-                make_float4(o[4 * h][cc], o[4 * h + 1][cc], o[4 * h + 2][cc], o[4 * h + 3][cc]);
+        for (int cc = 0; cc < 4; ++cc) {
+          float* oc = op + (cc >> 1) * 8 * 512 + 8 * (cc & 1);
+          *reinterpret_cast<float4*>(oc) = make_float4(o[0][cc], o[1][cc], o[2][cc], o[3][cc]);
+          *reinterpret_cast<float4*>(oc + 4) = make_float4(o[4][cc], o[5][cc], o[6][cc], o[7][cc]);
+        }
       }
       __syncwarp();
       if (lane == 0) {
@@ -662,7 +719,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
   }
 
   // ================= merges of the rows this CTA published last (all compute warps)
-  mla_wait(&sm.tk_done, 0, s_abort);
+  q4_wait(&sm.tk_done, 0, s_abort);
   const int n_pend = min(sm.n_pend, 2);
   float* s_m = reinterpret_cast<float*>(sm.ring);   // the drained ring
   for (int pi = 0; pi < n_pend; ++pi) {
