@@ -151,13 +151,15 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   if (!a->x || !a->ids || !a->y || !a->low || (a->adapters > 0 && (!a->a || !a->b || !a->ranks || !a->scales)) ||
       (a->n_base > 0 && !a->base))
     return fail(DSV2_ERR_INVALID, "lora: null pointer");
+  if (a->low_parts < 1 || a->low_parts > 64 || (a->tokens > kLoraTile && !a->order))
+    return fail(DSV2_ERR_INVALID, "lora: low_parts %d (1 .. 64), order is required above %d tokens", a->low_parts, kLoraTile);
   if (!a->token_row && a->ids_len < a->tokens)
     return fail(DSV2_ERR_INVALID, "lora: %d ids for %d tokens (pass token_row)", a->ids_len, a->tokens);
   if (a->k <= 0 || a->n <= 0 || a->rank <= 0 || a->k % 8 || a->n % 8 || a->rank % 8 || a->rank > 128)
     return fail(DSV2_ERR_UNSUPPORTED, "lora: k %d, n %d, rank %d (multiples of 8, rank at most 128)", a->k, a->n, a->rank);
   if (a->y_dtype != DSV2_BF16 && a->y_dtype != DSV2_F32) return fail(DSV2_ERR_UNSUPPORTED, "lora: y dtype %d", a->y_dtype);
   if (!aligned16(a->x) || !aligned16(a->a) || !aligned16(a->b) || !aligned16(a->base) || !aligned16(a->low) ||
-      !aligned16(a->y) || a->x_row_stride % 8 || a->base_part_stride % 4 || a->base_row_stride % 4 ||
+      !aligned16(a->order) || !aligned16(a->y) || a->x_row_stride % 8 || a->base_part_stride % 4 || a->base_row_stride % 4 ||
       a->y_row_stride % (a->y_dtype == DSV2_F32 ? 4 : 8))
     return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
   if (int rc = ensure_init(nullptr)) return rc;
@@ -177,6 +179,8 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   p.n = a->n;
   p.ids_len = a->ids_len;
   p.low = a->low;
+  p.low_parts = a->low_parts;
+  p.order = a->tokens > kLoraTile ? a->order : nullptr;
   p.base = a->base;
   p.base_parts = a->n_base;
   p.base_part_stride = a->base_part_stride;

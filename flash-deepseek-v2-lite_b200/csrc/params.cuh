@@ -172,7 +172,9 @@ struct LoraParams {
   const float* scales;         // [adapters]
   int adapters, rank, tokens, k, n;
   int ids_len;
-  float* low;                  // [tokens, rank] work buffer
+  float* low;                  // [low_parts, tokens, rank] work buffer
+  int low_parts;               // k splits of the first product
+  int* order;                  // [tokens] work buffer: tokens by adapter (nullptr: as they come)
   const float* base;           // optional fp32 partials of the shared projection, summed in order
   int base_parts;
   long long base_part_stride, base_row_stride;

@@ -30,7 +30,9 @@ __all__ = [
 
 
 def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current torch stream of the current device (torch.cuda.current_stream() builds a Stream
+    object first: 3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _cuda(t: torch.Tensor, name: str) -> None:
@@ -550,7 +552,7 @@ def _here(t: torch.Tensor) -> int:
     """The current stream, of the device that t lives on."""
     if t.device.index != torch.cuda.current_device():
         raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream
+    return stream()
 
 
 def latent4_cache(pages: int, page_size: int, device, layers: int | None = None) -> torch.Tensor:
@@ -691,12 +693,13 @@ def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tenso
 
 
 def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, ranks: torch.Tensor,
-         scales: torch.Tensor, y: torch.Tensor, low: torch.Tensor, base: torch.Tensor | None = None,
-         token_row: torch.Tensor | None = None) -> torch.Tensor:
+         scales: torch.Tensor, y: torch.Tensor, low: torch.Tensor, order: torch.Tensor | None = None,
+         base: torch.Tensor | None = None, token_row: torch.Tensor | None = None) -> torch.Tensor:
     """y[t] = sum of base[:, t] + scales[i] * b[i] (a[i] x[t]) with i = ids[token_row[t]] (or
     ids[t]); negative = no adapter.  x bf16 [T, K], a bf16 [adapters, rank, K], b bf16
     [adapters, N, rank], ids int32, ranks int32 and scales fp32 [adapters], y bf16 or fp32
-    [T, N], low fp32 work buffer of T * rank elements, base (optional) fp32 [parts, T, N]."""
+    [T, N], base (optional) fp32 [parts, T, N].  low / order: work buffers (lora_workspace; low
+    fp32 of a multiple of T * rank elements, order int32 [T], not needed up to 16 tokens)."""
     _cuda(x, "x")
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1:
         raise NotImplementedError("x must be bf16 [tokens, k] with a contiguous last dimension")
@@ -712,8 +715,9 @@ def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor
         x.data_ptr(), x.stride(0) if T > 1 else K, _need(a, "a", torch.bfloat16), _need(b, "b", torch.bfloat16),
         _need(ids, "ids", torch.int32), None if token_row is None else _need(token_row, "token_row", torch.int32, T),
         _need(ranks, "ranks", torch.int32, n_ad), _need(scales, "scales", torch.float32, n_ad), None, 0, 0,
-        _need(low, "low", torch.float32, T * rank), y.data_ptr(), y.stride(0) if T > 1 else N,
-        DSV2_F32 if y.dtype == torch.float32 else DSV2_BF16, 0, ids.numel(), n_ad, rank, T, K, N)
+        _need(low, "low", torch.float32, T * rank), None if order is None else _need(order, "order", torch.int32, T),
+        y.data_ptr(), y.stride(0) if T > 1 else N,
+        max(1, min(low.numel() // max(1, T * rank), 64)), DSV2_F32 if y.dtype == torch.float32 else DSV2_BF16, 0, ids.numel(), n_ad, rank, T, K, N)
     if base is not None:
         if base.dim() != 3 or base.dtype != torch.float32 or base.shape[1:] != y.shape or base.stride(2) != 1:
             raise ValueError(f"base must be fp32 [parts, {T}, {N}] with a contiguous last dimension")
@@ -731,7 +735,15 @@ def lora_workspace(tokens: int, n: int, k: int, rank: int, device) -> dict:
     if LORA_GEMV_TOKENS < tokens <= 256:   # decode batches: K split over the SMs, as the engine's projections
         splits = max(1, min(sms // ((n + 127) // 128), k // 64, 5))
     return {"parts": torch.empty((splits, tokens, n), device=device, dtype=torch.float32),
-            "low": torch.empty((tokens, rank), device=device, dtype=torch.float32)}
+            "low": torch.empty((lora_splits(tokens, k, sms), tokens, rank), device=device, dtype=torch.float32),
+            "order": torch.empty(tokens, device=device, dtype=torch.int32)}
+
+
+def lora_splits(tokens: int, k: int, num_sms: int) -> int:
+    """Pieces of k that the adapters' first product runs side by side: about two CTAs (of a tile
+    of 16 tokens) per SM, each with at least 128 of k, at most 16 pieces for the second product
+    to sum."""
+    return max(1, min(2 * num_sms // max(1, (tokens + 15) // 16), k // 128, 16))
 
 
 LORA_GEMV_TOKENS = 8   # up to here lora_linear's shared projection runs the small (GEMV) family
@@ -739,7 +751,7 @@ LORA_GEMV_TOKENS = 8   # up to here lora_linear's shared projection runs the sma
 
 def lora_linear(*, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
                 ranks: torch.Tensor, scales: torch.Tensor, y: torch.Tensor, parts: torch.Tensor, low: torch.Tensor,
-                token_row: torch.Tensor | None = None) -> torch.Tensor:
+                order: torch.Tensor | None = None, token_row: torch.Tensor | None = None) -> torch.Tensor:
     """The shared projection x @ w.T (w bf16 [N, K]) plus every token's low-rank adapter, rounded
     once to y's dtype: y[t] = w x[t] + scales[i] * b[i] (a[i] x[t]); see lora and
     lora_workspace."""
@@ -758,4 +770,5 @@ def lora_linear(*, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     else:
         linear(w=w, n_rows=w.shape[0], k=w.shape[1], x=x, y=parts[0], family=FAMILY_BATCH, epilogue=EPI_STORE_F32,
                n_tokens=T, x_group_rows=T, k_splits=parts.shape[0], y_split_stride=parts.stride(0))
-    return lora(x=x, a=a, b=b, ids=ids, ranks=ranks, scales=scales, y=y, low=low, base=parts, token_row=token_row)
+    return lora(x=x, a=a, b=b, ids=ids, ranks=ranks, scales=scales, y=y, low=low, order=order, base=parts,
+                token_row=token_row)

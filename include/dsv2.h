@@ -672,7 +672,8 @@ DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* strea
  * or token row: no adapter.  base: n_base fp32 partials of the shared projection (dsv2_linear
  * with DSV2_EPI_STORE_F32), 0 = none.  y: y_dtype DSV2_BF16 (one rounding of the fp32 sum) or
  * DSV2_F32 (with n_base = 0 the adapters' part alone, e.g. one more partial of the projection).
- * low: fp32 work buffer [tokens, rank].  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128. */
+ * low: fp32 work buffer [low_parts, tokens, rank] (low_parts >= 1 pieces of k run side by side);
+ * order: int32 work buffer [tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128. */
 typedef struct dsv2_lora_args {
   const void* x;
   int64_t x_row_stride;
@@ -686,8 +687,10 @@ typedef struct dsv2_lora_args {
   int64_t base_part_stride;
   int64_t base_row_stride;
   float* low;
+  int32_t* order;
   void* y;
   int64_t y_row_stride;
+  int32_t low_parts;
   int32_t y_dtype;
   int32_t n_base;
   int32_t ids_len;             /* entries of ids */
