@@ -162,7 +162,8 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
       !aligned16(a->order) || !aligned16(a->y) || a->x_row_stride % 8 || a->base_part_stride % 4 || a->base_row_stride % 4 ||
       a->y_row_stride % (a->y_dtype == DSV2_F32 ? 4 : 8))
     return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
-  if (int rc = ensure_init(nullptr)) return rc;
+  int sms = 0;
+  if (int rc = ensure_init(&sms)) return rc;
   LoraParams p = {};
   p.x = static_cast<const bf16*>(a->x);
   p.x_row_stride = a->x_row_stride;
@@ -188,7 +189,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   p.y = a->y;
   p.y_f32 = a->y_dtype == DSV2_F32;
   p.y_row_stride = a->y_row_stride;
-  return check_launch(launch_lora(p, static_cast<cudaStream_t>(stream)), "lora");
+  return check_launch(launch_lora(p, sms, static_cast<cudaStream_t>(stream)), "lora");
 }
 
 }  // extern "C"

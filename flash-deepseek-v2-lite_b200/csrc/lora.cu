@@ -36,57 +36,81 @@ __device__ __forceinline__ int lora_id(const LoraParams& p, int t) {
   return a < 0 ? -1 : a;
 }
 
-// order[pos] = t with pos = #{u: id_u < id_t} + #{u < t: id_u = id_t}: every pair of tokens is
-// compared once, 16 million at 4096 tokens (about 2 us over the GPU), with no histogram over the
-// adapters, whose number is the caller's.
-__global__ __launch_bounds__(256) void lora_sort_kernel(const LoraParams p) {
+// order[pos] = t, order[tokens + pos] = its adapter and order[2 tokens + pos] the adapter's rank, with pos = #{u: id_u < id_t} + #{u < t: id_u =
+// id_t}: every pair of tokens is compared once (16 million at 4096 tokens), with no histogram over
+// the adapters, whose number is the caller's.  A CTA's warps share 32 tokens: lane = token, warp = a part of
+// the others.
+constexpr int kLoraSortChunk = 4096;
+constexpr int kLoraSortThreads = 1024;
+__global__ __launch_bounds__(kLoraSortThreads) void lora_sort_kernel(const LoraParams p) {
   pdl_enter();
-  __shared__ int s_id[256];
+  __shared__ __align__(16) int s_id[kLoraSortChunk];
+  __shared__ int s_before[kLoraSortThreads];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // 8 warps share a group of 32 tokens: lane = token, warp = an eighth of the others
   const int t = blockIdx.x * 32 + lane;
   const int mine = t < p.tokens ? lora_id(p, t) : 0;
   int before = 0;
-  for (int u0 = 0; u0 < p.tokens; u0 += 256) {
+  for (int u0 = 0; u0 < p.tokens; u0 += kLoraSortChunk) {
     __syncthreads();
-    const int u = u0 + threadIdx.x;
-    s_id[threadIdx.x] = u < p.tokens ? lora_id(p, u) : 0x7fffffff;
+    int v[kLoraSortChunk / kLoraSortThreads];
+#pragma unroll
+    for (int i = 0; i < kLoraSortChunk / kLoraSortThreads; ++i) {
+      const int u = u0 + i * kLoraSortThreads + threadIdx.x;
+      v[i] = u < p.tokens ? lora_id(p, u) : 0x7fffffff;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoraSortChunk / kLoraSortThreads; ++i) s_id[i * kLoraSortThreads + threadIdx.x] = v[i];
     __syncthreads();
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-      const int v = s_id[warp * 32 + i];
-      before += (v < mine || (v == mine && u0 + warp * 32 + i < t)) ? 1 : 0;
+    const int n = min(kLoraSortChunk, p.tokens - u0);
+    const int4* q = reinterpret_cast<const int4*>(s_id);
+    const int rel = t - u0;
+    for (int i = warp; i < (n + 3) / 4; i += kLoraSortThreads / 32) {
+      const int4 w = q[i];
+      // w < mine, or equal and earlier: equal counts when the index is below this token's
+      before += (w.x < mine + (4 * i < rel)) + (w.y < mine + (4 * i + 1 < rel)) + (w.z < mine + (4 * i + 2 < rel)) +
+                (w.w < mine + (4 * i + 3 < rel));
     }
   }
-  __syncthreads();
-  s_id[threadIdx.x] = before;
+  s_before[threadIdx.x] = before;
   __syncthreads();
   if (warp == 0 && t < p.tokens) {
-    for (int w = 1; w < 8; ++w) before += s_id[w * 32 + lane];
+    for (int w = 1; w < kLoraSortThreads / 32; ++w) before += s_before[w * 32 + lane];
     p.order[before] = t;
+    p.order[p.tokens + before] = mine;
+    p.order[2 * p.tokens + before] = mine >= 0 ? min(max(p.ranks[mine], 0), p.rank) : 0;
   }
 }
 
-// The 16 tokens of tile i and their adapters, in shared memory; -2 marks a place without a token.
-__device__ __forceinline__ void lora_tile(const LoraParams& p, int tile, int* s_tok, int* s_ad) {
-  if (threadIdx.x < kLoraTile) {
-    const int i = tile * kLoraTile + threadIdx.x;
-    const int t = i < p.tokens ? (p.order ? p.order[i] : i) : -1;
-    s_tok[threadIdx.x] = t;
-    s_ad[threadIdx.x] = t >= 0 ? lora_id(p, t) : -2;
+// The 16 tokens of a tile and its adapters, in shared memory.
+struct LoraTile {
+  int tok[kLoraTile];    // token of each row, -1 = none
+  int which[kLoraTile];  // the row's adapter as an index into list, -1 = a token without one, -2 = no token
+  int list[kLoraTile];   // the different adapters, their ranks
+  int rank[kLoraTile];
+  int n;
+};
+__device__ __forceinline__ void lora_tile(const LoraParams& p, int tile, LoraTile& s) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, i = tile * kLoraTile + lane;
+    const bool in = lane < kLoraTile && i < p.tokens;
+    const int t = in ? (p.order ? p.order[i] : i) : -1;
+    const int a = in ? (p.order ? p.order[p.tokens + i] : lora_id(p, i)) : -2;
+    const int rank = a < 0 ? 0 : p.order ? p.order[2 * p.tokens + i] : min(max(p.ranks[a], 0), p.rank);
+    const unsigned same = __match_any_sync(0xffffffffu, a);
+    const int leader = __ffs(same) - 1;
+    const unsigned leaders = __ballot_sync(0xffffffffu, a >= 0 && leader == lane);
+    const int idx = __popc(leaders & ((1u << leader) - 1));
+    if (lane < kLoraTile) {
+      s.tok[lane] = t;
+      s.which[lane] = a >= 0 ? idx : a;
+      if (a >= 0 && leader == lane) {
+        s.list[idx] = a;
+        s.rank[idx] = rank;
+      }
+    }
+    if (lane == 0) s.n = __popc(leaders);
   }
   __syncthreads();
-}
-
-// next adapter above `last` in the tile, or a large number
-__device__ __forceinline__ int lora_next(const int* s_ad, int last) {
-  int a = 0x7fffffff;
-#pragma unroll
-  for (int i = 0; i < kLoraTile; ++i) {
-    const int v = s_ad[i];
-    if (v > last) a = min(a, v);
-  }
-  return a;
 }
 
 __device__ __forceinline__ uint4 ld_or_zero(const void* q, bool in) {
@@ -97,25 +121,27 @@ __device__ __forceinline__ uint4 ld_or_zero(const void* q, bool in) {
 template <int NT>
 __global__ __launch_bounds__(kLoraLowWarps * 32) void lora_low_kernel(const LoraParams p) {
   pdl_enter();
-  __shared__ int s_tok[kLoraTile], s_ad[kLoraTile];
+  __shared__ LoraTile s;
   __shared__ float s_sum[kLoraLowWarps][kLoraTile][8 * NT + 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-  lora_tile(p, blockIdx.x, s_tok, s_ad);
+  lora_tile(p, blockIdx.x, s);
   // this CTA's k range, in steps of 32, and this warp's part of it
   const int steps = (p.k + 31) / 32, splits = gridDim.y * kLoraLowWarps, part = blockIdx.y * kLoraLowWarps + warp;
   const int k0 = static_cast<int>(static_cast<long long>(steps) * part / splits) * 32;
   const int k1 = static_cast<int>(static_cast<long long>(steps) * (part + 1) / splits) * 32;
-  const int t0 = s_tok[gq], t1 = s_tok[gq + 8];
+  const int t0 = s.tok[gq], t1 = s.tok[gq + 8];
   const bf16* x0 = p.x + (t0 >= 0 ? t0 : 0) * p.x_row_stride;
   const bf16* x1 = p.x + (t1 >= 0 ? t1 : 0) * p.x_row_stride;
-  for (int a = lora_next(s_ad, -1); a != 0x7fffffff; a = lora_next(s_ad, a)) {
+  // the adapters of a tile are dealt out to the CTAs that share it
+  for (int ai = blockIdx.z; ai < s.n; ai += gridDim.z) {
+    const int a = s.list[ai], rank = s.rank[ai], nt = (rank + 7) / 8;
     const bf16* w = p.a + static_cast<long long>(a) * p.rank * p.k;
-    const int rank = min(max(p.ranks[a], 0), p.rank), nt = (rank + 7) / 8;
+    const float scale = p.scales[a];
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    const bool m0 = s_ad[gq] == a, m1 = s_ad[gq + 8] == a;
-#pragma unroll 2
+    const bool m0 = s.which[gq] == ai, m1 = s.which[gq + 8] == ai;
+#pragma unroll (NT <= 4 ? 4 : 2)
     for (int k = k0 + 8 * tq; k < k1; k += 32) {
       const bool in = k < p.k;
       const uint4 u0 = ld_or_zero(x0 + k, in && m0), u1 = ld_or_zero(x1 + k, in && m1);
@@ -140,141 +166,167 @@ __global__ __launch_bounds__(kLoraLowWarps * 32) void lora_low_kernel(const Lora
       s_sum[warp][gq + 8][8 * n + 2 * tq + 1] = acc[n][3];
     }
     __syncthreads();
-    const float scale = p.scales[a];
     for (int i = threadIdx.x; i < kLoraTile * 8 * NT; i += kLoraLowWarps * 32) {
       const int r = i / (8 * NT), j = i % (8 * NT);
-      if (s_ad[r] != a || j >= p.rank) continue;
+      if (s.which[r] != ai || j >= p.rank) continue;
       float v = 0.f;
 #pragma unroll
       for (int q = 0; q < kLoraLowWarps; ++q) v += s_sum[q][r][j];
       // columns past the adapter's rank hold whatever its padding holds
-      p.low[(static_cast<long long>(blockIdx.y) * p.tokens + s_tok[r]) * p.rank + j] = j < rank ? v * scale : 0.f;
+      p.low[(static_cast<long long>(blockIdx.y) * p.tokens + s.tok[r]) * p.rank + j] = j < rank ? v * scale : 0.f;
     }
   }
 }
 
-// y tile: 16 tokens x 256 columns.  A warp owns 32 columns as two pairs of n-tiles; column 2 q + e of
-// n-tile u of a pair is column 4 q + 2 u + e of its 16, so that a lane ends with 4 consecutive
-// columns: whole sectors of the partials in, of y out.  low is used as the sum of two bf16 numbers
-// (16 significant bits), so that it adds no rounding of its own to y.
-__global__ __launch_bounds__(kLoraOutWarps * 32) void lora_out_kernel(const LoraParams p) {
+// y: a tile of 16 tokens x kChunks blocks of 256 columns.  A warp takes 32 columns as two pairs of
+// n-tiles; column 2 q + e of n-tile u of a pair is column 4 q + 2 u + e of its 16, so that a lane ends
+// with 4 consecutive columns: whole sectors of the partials in, of y out.  low is used as the sum of
+// two bf16 numbers (16 significant bits), so that it adds no rounding of its own to y.  A CTA writes
+// the rows of its adapters (blockIdx.z 0 also those of none).
+template <int kChunks>
+__global__ __launch_bounds__(kLoraOutWarps * 32, 4) void lora_out_kernel(const LoraParams p) {
   pdl_enter();
-  __shared__ int s_tok[kLoraTile], s_ad[kLoraTile];
+  __shared__ LoraTile s;
   __shared__ __align__(16) uint32_t s_hi[kLoraTile][68], s_lo[kLoraTile][68];   // bf16 pairs, up to 128 ranks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-  lora_tile(p, blockIdx.y, s_tok, s_ad);
+  lora_tile(p, blockIdx.y, s);
+  const int z = blockIdx.z, zs = gridDim.z;   // zs is a power of two
+  if (z > 0 && z >= s.n) return;
+  const int ad0 = s.which[gq], ad1 = s.which[gq + 8];
+  // this CTA's rows
+  const bool own0 = ad0 >= 0 ? (ad0 & (zs - 1)) == z : ad0 == -1 && z == 0;
+  const bool own1 = ad1 >= 0 ? (ad1 & (zs - 1)) == z : ad1 == -1 && z == 0;
   // the tile's low rows: the k splits summed in order, as high and low bf16 parts; 0 past the rank
-  const int pairs = (p.rank + 31) / 32 * 16;
-  for (int i = threadIdx.x; i < kLoraTile * pairs; i += kLoraOutWarps * 32) {
-    const int r = i / pairs, j = 2 * (i % pairs);
+  const int shift = p.rank <= 32 ? 4 : p.rank <= 64 ? 5 : 6;   // log2 of the pairs staged per row
+  for (int i = threadIdx.x; i < kLoraTile << shift; i += kLoraOutWarps * 32) {
+    const int r = i >> shift, pair = i & ((1 << shift) - 1), j = 2 * pair;
     float v0 = 0.f, v1 = 0.f;
-    if (s_ad[r] >= 0 && j < p.rank) {
-      for (int q = 0; q < p.low_parts; ++q) {
-        const float2 v = *reinterpret_cast<const float2*>(p.low + (static_cast<long long>(q) * p.tokens + s_tok[r]) * p.rank + j);
+    if (s.which[r] >= 0 && j < p.rank) {
+      const float* src = p.low + static_cast<long long>(s.tok[r]) * p.rank + j;
+      const long long step = static_cast<long long>(p.tokens) * p.rank;
+#pragma unroll 4
+      for (int q = 0; q < p.low_parts; ++q, src += step) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
         v0 += v.x;
         v1 += v.y;
       }
     }
     const uint32_t hi = pack_bf16x2(v0, v1);
-    s_hi[r][i % pairs] = hi;
-    s_lo[r][i % pairs] = pack_bf16x2(v0 - bf16lo(hi), v1 - bf16hi(hi));
-  }
-  const int n0 = blockIdx.x * kLoraOutCols + warp * 32;
-  const int t0 = s_tok[gq], t1 = s_tok[gq + 8];
-  float acc[4][4];   // n-tiles 0, 1: columns n0 .. + 16; 2, 3: + 16 .. + 32
-#pragma unroll
-  for (int u = 0; u < 4; ++u) acc[u][0] = acc[u][1] = acc[u][2] = acc[u][3] = 0.f;
-  // shared projection: 4 consecutive columns of two tokens per pair
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int n = n0 + 16 * h + 4 * tq;
-    if (n >= p.n) continue;
-    for (int q = 0; q < p.base_parts; ++q) {
-      const float* b = p.base + q * p.base_part_stride + n;
-      if (t0 >= 0) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(b + t0 * p.base_row_stride));
-        acc[2 * h][0] += v.x;
-        acc[2 * h][1] += v.y;
-        acc[2 * h + 1][0] += v.z;
-        acc[2 * h + 1][1] += v.w;
-      }
-      if (t1 >= 0) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(b + t1 * p.base_row_stride));
-        acc[2 * h][2] += v.x;
-        acc[2 * h][3] += v.y;
-        acc[2 * h + 1][2] += v.z;
-        acc[2 * h + 1][3] += v.w;
-      }
-    }
+    s_hi[r][pair] = hi;
+    s_lo[r][pair] = pack_bf16x2(v0 - bf16lo(hi), v1 - bf16hi(hi));
   }
   __syncthreads();
-  for (int a = lora_next(s_ad, -1); a != 0x7fffffff; a = lora_next(s_ad, a)) {
-    const int rank = min(max(p.ranks[a], 0), p.rank);
-    const bool m0 = s_ad[gq] == a, m1 = s_ad[gq + 8] == a;
-    for (int j = 0; j < rank; j += 32) {
-      // lane tq takes ranks j + 8 tq .. + 8 (4 words of the staged pairs)
-      const int jw = j / 2 + 4 * tq;
-      uint4 h0 = make_uint4(0, 0, 0, 0), h1 = h0, l0 = h0, l1 = h0;
-      if (m0) {
-        h0 = *reinterpret_cast<const uint4*>(&s_hi[gq][jw]);
-        l0 = *reinterpret_cast<const uint4*>(&s_lo[gq][jw]);
-      }
-      if (m1) {
-        h1 = *reinterpret_cast<const uint4*>(&s_hi[gq + 8][jw]);
-        l1 = *reinterpret_cast<const uint4*>(&s_lo[gq + 8][jw]);
-      }
-      const uint32_t ah0[4] = {h0.x, h1.x, h0.y, h1.y}, ah1[4] = {h0.z, h1.z, h0.w, h1.w};
-      const uint32_t al0[4] = {l0.x, l1.x, l0.y, l1.y}, al1[4] = {l0.z, l1.z, l0.w, l1.w};
-      const int mine = rank - j - 8 * tq;   // ranks of this lane's 8 that exist
-      uint4 b[4];
+  const int col = blockIdx.x * (kChunks * kLoraOutCols) + warp * 32;
+  const float* base0 = p.base + (own0 ? s.tok[gq] * p.base_row_stride : 0) + col + 4 * tq;
+  const float* base1 = p.base + (own1 ? s.tok[gq + 8] * p.base_row_stride : 0) + col + 4 * tq;
+  const long long y0 = (own0 ? s.tok[gq] * p.y_row_stride : 0) + col + 4 * tq;
+  const long long y1 = (own1 ? s.tok[gq + 8] * p.y_row_stride : 0) + col + 4 * tq;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int n = n0 + 16 * (u >> 1) + 4 * (gq >> 1) + 2 * (u & 1) + (gq & 1);
-        b[u] = ld_or_zero(p.b + (static_cast<long long>(a) * p.n + n) * p.rank + j + 8 * tq, n < p.n && mine > 0);
-        if (mine > 0 && mine < 8) {
+  for (int ch = 0; ch < kChunks; ++ch) {
+    const int n0 = col + ch * kLoraOutCols;
+    if (n0 >= p.n) break;
+    // shared projection: 4 consecutive columns of two tokens per pair of n-tiles
+    float4 v[2][2];   // [pair][token]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) v[h][0] = v[h][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool in0 = n0 + 4 * tq < p.n, in1 = n0 + 16 + 4 * tq < p.n;
+    const float *q0 = base0 + ch * kLoraOutCols, *q1 = base1 + ch * kLoraOutCols;
+    for (int q = 0; q < p.base_parts; ++q, q0 += p.base_part_stride, q1 += p.base_part_stride) {
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 x00 = own0 && in0 ? __ldcg(reinterpret_cast<const float4*>(q0)) : zero;
+      const float4 x10 = own0 && in1 ? __ldcg(reinterpret_cast<const float4*>(q0 + 16)) : zero;
+      const float4 x01 = own1 && in0 ? __ldcg(reinterpret_cast<const float4*>(q1)) : zero;
+      const float4 x11 = own1 && in1 ? __ldcg(reinterpret_cast<const float4*>(q1 + 16)) : zero;
+      v[0][0] = make_float4(v[0][0].x + x00.x, v[0][0].y + x00.y, v[0][0].z + x00.z, v[0][0].w + x00.w);
+      v[1][0] = make_float4(v[1][0].x + x10.x, v[1][0].y + x10.y, v[1][0].z + x10.z, v[1][0].w + x10.w);
+      v[0][1] = make_float4(v[0][1].x + x01.x, v[0][1].y + x01.y, v[0][1].z + x01.z, v[0][1].w + x01.w);
+      v[1][1] = make_float4(v[1][1].x + x11.x, v[1][1].y + x11.y, v[1][1].z + x11.z, v[1][1].w + x11.w);
+    }
+    float acc[4][4];   // n-tiles 0, 1: columns n0 .. + 16; 2, 3: + 16 .. + 32
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      acc[2 * h][0] = v[h][0].x;
+      acc[2 * h][1] = v[h][0].y;
+      acc[2 * h + 1][0] = v[h][0].z;
+      acc[2 * h + 1][1] = v[h][0].w;
+      acc[2 * h][2] = v[h][1].x;
+      acc[2 * h][3] = v[h][1].y;
+      acc[2 * h + 1][2] = v[h][1].z;
+      acc[2 * h + 1][3] = v[h][1].w;
+    }
+    const int nb = n0 + 4 * (gq >> 1) + (gq & 1);   // row of B of column gq of n-tile 0; + 2, + 16, + 18
+    for (int ai = z; ai < s.n; ai += zs) {
+      const int rank = s.rank[ai];
+      const bf16* src = p.b + (static_cast<long long>(s.list[ai]) * p.n + nb) * p.rank + 8 * tq;
+      for (int j = 0; j < rank; j += 32, src += 32) {
+        // lane tq takes ranks j + 8 tq .. + 8 of four rows of B
+        const int have = rank - j - 8 * tq;   // ranks of this lane's 8 that exist
+        uint4 b[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int dn = 16 * (u >> 1) + 2 * (u & 1);
+          b[u] = ld_or_zero(src + dn * p.rank, have > 0 && nb + dn < p.n);
+        }
+        if (have > 0 && have < 8) {
           // padding past the rank may be anything, and 0 * NaN is not 0
-          uint32_t* bw = reinterpret_cast<uint32_t*>(&b[u]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (2 * i >= mine) bw[i] = 0;
-            else if (2 * i + 1 >= mine) bw[i] &= 0xffffu;
+          for (int u = 0; u < 4; ++u) {
+            uint32_t* bw = reinterpret_cast<uint32_t*>(&b[u]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (2 * i >= have) bw[i] = 0;
+              else if (2 * i + 1 >= have) bw[i] &= 0xffffu;
+            }
           }
         }
-      }
+        const int jw = j / 2 + 4 * tq;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const uint4 h0 = ad0 == ai ? *reinterpret_cast<const uint4*>(&s_hi[gq][jw]) : zero;
+        const uint4 h1 = ad1 == ai ? *reinterpret_cast<const uint4*>(&s_hi[gq + 8][jw]) : zero;
+        const uint4 l0 = ad0 == ai ? *reinterpret_cast<const uint4*>(&s_lo[gq][jw]) : zero;
+        const uint4 l1 = ad1 == ai ? *reinterpret_cast<const uint4*>(&s_lo[gq + 8][jw]) : zero;
+        const uint32_t ah0[4] = {h0.x, h1.x, h0.y, h1.y}, ah1[4] = {h0.z, h1.z, h0.w, h1.w};
+        const uint32_t al0[4] = {l0.x, l1.x, l0.y, l1.y}, al1[4] = {l0.z, l1.z, l0.w, l1.w};
+        __syncwarp();
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        mma_bf16_16816(acc[u], ah0, b[u].x, b[u].y);
-        mma_bf16_16816(acc[u], al0, b[u].x, b[u].y);
-        mma_bf16_16816(acc[u], ah1, b[u].z, b[u].w);
-        mma_bf16_16816(acc[u], al1, b[u].z, b[u].w);
+        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], ah0, b[u].x, b[u].y);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], al0, b[u].x, b[u].y);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], ah1, b[u].z, b[u].w);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], al1, b[u].z, b[u].w);
       }
     }
-  }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int n = n0 + 16 * h + 4 * tq;
-    if (n >= p.n) continue;
+    for (int h = 0; h < 2; ++h) {
+      if (!(h ? in1 : in0)) continue;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int t = c ? t1 : t0;
-      if (t < 0) continue;
-      const float v0 = acc[2 * h][2 * c], v1 = acc[2 * h][2 * c + 1], v2 = acc[2 * h + 1][2 * c], v3 = acc[2 * h + 1][2 * c + 1];
-      const long long off = t * p.y_row_stride + n;
-      if (p.y_f32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + off) = make_float4(v0, v1, v2, v3);
-      else *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(p.y) + off) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
+      for (int c = 0; c < 2; ++c) {
+        if (!(c ? own1 : own0)) continue;
+        const float v0 = acc[2 * h][2 * c], v1 = acc[2 * h][2 * c + 1], v2 = acc[2 * h + 1][2 * c], v3 = acc[2 * h + 1][2 * c + 1];
+        const long long off = (c ? y1 : y0) + ch * kLoraOutCols + 16 * h;
+        if (p.y_f32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + off) = make_float4(v0, v1, v2, v3);
+        else *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(p.y) + off) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
+      }
     }
   }
 }
 
-cudaError_t launch_lora(const LoraParams& p, cudaStream_t st) {
+// Launch shapes.  A tile of few tokens can hold many adapters: with few tiles they are dealt out to
+// 4 CTAs.  With many tiles a CTA of the second product takes 512 columns, which share its set-up.
+cudaError_t launch_lora(const LoraParams& p, int num_sms, cudaStream_t st) {
   const int tiles = (p.tokens + kLoraTile - 1) / kLoraTile;
-  if (p.order) launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, 256, 0, st, p);
-  const dim3 grid(tiles, p.low_parts), block(kLoraLowWarps * 32);
+  const int deal = p.tokens > 1 && tiles < num_sms / 4 ? 4 : 1;
+  if (p.order) launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, kLoraSortThreads, 0, st, p);
+  const dim3 grid(tiles, p.low_parts, deal), block(kLoraLowWarps * 32);
   if (p.rank <= 16) launch_kernel(lora_low_kernel<2>, grid, block, 0, st, p);
   else if (p.rank <= 32) launch_kernel(lora_low_kernel<4>, grid, block, 0, st, p);
   else if (p.rank <= 64) launch_kernel(lora_low_kernel<8>, grid, block, 0, st, p);
   else launch_kernel(lora_low_kernel<16>, grid, block, 0, st, p);
-  launch_kernel(lora_out_kernel, dim3((p.n + kLoraOutCols - 1) / kLoraOutCols, tiles), kLoraOutWarps * 32, 0, st, p);
+  const unsigned cols = (p.n + kLoraOutCols - 1) / kLoraOutCols;
+  if (tiles >= num_sms) launch_kernel(lora_out_kernel<2>, dim3((cols + 1) / 2, tiles), kLoraOutWarps * 32, 0, st, p);
+  else launch_kernel(lora_out_kernel<1>, dim3(cols, tiles, deal), kLoraOutWarps * 32, 0, st, p);
   return cudaGetLastError();
 }
 

@@ -174,7 +174,7 @@ struct LoraParams {
   int ids_len;
   float* low;                  // [low_parts, tokens, rank] work buffer
   int low_parts;               // k splits of the first product
-  int* order;                  // [tokens] work buffer: tokens by adapter (nullptr: as they come)
+  int* order;                  // [3, tokens] work buffer: tokens by adapter, adapters, ranks (nullptr: as they come)
   const float* base;           // optional fp32 partials of the shared projection, summed in order
   int base_parts;
   long long base_part_stride, base_row_stride;
@@ -249,7 +249,7 @@ cudaError_t launch_latent4_read(const Latent4Params&, cudaStream_t);
 cudaError_t launch_page_plan(const PagePlanParams&, int num_sms, cudaStream_t);
 cudaError_t mla_q4_init();
 cudaError_t launch_mla_q4(const MlaQ4Params&, int num_sms, cudaStream_t);
-cudaError_t launch_lora(const LoraParams&, cudaStream_t);
+cudaError_t launch_lora(const LoraParams&, int num_sms, cudaStream_t);
 cudaError_t mla_decode_init();
 int mla_decode_grid(const MlaDecodeParams&, int num_sms, long long part_slots);
 cudaError_t launch_mla_decode(const MlaDecodeParams&, const CUtensorMap& tm_kv, const CUtensorMap& tm_qa,

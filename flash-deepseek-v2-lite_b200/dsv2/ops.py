@@ -699,7 +699,7 @@ def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor
     ids[t]); negative = no adapter.  x bf16 [T, K], a bf16 [adapters, rank, K], b bf16
     [adapters, N, rank], ids int32, ranks int32 and scales fp32 [adapters], y bf16 or fp32
     [T, N], base (optional) fp32 [parts, T, N].  low / order: work buffers (lora_workspace; low
-    fp32 of a multiple of T * rank elements, order int32 [T], not needed up to 16 tokens)."""
+    fp32 of a multiple of T * rank elements, order int32 [3, T], not needed up to 16 tokens)."""
     _cuda(x, "x")
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1:
         raise NotImplementedError("x must be bf16 [tokens, k] with a contiguous last dimension")
@@ -715,7 +715,7 @@ def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor
         x.data_ptr(), x.stride(0) if T > 1 else K, _need(a, "a", torch.bfloat16), _need(b, "b", torch.bfloat16),
         _need(ids, "ids", torch.int32), None if token_row is None else _need(token_row, "token_row", torch.int32, T),
         _need(ranks, "ranks", torch.int32, n_ad), _need(scales, "scales", torch.float32, n_ad), None, 0, 0,
-        _need(low, "low", torch.float32, T * rank), None if order is None else _need(order, "order", torch.int32, T),
+        _need(low, "low", torch.float32, T * rank), None if order is None else _need(order, "order", torch.int32, 3 * T),
         y.data_ptr(), y.stride(0) if T > 1 else N,
         max(1, min(low.numel() // max(1, T * rank), 64)), DSV2_F32 if y.dtype == torch.float32 else DSV2_BF16, 0, ids.numel(), n_ad, rank, T, K, N)
     if base is not None:
@@ -736,14 +736,14 @@ def lora_workspace(tokens: int, n: int, k: int, rank: int, device) -> dict:
         splits = max(1, min(sms // ((n + 127) // 128), k // 64, 5))
     return {"parts": torch.empty((splits, tokens, n), device=device, dtype=torch.float32),
             "low": torch.empty((lora_splits(tokens, k, sms), tokens, rank), device=device, dtype=torch.float32),
-            "order": torch.empty(tokens, device=device, dtype=torch.int32)}
+            "order": torch.empty((3, tokens), device=device, dtype=torch.int32)}
 
 
 def lora_splits(tokens: int, k: int, num_sms: int) -> int:
-    """Pieces of k that the adapters' first product runs side by side: about two CTAs (of a tile
-    of 16 tokens) per SM, each with at least 128 of k, at most 16 pieces for the second product
+    """Pieces of k that the adapters' first product runs side by side: about six CTAs (of a tile
+    of 16 tokens) per SM, each with at least 256 of k, at most 16 pieces for the second product
     to sum."""
-    return max(1, min(2 * num_sms // max(1, (tokens + 15) // 16), k // 128, 16))
+    return max(1, min(6 * num_sms // max(1, (tokens + 15) // 16), k // 256, 16))
 
 
 LORA_GEMV_TOKENS = 8   # up to here lora_linear's shared projection runs the small (GEMV) family

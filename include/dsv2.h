@@ -673,7 +673,7 @@ DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* strea
  * with DSV2_EPI_STORE_F32), 0 = none.  y: y_dtype DSV2_BF16 (one rounding of the fp32 sum) or
  * DSV2_F32 (with n_base = 0 the adapters' part alone, e.g. one more partial of the projection).
  * low: fp32 work buffer [low_parts, tokens, rank] (low_parts >= 1 pieces of k run side by side);
- * order: int32 work buffer [tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128. */
+ * order: int32 work buffer [3 * tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128. */
 typedef struct dsv2_lora_args {
   const void* x;
   int64_t x_row_stride;

@@ -483,7 +483,7 @@ def test_lora_alone_strided_and_by_request(D, T):
     y = torch.full((T, 208), 5.0, device=DEV)
     low = torch.empty(T * 16, device=DEV)
     D.lora(x=x[:, 8:264], a=c["a"].to(DEV), b=c["b"].to(DEV), ids=by_req.to(DEV), token_row=token_row.to(DEV),
-           ranks=c["ranks"].to(DEV), scales=c["scales"].to(DEV), y=y[:, :200], low=low, order=torch.empty(T, dtype=torch.int32, device=DEV))
+           ranks=c["ranks"].to(DEV), scales=c["scales"].to(DEV), y=y[:, :200], low=low, order=torch.empty(3 * T, dtype=torch.int32, device=DEV))
     check_lora(y[:, :200], c, w=False, out_bits=20)
     assert bool((y[:, 200:] == 5).all())
     assert not bool(y[:, :200][c["ids"].to(DEV) < 0].any())
