@@ -4,6 +4,8 @@
 
 namespace {
 
+// up to here a shared projection with one partial runs the small (GEMV) family
+constexpr int kLoraGemvTokens = 8;
 constexpr int kQ4MinUnits = 4;   // 64 positions: shorter pieces cost more in merges than they save
 
 // rows of a latent4 call: [n, 576] bf16 with 16-byte aligned rows
@@ -148,6 +150,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   if (a->tokens < 0 || a->adapters < 0 || a->n_base < 0 || a->ids_len < 0)
     return fail(DSV2_ERR_INVALID, "lora: tokens %d adapters %d partials %d", a->tokens, a->adapters, a->n_base);
   if (a->tokens == 0) return DSV2_OK;
+  if (a->w && (!a->base || a->n_base < 1)) return fail(DSV2_ERR_INVALID, "lora: w needs base and n_base for its partials");
   if (!a->x || !a->ids || !a->y || !a->low || (a->adapters > 0 && (!a->a || !a->b || !a->ranks || !a->scales)) ||
       (a->n_base > 0 && !a->base))
     return fail(DSV2_ERR_INVALID, "lora: null pointer");
@@ -164,6 +167,26 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
     return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
   int sms = 0;
   if (int rc = ensure_init(&sms)) return rc;
+  if (a->w) {
+    dsv2_linear_args l = {};
+    l.w = a->w;
+    l.w_row_stride = a->w_row_stride;
+    l.n_rows = a->n;
+    l.k = a->k;
+    l.x = a->x;
+    l.x_row_stride = a->x_row_stride;
+    l.y = const_cast<float*>(a->base);
+    l.y_row_stride = a->base_row_stride;
+    l.epilogue = DSV2_EPI_STORE_F32;
+    l.n_groups = 1;
+    l.n_tokens = a->tokens;
+    l.w_group_rows = a->n;
+    l.x_group_rows = a->tokens;
+    l.k_splits = a->n_base;
+    l.y_split_stride = a->base_part_stride;
+    const bool small = a->tokens <= kLoraGemvTokens && a->n_base == 1;
+    if (int rc = dsv2_linear(&l, small ? DSV2_FAMILY_SMALL : DSV2_FAMILY_BATCH, stream)) return rc;
+  }
   LoraParams p = {};
   p.x = static_cast<const bf16*>(a->x);
   p.x_row_stride = a->x_row_stride;

@@ -131,7 +131,7 @@ class MlaDecodeQ4Args(ctypes.Structure):
 class LoraArgs(ctypes.Structure):
     _fields_ = [
         ("x", c_vp), ("x_row_stride", c_i64), ("a", c_vp), ("b", c_vp), ("ids", c_vp), ("token_row", c_vp),
-        ("ranks", c_vp), ("scales", c_vp), ("base", c_vp), ("base_part_stride", c_i64),
+        ("ranks", c_vp), ("scales", c_vp), ("w", c_vp), ("w_row_stride", c_i64), ("base", c_vp), ("base_part_stride", c_i64),
         ("base_row_stride", c_i64), ("low", c_vp), ("order", c_vp), ("y", c_vp),
         ("y_row_stride", c_i64), ("low_parts", c_i32), ("y_dtype", c_i32), ("n_base", c_i32), ("ids_len", c_i32), ("adapters", c_i32), ("rank", c_i32),
         ("tokens", c_i32), ("k", c_i32), ("n", c_i32),
@@ -225,7 +225,9 @@ def check(rc: int, what: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args), name)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc:
+        check(rc, name)
 
 
 def peer_alloc(nbytes: int) -> int:

@@ -537,11 +537,11 @@ L4_BLOCK_BYTES = 6400    # its bytes (include/dsv2.h describes them)
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int | None = None) -> int:
     """Address of a contiguous CUDA tensor of this dtype (and at least numel elements) on the
     current device."""
-    if not t.is_cuda:
-        raise NotImplementedError(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if not t.is_contiguous():
+    if not (t.is_cuda and t.dtype is dtype and t.is_contiguous()):
+        if not t.is_cuda:
+            raise NotImplementedError(f"{name} must be a CUDA tensor")
+        if t.dtype is not dtype:
+            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
         raise NotImplementedError(f"{name} must be contiguous")
     if numel is not None and t.numel() < numel:
         raise ValueError(f"{name} holds {t.numel()} elements, {numel} needed")
@@ -550,9 +550,10 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int | None = No
 
 def _here(t: torch.Tensor) -> int:
     """The current stream, of the device that t lives on."""
-    if t.device.index != torch.cuda.current_device():
+    dev = t.get_device()
+    if dev != torch.cuda.current_device():
         raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return stream()
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def latent4_cache(pages: int, page_size: int, device, layers: int | None = None) -> torch.Tensor:
@@ -670,11 +671,10 @@ def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tenso
     query row r attends positions 0 .. positions[r] of block-table row seq_rows[r] (default r);
     position -1 or a negative seq_rows entry gives a row of zeros.  Buffers: mla_q4_workspace."""
     rows = q_abs.shape[0]
-    if tuple(q_abs.shape) != (rows, 16, 512) or tuple(q_pe.shape) != (rows, 16, 64) or o_lat.shape != q_abs.shape:
+    if q_abs.shape != (rows, 16, 512) or q_pe.shape != (rows, 16, 64) or o_lat.shape != (rows, 16, 512):
         raise ValueError("q_abs and o_lat must be [rows, 16, 512] and q_pe [rows, 16, 64]")
-    for name, t in (("q_abs", q_abs), ("q_pe", q_pe), ("o_lat", o_lat)):
-        if t.dtype != torch.bfloat16:
-            raise NotImplementedError(f"mla_decode_q4 supports bf16 only ({name} is {t.dtype})")
+    if not (q_abs.dtype is q_pe.dtype is o_lat.dtype is torch.bfloat16):
+        raise NotImplementedError("mla_decode_q4 supports bf16 queries and outputs only")
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
         raise NotImplementedError("block_table must be int32 [sequences, width] with contiguous rows")
     _cuda(block_table, "block_table")
@@ -692,6 +692,39 @@ def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tenso
     return o_lat
 
 
+def _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, base, token_row) -> None:
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1 or not x.is_cuda:
+        raise NotImplementedError("x must be a CUDA bf16 tensor [tokens, k] with a contiguous last dimension")
+    T, K = x.shape
+    if a.dim() != 3 or b.dim() != 3:
+        raise ValueError("a must be [adapters, rank, k] and b [adapters, n, rank]")
+    n_ad, rank, ka = a.shape
+    nb, N, rb = b.shape
+    if ka != K or nb != n_ad or rb != rank:
+        raise ValueError(f"a must be [adapters, rank, {K}] and b [adapters, n, rank]")
+    if y.shape != (T, N) or y.stride(1) != 1 or not y.is_cuda:
+        raise ValueError(f"y must be a CUDA tensor [{T}, {N}] with a contiguous last dimension")
+    y_dt = {torch.bfloat16: DSV2_BF16, torch.float32: DSV2_F32}.get(y.dtype)
+    if y_dt is None:
+        raise NotImplementedError(f"lora output dtype {y.dtype}")
+    base_ptr, base_ps, base_rs, n_base = None, 0, 0, 0
+    if base is not None:
+        if base.dim() != 3 or base.dtype != torch.float32 or base.shape[1:] != y.shape or base.stride(2) != 1:
+            raise ValueError(f"base must be fp32 [parts, {T}, {N}] with a contiguous last dimension")
+        _cuda(base, "base")
+        n_base, base_ps, base_rs = base.shape[0], base.stride(0), base.stride(1)
+        base_ptr = base.data_ptr()
+    args = LoraArgs(
+        x.data_ptr(), x.stride(0) if T > 1 else K, _need(a, "a", torch.bfloat16), _need(b, "b", torch.bfloat16),
+        _need(ids, "ids", torch.int32), None if token_row is None else _need(token_row, "token_row", torch.int32, T),
+        _need(ranks, "ranks", torch.int32, n_ad), _need(scales, "scales", torch.float32, n_ad),
+        None if w is None else w.data_ptr(), 0 if w is None else w.stride(0), base_ptr, base_ps, base_rs,
+        _need(low, "low", torch.float32, T * rank), None if order is None else _need(order, "order", torch.int32, 3 * T),
+        y.data_ptr(), y.stride(0) if T > 1 else N, max(1, min(low.numel() // max(1, T * rank), 64)), y_dt, n_base,
+        ids.numel(), n_ad, rank, T, K, N)
+    _lib.call("dsv2_lora", ctypes.byref(args), _here(x))
+
+
 def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, ranks: torch.Tensor,
          scales: torch.Tensor, y: torch.Tensor, low: torch.Tensor, order: torch.Tensor | None = None,
          base: torch.Tensor | None = None, token_row: torch.Tensor | None = None) -> torch.Tensor:
@@ -700,31 +733,7 @@ def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor
     [adapters, N, rank], ids int32, ranks int32 and scales fp32 [adapters], y bf16 or fp32
     [T, N], base (optional) fp32 [parts, T, N].  low / order: work buffers (lora_workspace; low
     fp32 of a multiple of T * rank elements, order int32 [3, T], not needed up to 16 tokens)."""
-    _cuda(x, "x")
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1:
-        raise NotImplementedError("x must be bf16 [tokens, k] with a contiguous last dimension")
-    T, K = x.shape
-    if a.dim() != 3 or b.dim() != 3 or a.shape[2] != K or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[1]:
-        raise ValueError(f"a must be [adapters, rank, {K}] and b [adapters, n, rank]")
-    n_ad, rank, N = a.shape[0], a.shape[1], b.shape[1]
-    if tuple(y.shape) != (T, N) or y.stride(1) != 1 or not y.is_cuda:
-        raise ValueError(f"y must be a CUDA tensor [{T}, {N}] with a contiguous last dimension")
-    if y.dtype not in (torch.bfloat16, torch.float32):
-        raise NotImplementedError(f"lora output dtype {y.dtype}")
-    args = LoraArgs(
-        x.data_ptr(), x.stride(0) if T > 1 else K, _need(a, "a", torch.bfloat16), _need(b, "b", torch.bfloat16),
-        _need(ids, "ids", torch.int32), None if token_row is None else _need(token_row, "token_row", torch.int32, T),
-        _need(ranks, "ranks", torch.int32, n_ad), _need(scales, "scales", torch.float32, n_ad), None, 0, 0,
-        _need(low, "low", torch.float32, T * rank), None if order is None else _need(order, "order", torch.int32, 3 * T),
-        y.data_ptr(), y.stride(0) if T > 1 else N,
-        max(1, min(low.numel() // max(1, T * rank), 64)), DSV2_F32 if y.dtype == torch.float32 else DSV2_BF16, 0, ids.numel(), n_ad, rank, T, K, N)
-    if base is not None:
-        if base.dim() != 3 or base.dtype != torch.float32 or base.shape[1:] != y.shape or base.stride(2) != 1:
-            raise ValueError(f"base must be fp32 [parts, {T}, {N}] with a contiguous last dimension")
-        _cuda(base, "base")
-        args.base, args.base_part_stride, args.base_row_stride = base.data_ptr(), base.stride(0), base.stride(1)
-        args.n_base = base.shape[0]
-    _lib.call("dsv2_lora", ctypes.byref(args), _here(x))
+    _lora_call(x, None, a, b, ids, ranks, scales, y, low, order, base, token_row)
     return y
 
 
@@ -755,20 +764,9 @@ def lora_linear(*, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     """The shared projection x @ w.T (w bf16 [N, K]) plus every token's low-rank adapter, rounded
     once to y's dtype: y[t] = w x[t] + scales[i] * b[i] (a[i] x[t]); see lora and
     lora_workspace."""
-    if w.dim() != 2 or w.dtype != torch.bfloat16 or w.stride(1) != 1 or not w.is_cuda or x.dtype != torch.bfloat16:
-        raise NotImplementedError("lora_linear supports bf16 x [T, K] and CUDA w [N, K] with contiguous rows")
-    T = x.shape[0]
-    if x.dim() != 2 or w.shape[1] != x.shape[1] or tuple(parts.shape[1:]) != (T, w.shape[0]) or b.shape[1] != w.shape[0]:
-        raise ValueError("lora_linear: inconsistent shapes of x, w, b and parts")
-    _need(parts, "parts", torch.float32)
-    if T == 0:
-        return y
-    if T <= LORA_GEMV_TOKENS:
-        linear(w=w, n_rows=w.shape[0], k=w.shape[1], x=x, y=parts[0], family=FAMILY_SMALL, epilogue=EPI_STORE_F32,
-               n_tokens=T, x_group_rows=T)
-        parts = parts[:1]
-    else:
-        linear(w=w, n_rows=w.shape[0], k=w.shape[1], x=x, y=parts[0], family=FAMILY_BATCH, epilogue=EPI_STORE_F32,
-               n_tokens=T, x_group_rows=T, k_splits=parts.shape[0], y_split_stride=parts.stride(0))
-    return lora(x=x, a=a, b=b, ids=ids, ranks=ranks, scales=scales, y=y, low=low, order=order, base=parts,
-                token_row=token_row)
+    if w.dim() != 2 or w.dtype != torch.bfloat16 or w.stride(1) != 1 or not w.is_cuda:
+        raise NotImplementedError("lora_linear supports a CUDA bf16 w [N, K] with contiguous rows")
+    if w.shape[1] != x.shape[-1] or w.shape[0] != y.shape[-1]:
+        raise ValueError("lora_linear: inconsistent shapes of x, w and y")
+    _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, parts, token_row)
+    return y

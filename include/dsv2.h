@@ -669,8 +669,10 @@ DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* strea
  *   y[t, :] = sum_i base[i, t, :] + scales[a] * B_a (A_a x[t]),   a = ids[token_row ? token_row[t] : t]
  * a: [adapters, rank, k], b: [adapters, n, rank] bf16 contiguous; of adapter a the first
  * ranks[a] of its `rank` rows are used (the rest are not read into the result).  A negative id
- * or token row: no adapter.  base: n_base fp32 partials of the shared projection (dsv2_linear
- * with DSV2_EPI_STORE_F32), 0 = none.  y: y_dtype DSV2_BF16 (one rounding of the fp32 sum) or
+ * or token row: no adapter.  base: n_base fp32 partials of the shared projection, 0 = none; with w
+ * ([n, k] bf16 rows at w_row_stride) they are computed here (base is then a work buffer and n_base
+ * the number of pieces of k, as dsv2_linear's k_splits), else they are the caller's (dsv2_linear
+ * with DSV2_EPI_STORE_F32).  y: y_dtype DSV2_BF16 (one rounding of the fp32 sum) or
  * DSV2_F32 (with n_base = 0 the adapters' part alone, e.g. one more partial of the projection).
  * low: fp32 work buffer [low_parts, tokens, rank] (low_parts >= 1 pieces of k run side by side);
  * order: int32 work buffer [3 * tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128. */
@@ -683,6 +685,8 @@ typedef struct dsv2_lora_args {
   const int32_t* token_row;
   const int32_t* ranks;
   const float* scales;
+  const void* w;
+  int64_t w_row_stride;
   const float* base;
   int64_t base_part_stride;
   int64_t base_row_stride;

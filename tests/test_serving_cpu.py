@@ -110,12 +110,12 @@ def test_lora_refusals():
     from dsv2 import _lib
 
     def args(**kw):
-        a = _lib.LoraArgs(4096, 64, 4096, 4096, 4096, None, 4096, 4096, None, 0, 0, 4096, None, 4096, 16, 1, 0, 0, 3, 2, 8, 3, 64, 16)
+        a = _lib.LoraArgs(4096, 64, 4096, 4096, 4096, None, 4096, 4096, None, 0, None, 0, 0, 4096, None, 4096, 16, 1, 0, 0, 3, 2, 8, 3, 64, 16)
         for k, v in kw.items():
             setattr(a, k, v)
         return ctypes.byref(a), None
     for kw in (dict(x=None), dict(y=None), dict(a=None), dict(low=None), dict(n_base=1), dict(ids_len=2), dict(x=4104),
-               dict(x_row_stride=60), dict(y_row_stride=20), dict(tokens=-1), dict(adapters=-1), dict(low_parts=0),
+               dict(x_row_stride=60), dict(y_row_stride=20), dict(tokens=-1), dict(adapters=-1), dict(low_parts=0), dict(w=4096),
                dict(tokens=17, ids_len=17)):
         with pytest.raises(ValueError):
             _call("dsv2_lora", *args(**kw))
