@@ -14,6 +14,11 @@ RMSNorm, and the two shared experts run inside the grouped MoE launch.  With
 world > 1 the routed experts are sharded across ranks (expert parallel) and the
 batch rows across ranks (attention data parallel); the MoE activations are
 all-gathered and the expert outputs reduce-scattered with NCCL inside the graph.
+
+kv_format="int4" keeps the latent cache in 4 bits in pages (dsv2.serving.PagedCache4): every
+step first plans its pages and slots on the device, then quantises the new rows into them and
+attends over the pages.  adapters= adds each request's low-rank adapter to the query + latent
+and the output projection.  Both are for one rank.
 """
 from __future__ import annotations
 
@@ -22,7 +27,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import ops
+from . import ops, serving
 from .expert_parallel import ep_shard, gather_routing, scatter_sum
 from .model import (HIDDEN, KV_LORA, LATENT_ROW, N_HEADS, QK_NOPE, QKVA_ROWS, Q_DIM, SLOTS, TOPK,
                     V_DIM, LayerPack, check_config, pack_layer, rope_tables)
@@ -86,7 +91,9 @@ class DecodeEngine:
     def __init__(self, model, batch: int, max_len: int, family: str = "batch", *,
                  rank: int = 0, world: int = 1, group=None, gate_bias: torch.Tensor | None = None,
                  alias_hf: bool = True, fused_moe: bool = True, keep_logits: bool = False,
-                 cache: torch.Tensor | None = None):
+                 cache: torch.Tensor | None = None, kv_format: str = "bf16", page_size: int = 64,
+                 pages: int | None = None, adapters: serving.Adapters | None = None,
+                 plan: serving.PagePlan | None = None):
         cfg = model.config
         check_config(cfg)
         if family not in FAMILIES:
@@ -105,6 +112,14 @@ class DecodeEngine:
         self.defer_mla_merge = True
         self._gate_bias = gate_bias
         self.keep_logits = keep_logits   # also materialise the bf16 logits every step
+        if kv_format not in ("bf16", "int4"):
+            raise ValueError(f"unknown kv_format {kv_format!r} (bf16 or int4)")
+        if world > 1 and (kv_format == "int4" or adapters is not None):
+            raise NotImplementedError("the paged 4-bit cache and adapters are for one rank")
+        self.kv_format = "int4" if plan is not None else kv_format
+        self.page_size, self._pages = page_size, pages
+        self.plan = plan                     # given: rows are the plan's tokens (kernel prefill)
+        self.adapters = adapters
         # cache given: rows of this engine are tokens of the cache's sequences (kernel
         # prefill); cache_rows[b] names the sequence of row b
         self._external_cache = cache
@@ -129,6 +144,8 @@ class DecodeEngine:
         self.split_len = choose_split_len(self.B, self.max_len, self.num_sms)
         self.n_splits = ops.mla_splits(self.B, self.max_len, self.split_len, self.num_sms)
         self._alloc()
+        if adapters is not None and len(adapters.layers) != self.L:
+            raise ValueError(f"adapters for {len(adapters.layers)} layers, the model has {self.L}")
         self.graph = None
         self._saved = None
 
@@ -136,7 +153,16 @@ class DecodeEngine:
     def _alloc(self):
         B, dev, bf = self.B, self.dev, torch.bfloat16
         f32, i32, i64 = torch.float32, torch.int32, torch.int64
-        if self._external_cache is not None:
+        self.cached = None        # lengths before the step, where they are not self.positions
+        if self.kv_format == "int4":
+            self.cache, self.cache_rows = None, None
+            if self.plan is None:
+                self.paged = serving.PagedCache4(self.L, B, self.max_len, self.page_size, dev, self._pages)
+                self.plan = serving.PagePlan(self.paged, B)
+            else:
+                self.paged = self.plan.paged
+            self.q4_ws = ops.mla_q4_workspace(B, dev)
+        elif self._external_cache is not None:
             self.cache = self._external_cache
             self.cache_rows = torch.zeros(B, device=dev, dtype=i32)
         else:
@@ -155,11 +181,17 @@ class DecodeEngine:
         if self.split_k:
             s_q = split_count(QKVA_ROWS, HIDDEN, self.num_sms, B)
             s_o = split_count(HIDDEN, N_HEADS * V_DIM, self.num_sms, B)
-            self.qkva_part = torch.zeros((s_q, B, QKVA_ROWS), device=dev, dtype=f32)
-            self.o_proj_part = torch.zeros((s_o, B, HIDDEN), device=dev, dtype=f32)
+            # adapters add one more partial to the projections' sums
+            extra = 1 if self.adapters is not None else 0
+            self.qkva_part = torch.zeros((s_q + extra, B, QKVA_ROWS), device=dev, dtype=f32)
+            self.o_proj_part = torch.zeros((s_o + extra, B, HIDDEN), device=dev, dtype=f32)
             dense_k = max([lp.dense.inter for lp in self.layers if lp.dense is not None], default=0)
             s_d = split_count(HIDDEN, dense_k, self.num_sms, B) if dense_k else 1
             self.dense_part = torch.zeros((s_d, B, HIDDEN), device=dev, dtype=f32)
+        if self.adapters is not None:
+            self.lora_ws = ops.lora_workspace(B, QKVA_ROWS, HIDDEN, self.adapters.rank, dev)
+            if self.split_k:
+                del self.lora_ws["parts"]
         self.q_abs = torch.zeros((B, N_HEADS, KV_LORA), device=dev, dtype=bf)
         self.o_lat = torch.zeros((B, N_HEADS, KV_LORA), device=dev, dtype=bf)
         self.attn_o = torch.zeros((B, N_HEADS * V_DIM), device=dev, dtype=bf)
@@ -266,11 +298,21 @@ class DecodeEngine:
     def _linear(self, **kw):
         ops.linear(family=self.family, **kw)
 
-    def _split_linear(self, *, w, n_rows, k, x, out, **kw) -> torch.Tensor:
+    def _lora_args(self, a: torch.Tensor, b: torch.Tensor) -> dict:
+        ad = self.adapters
+        # rows that are tokens name their request (kernel prefill), others are the requests
+        rows = self.plan.token_row if self.kv_format == "int4" else self.cache_rows
+        return dict(a=a, b=b, ids=ad.ids, ranks=ad.ranks, scales=ad.scales, token_row=rows)
+
+    def _split_linear(self, *, w, n_rows, k, x, out, lora: tuple | None = None, **kw) -> torch.Tensor:
         """Dense linear into fp32 split-K partials out[S, B, n_rows] (batch family): every
         token stays in one tile, so the weights are streamed once, and the K split spreads
-        the launch over the SMs.  Returns the [B, S, n_rows] view the consumers sum."""
+        the launch over the SMs.  lora (A, B of all adapters): the last partial is the tokens'
+        adapters.  Returns the [B, S, n_rows] view the consumers sum."""
         S = out.shape[0]
+        if lora is not None:
+            S -= 1
+            ops.lora(x=x, y=out[S], **self._lora_args(*lora), **self.lora_ws)
         self._linear(w=w, n_rows=n_rows, k=k, x=x, y=out[0], epilogue=ops.EPI_STORE_F32, n_tokens=self.B,
                      x_group_rows=self.B, k_splits=S, y_split_stride=out.stride(0), **kw)
         return out.permute(1, 0, 2)
@@ -278,16 +320,25 @@ class DecodeEngine:
     def _attention(self, li: int, lp: LayerPack) -> torch.Tensor:
         """Attention sublayer; returns its output (bf16 [B, 2048] or fp32 partials [B, S, 2048])."""
         a, B = lp.attn, self.B
+        ad = self.adapters.layers[li] if self.adapters is not None else None
         if self.split_k:
-            self._split_linear(w=a.qkva, n_rows=QKVA_ROWS, k=HIDDEN, x=self.x, out=self.qkva_part)
+            self._split_linear(w=a.qkva, n_rows=QKVA_ROWS, k=HIDDEN, x=self.x, out=self.qkva_part,
+                               lora=None if ad is None else (ad.qkva_a, ad.qkva_b))
             qkva = self.qkva_part
+        elif ad is not None:
+            qkva = ops.lora_linear(x=self.x, w=a.qkva, y=self.qkva, **self._lora_args(ad.qkva_a, ad.qkva_b), **self.lora_ws)
         else:
             self._linear(w=a.qkva, n_rows=QKVA_ROWS, k=HIDDEN, x=self.x, y=self.qkva, n_tokens=B,
                          x_group_rows=B)
             qkva = self.qkva
-        ops.mla_prep(qkva=qkva, kv_norm_w=a.kv_norm_w, eps=a.kv_norm_eps, cos=self.cos, sin=self.sin,
-                     positions=self.positions, cache=self.cache[li], q_pe_out=self.q_pe, q_nope_out=self.q_nope,
-                     cache_rows=self.cache_rows)
+        if self.kv_format == "int4":
+            ops.mla_prep_q4(qkva=qkva, kv_norm_w=a.kv_norm_w, eps=a.kv_norm_eps, cos=self.cos, sin=self.sin,
+                            positions=self.plan.positions, slots=self.plan.slots, cache=self.paged.cache[li],
+                            q_pe_out=self.q_pe, q_nope_out=self.q_nope)
+        else:
+            ops.mla_prep(qkva=qkva, kv_norm_w=a.kv_norm_w, eps=a.kv_norm_eps, cos=self.cos, sin=self.sin,
+                         positions=self.positions, cache=self.cache[li], q_pe_out=self.q_pe, q_nope_out=self.q_nope,
+                         cache_rows=self.cache_rows)
         # q_abs[b, h] = q_nope[b, h] @ W_UK[h]
         self._linear(w=a.w_uk_t, n_rows=KV_LORA, k=QK_NOPE, w_row_stride=QK_NOPE,
                      w_group_stride=KV_LORA * QK_NOPE, x=self.q_nope, x_row_stride=N_HEADS * QK_NOPE,
@@ -295,11 +346,17 @@ class DecodeEngine:
                      y_group_stride=KV_LORA, n_groups=N_HEADS, n_tokens=B, w_group_rows=KV_LORA,
                      x_group_rows=B)
         defer = (self.defer_mla_merge and self.family == ops.FAMILY_SMALL and B == 1
-                 and self.cache_rows is None)
-        ops.mla_decode(q_abs=self.q_abs, q_pe=self.q_pe, cache=self.cache[li], positions=self.positions,
-                       softmax_scale=self.scale, split_len=self.split_len, o_part=self.o_part,
-                       ml_part=self.ml_part, o_lat=self.o_lat, inputs_prior=True, row_sync=self.mla_sync,
-                       cache_rows=self.cache_rows, part_count=self.mla_parts if defer else None)
+                 and self.cache_rows is None and self.kv_format == "bf16")
+        if self.kv_format == "int4":
+            ops.mla_decode_q4(q_abs=self.q_abs, q_pe=self.q_pe, cache=self.paged.cache[li],
+                              block_table=self.paged.block_table, positions=self.plan.positions,
+                              seq_rows=self.plan.token_row, page_size=self.paged.page_size,
+                              softmax_scale=self.scale, o_lat=self.o_lat, **self.q4_ws)
+        else:
+            ops.mla_decode(q_abs=self.q_abs, q_pe=self.q_pe, cache=self.cache[li], positions=self.positions,
+                           softmax_scale=self.scale, split_len=self.split_len, o_part=self.o_part,
+                           ml_part=self.ml_part, o_lat=self.o_lat, inputs_prior=True, row_sync=self.mla_sync,
+                           cache_rows=self.cache_rows, part_count=self.mla_parts if defer else None)
         # o[b, h] = o_lat[b, h] @ W_UV[h]^T,  W_UV[h] = kv_b[h*256 + 128 : h*256 + 256]
         self._linear(w=a.kv_b[QK_NOPE:], n_rows=V_DIM, k=KV_LORA, w_row_stride=KV_LORA,
                      w_group_stride=(QK_NOPE + V_DIM) * KV_LORA, x=self.o_lat, x_row_stride=N_HEADS * KV_LORA,
@@ -307,7 +364,11 @@ class DecodeEngine:
                      y_group_stride=V_DIM, n_groups=N_HEADS, n_tokens=B, w_group_rows=V_DIM,
                      x_group_rows=B, x_parts=(self.o_part, self.ml_part, self.mla_parts) if defer else None)
         if self.split_k:
-            return self._split_linear(w=a.o, n_rows=HIDDEN, k=N_HEADS * V_DIM, x=self.attn_o, out=self.o_proj_part)
+            return self._split_linear(w=a.o, n_rows=HIDDEN, k=N_HEADS * V_DIM, x=self.attn_o, out=self.o_proj_part,
+                                      lora=None if ad is None else (ad.o_a, ad.o_b))
+        if ad is not None:
+            ws = dict(self.lora_ws, parts=self.lora_ws["parts"].view(-1)[:B * HIDDEN].view(1, B, HIDDEN))
+            return ops.lora_linear(x=self.attn_o, w=a.o, y=self.attn_out, **self._lora_args(ad.o_a, ad.o_b), **ws)
         self._linear(w=a.o, n_rows=HIDDEN, k=N_HEADS * V_DIM, x=self.attn_o, y=self.attn_out, n_tokens=B,
                      x_group_rows=B)
         return self.attn_out
@@ -446,6 +507,8 @@ class DecodeEngine:
         embeddings), the router's top-6 ids of every MoE layer ("routes") and the
         normalised activations that router read ("moe_x", bf16 [B, 2048])."""
         lp0 = self.layers[0]
+        if self.kv_format == "int4":
+            self.plan.run(self.positions if self.cached is None else self.cached)
         ops.embed_rmsnorm(self.input_ids, self.embed, lp0.in_norm_w, lp0.eps, self.h, self.x)
         if trace is not None:
             trace.setdefault("hidden", []).append(self.h.float().clone())
@@ -491,15 +554,20 @@ class DecodeEngine:
     def set_state(self, positions: torch.Tensor, input_ids: torch.Tensor) -> None:
         self.positions.copy_(positions.to(self.positions))
         self.input_ids.copy_(input_ids.to(self.input_ids).view(-1))
-        self._saved = (self.positions.clone(), self.input_ids.clone())
+        # the ring of free pages goes back with the positions: the steps after restore() take the
+        # same pages again
+        self._saved = (self.positions.clone(), self.input_ids.clone(),
+                       self.paged.ring.clone() if self.kv_format == "int4" else None)
 
     def restore(self) -> None:
         """Roll back positions / next tokens to the post-prefill state.  Cache rows at or
         beyond a row's position are never read before being rewritten, so the latent cache
         needs no snapshot (unlike the expanded cache of src/run.py:161-217)."""
-        pos, ids = self._saved
+        pos, ids, ring = self._saved
         self.positions.copy_(pos)
         self.input_ids.copy_(ids)
+        if ring is not None:
+            self.paged.ring.copy_(ring)
 
     def capture(self, warmup: int = 3) -> None:
         """Warm up eagerly (rolled back), then capture one decode step in a CUDA graph."""
@@ -542,7 +610,8 @@ class DecodeEngine:
                 raise _lib.Dsv2Error(f"device error {code} in an expert-parallel step: rebuild the engine "
                                      "on every rank")
             s = ops.stream()
-            for t in (getattr(self, "moe_sync", None), self.mla_sync):
+            q4 = (self.q4_ws["row_sync"], self.plan.buf["sync"]) if self.kv_format == "int4" else ()
+            for t in (getattr(self, "moe_sync", None), self.mla_sync, *q4):
                 if t is not None:
                     _lib.reset_progress(t.data_ptr(), t.numel(), s)
             torch.cuda.synchronize(self.dev)
@@ -586,19 +655,31 @@ class DecodeEngine:
         first = torch.zeros(self.B, dtype=torch.int64, device=dev)
         n = tokens.numel()
         subs: dict[int, DecodeEngine] = {}
+        q4 = self.kv_format == "int4"
+        if q4:
+            self.paged.reset()
+            start = torch.cumsum(lens_t, 0) - lens_t
         try:
             for c0 in range(0, n, max_tokens_per_chunk):
                 c1 = min(n, c0 + max_tokens_per_chunk)
                 t = c1 - c0
                 sub = subs.get(t)
                 if sub is None:
+                    plan = serving.PagePlan(self.paged, t) if q4 else None
                     sub = DecodeEngine(self.model, t, self.max_len, "batch", cache=self.cache,
-                                       gate_bias=self._gate_bias)
+                                       gate_bias=self._gate_bias, plan=plan, adapters=self.adapters)
                     subs[t] = sub
-                sub.cache_rows.copy_(seq[c0:c1])
+                if q4:
+                    # what every prompt holds before and after this chunk of the tokens laid end to end
+                    sub.cached = torch.minimum((c0 - start).clamp(min=0), lens_t)
+                    sub.plan.new.copy_(torch.minimum((c1 - start).clamp(min=0), lens_t) - sub.cached)
+                else:
+                    sub.cache_rows.copy_(seq[c0:c1])
                 sub.positions.copy_(pos[c0:c1])
                 sub.input_ids.copy_(tokens[c0:c1])
                 sub.step()
+                if q4:
+                    sub.plan.check()
                 rows = [(b, int(last[b]) - c0) for b in range(self.B) if c0 <= int(last[b]) < c1]
                 if rows:
                     bi = torch.tensor([r[0] for r in rows], device=dev)
@@ -621,10 +702,20 @@ class DecodeEngine:
         """
         if len(prompts) != self.B:
             raise ValueError(f"expected {self.B} prompts, got {len(prompts)}")
+        if self.adapters is not None:
+            raise NotImplementedError("the HF forward knows no adapters: prefill with method=\"kernels\"")
         model = self.model
         lens = [int(p.numel()) for p in prompts]
         if max(lens) >= self.max_len:
             raise ValueError("prompt longer than the cache")
+        if self.kv_format == "int4":
+            self.paged.reset()
+            plan = serving.PagePlan(self.paged, sum(lens), torch.tensor(lens, device=self.dev, dtype=torch.int32))
+            plan.run(torch.zeros(self.B, device=self.dev, dtype=torch.int32))
+            plan.check()
+            starts = [0]
+            for n in lens:
+                starts.append(starts[-1] + n)
         captured: dict[int, torch.Tensor] = {}
         hooks = []
         for li, layer in enumerate(model.model.layers):
@@ -652,8 +743,12 @@ class DecodeEngine:
                 last = hid[torch.arange(nr, device=self.dev), idx]
                 first[r0:r1] = torch.argmax(model.lm_head(last), dim=-1)
                 for li, lp in enumerate(self.layers):
-                    self.cache[li, r0:r1, :T] = latent_rows(captured[li], lp.attn.kv_norm_w,
-                                                            lp.attn.kv_norm_eps, self.cos[:T], self.sin[:T])
+                    lat = latent_rows(captured[li], lp.attn.kv_norm_w, lp.attn.kv_norm_eps, self.cos[:T], self.sin[:T])
+                    if self.kv_format == "bf16":
+                        self.cache[li, r0:r1, :T] = lat
+                        continue
+                    live = torch.cat([lat[i, :lens[r0 + i]] for i in range(nr)])
+                    ops.latent4_write(rows=live, slots=plan.slots[starts[r0]:starts[r1]], cache=self.paged.cache[li])
                 captured.clear()
                 r0 = r1
         finally:

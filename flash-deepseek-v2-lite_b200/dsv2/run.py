@@ -3,6 +3,7 @@
     python -m dsv2.run [--model-path DIR] [--batch-size B | --batch-sizes "1 32 256"]
                        [--max-new-tokens N] [--kernel-family small|batch]
                        [--dump-token-ids] [--dump-step-trace]
+                       [--kv-cache bf16|int4] [--page-size N] [--lora-adapters N [--lora-rank R]]
 
 Mirrors the reference runner (src/run.py:220-236 options, :591-688 harness, :690-757
 output): greedy decode of one prompt replicated over the batch, the decode time taken
@@ -25,6 +26,7 @@ import time
 import torch
 
 from .engine import FAMILIES, DecodeEngine
+from .serving import random_adapters
 
 
 def _parse_args(argv=None):
@@ -43,6 +45,12 @@ def _parse_args(argv=None):
     ap.add_argument("--device", type=str, default="cuda:0")
     ap.add_argument("--prefill", choices=["kernels", "eager"], default="kernels",
                     help="prompt prefill through the decode kernels or the HF forward")
+    ap.add_argument("--kv-cache", choices=["bf16", "int4"], default="bf16",
+                    help="latent cache: dense bf16 rows, or pages of the 4-bit format")
+    ap.add_argument("--page-size", type=int, default=64, help="int4 cache: tokens per page (a multiple of 16)")
+    ap.add_argument("--lora-adapters", type=int, default=0,
+                    help="seeded low-rank adapters, request r with adapter r %% (N + 1) - 1 (-1: none)")
+    ap.add_argument("--lora-rank", type=int, default=16, help="their rank (a multiple of 8)")
     ap.add_argument("--dump-token-ids", action="store_true")
     ap.add_argument("--dump-step-trace", action="store_true")
     return ap.parse_args(argv)
@@ -98,13 +106,17 @@ def hardware_info(dev: torch.device) -> dict:
 
 def run_graph_decode(model, prompt: torch.Tensor, batch: int, max_new_tokens: int, family: str,
                      dump_token_ids: bool = False, dump_step_trace: bool = False,
-                     prefill: str = "kernels") -> dict:
+                     prefill: str = "kernels", kv_cache: str = "bf16", page_size: int = 64,
+                     lora_adapters: int = 0, lora_rank: int = 16) -> dict:
     """Prefill + graph decode of `prompt` replicated over `batch` rows; returns the
     reference runner's per-batch result fields."""
     dev = prompt.device
     prompt_len = int(prompt.numel())
     max_len = prompt_len + max_new_tokens + 8
-    eng = DecodeEngine(model, batch, max_len, family)
+    adapters = None
+    if lora_adapters > 0:
+        adapters = random_adapters(len(model.model.layers), lora_adapters, lora_rank, batch, dev)
+    eng = DecodeEngine(model, batch, max_len, family, kv_format=kv_cache, page_size=page_size, adapters=adapters)
     torch.cuda.synchronize(dev)
     t0 = time.perf_counter()
     first = eng.prefill([prompt] * batch, method=prefill)
@@ -141,6 +153,8 @@ def run_graph_decode(model, prompt: torch.Tensor, batch: int, max_new_tokens: in
     decode_tokens = batch * max(max_new_tokens - 1, 0)
     out = {"batch_size": batch, "path": f"dsv2_{family}_graph", "ttft_ms": prefill_s * 1000.0,
            "tps": decode_tokens / decode_s if decode_s > 0 else 0.0, "decode_tokens": decode_tokens}
+    if kv_cache != "bf16" or lora_adapters:
+        out.update(kv_cache=kv_cache, lora_adapters=lora_adapters)
     if dump_token_ids:
         out["generated_token_ids"] = generated[0] if batch == 1 else generated
     if dump_step_trace:
@@ -159,7 +173,9 @@ def main(argv=None) -> None:
     for b in _batch_sizes(args):
         family = args.kernel_family or ("small" if b <= 4 else "batch")
         results.append(run_graph_decode(model, prompt, b, args.max_new_tokens, family,
-                                        args.dump_token_ids, args.dump_step_trace, prefill=args.prefill))
+                                        args.dump_token_ids, args.dump_step_trace, prefill=args.prefill,
+                                        kv_cache=args.kv_cache, page_size=args.page_size,
+                                        lora_adapters=args.lora_adapters, lora_rank=args.lora_rank))
     hw = hardware_info(dev)
     doc = dict(results[0], hardware=hw) if len(results) == 1 else {"results": results, "hardware": hw}
     print(json.dumps(doc, ensure_ascii=False, indent=2))
