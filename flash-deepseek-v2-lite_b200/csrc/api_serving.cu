@@ -106,7 +106,7 @@ int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* a, void* stream) {
                 (long long)a->n_blocks);
   if (a->rows == 0) return DSV2_OK;
   if (!a->q_abs || !a->q_pe || !a->cache || !a->block_table || !a->positions || !a->o_lat || !a->o_part ||
-      !a->ml_part || !a->row_sync)
+      !a->ml_part || !a->cuts)
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: null pointer");
   if (a->part_slots < 2) return fail(DSV2_ERR_INVALID, "mla_decode_q4: %d partial slots (at least 2)", a->part_slots);
   if (a->page_size <= 0 || a->page_size % DSV2_L4_BLOCK_TOKENS)
@@ -116,7 +116,7 @@ int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* a, void* stream) {
     return fail(DSV2_ERR_UNSUPPORTED, "mla_decode_q4: a table row of %d pages of %d tokens exceeds 2^31 tokens",
                 a->width, a->page_size);
   if (!aligned16(a->q_abs) || !aligned16(a->q_pe) || !aligned16(a->cache) || !aligned16(a->o_lat) ||
-      !aligned16(a->o_part))
+      !aligned16(a->o_part) || !aligned16(a->ml_part) || !aligned16(a->cuts))
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: operands must be 16-byte aligned");
   int sms = 0;
   if (int rc = ensure_init(&sms)) return rc;
@@ -139,7 +139,7 @@ int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* a, void* stream) {
   p.o_part = a->o_part;
   p.ml_part = a->ml_part;
   p.part_slots = a->part_slots;
-  p.row_sync = a->row_sync;
+  p.cuts = reinterpret_cast<int4*>(a->cuts);
   if (!a->seq_rows && a->seqs < a->rows)
     return fail(DSV2_ERR_INVALID, "mla_decode_q4: %d query rows, %d table rows (pass seq_rows)", a->rows, a->seqs);
   return check_launch(launch_mla_q4(p, sms, static_cast<cudaStream_t>(stream)), "mla_decode_q4");

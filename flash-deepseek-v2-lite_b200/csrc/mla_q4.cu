@@ -16,7 +16,7 @@ constexpr int kQ4SegUnits = 4;                               // per-row cost in 
 constexpr int kQ4ScoreWarps = 8;                             // a block of a tile each
 constexpr int kQ4PvWarps = 8;                                // 64 latent dims each
 constexpr int kQ4Compute = (kQ4ScoreWarps + kQ4PvWarps) * 32;
-constexpr int kQ4ProducerWarp = kQ4ScoreWarps + kQ4PvWarps;  // warp 16: copies, then tickets
+constexpr int kQ4ProducerWarp = kQ4ScoreWarps + kQ4PvWarps;  // warp 16: copies
 constexpr int kQ4Threads = kQ4Compute + 32;
 constexpr int kQ4QBytes = kHeads * (1024 + 128);             // a query row: q_abs, then q_pe
 constexpr int kQ4Steps = 32;                                 // k-steps of 16 latent dims; 4 roped ones follow
@@ -170,22 +170,22 @@ struct Q4Smem {
   float lsum[kQ4ScoreWarps][kHeads];
   float fin[2][kHeads];
   uint64_t full[kQ4Stages], empty[kQ4Stages];
-  uint64_t p_full[2], p_empty[2], q_full[2], q_empty[2], fin_full[2], fin_empty[2], tk_full[2], tk_done;
-  long long ll[4];                          // first row's stream position, two pending rows'
+  uint64_t p_full[2], p_empty[2], q_full[2], q_empty[2], fin_full[2], fin_empty[2];
+  long long first_S;                        // stream position of the CTA's first row
   int wsum[32];
   int rescale[2];
-  int first_row, abort, n_pend, pend_row[2], pend_blocks[2];
+  int first_row, abort;
 };
 static_assert(sizeof(Q4Smem) <= 232448, "4-bit latent attention: shared memory exceeds 227 KB");
 
 // One launch, persistent: the rows form one stream of units (kQ4SegUnits of per-row cost, then
 // the row's 16-token blocks), cut into equal ranges, one CTA (17 warps) per SM.  A row inside
-// one range writes o_lat; a row cut by a boundary leaves (o, m, l) partials that the last of
-// its CTAs merges (row tickets).
+// one range writes o_lat; a row cut by a boundary leaves (o, m, l) partials, two slots per CTA
+// (slot 0: a row that began before the range), which mla_q4_merge_kernel joins.
 //  - warps 0-7, scores: one block (16 positions) of a tile each, all dims; the row's query
 //    fragments are made once per row, in shared memory, as fp16 scaled by a power of two per head;
 //  - warps 8-15, P V: 64 latent dims each;
-//  - warp 16: copies blocks (looked up 32 at a time) and query rows, then publishes tickets.
+//  - warp 16: copies blocks (looked up 32 at a time) and query rows, and notes each row's partials.
 // The maximum that P is taken against is kept until a score exceeds it by 2^kQ4Slack: the score
 // warps then agree on a new one and the P V warps rescale.
 __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params p) {
@@ -206,9 +206,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
       mbar_init(&sm.q_empty[i], kQ4ScoreWarps);
       mbar_init(&sm.fin_full[i], 1);
       mbar_init(&sm.fin_empty[i], kQ4PvWarps);
-      mbar_init(&sm.tk_full[i], 1 + kQ4PvWarps);
     }
-    mbar_init(&sm.tk_done, 1);
     sm.abort = 0;
     fence_mbar_init();
   }
@@ -238,7 +236,10 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
   }
   const long long c = blockIdx.x;
   const long long n_cta = min(static_cast<long long>(gridDim.x), (T + p.min_units - 1) / p.min_units);
-  if (c >= n_cta) return;
+  if (c >= n_cta) {
+    if (tid == 0) p.cuts[c] = make_int4(-1, 0, 0, 0);
+    return;
+  }
   const long long start = mla_range_start(c, T, n_cta), end = mla_range_start(c + 1, T, n_cta);
   if (R <= kQ4Threads) {
     long long off = 0;
@@ -247,7 +248,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
       if (w < warp) off += sm.wsum[w];
     const long long S = off + incl0 - mine0;
     if (tid < R && S <= start && start < S + mine0) {
-      sm.ll[0] = S;
+      sm.first_S = S;
       sm.first_row = tid;
     }
   } else {
@@ -272,14 +273,14 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
       }
       const long long S = off + v - u;
       if (r < R && S <= start && start < S + u) {
-        sm.ll[0] = S;
+        sm.first_S = S;
         sm.first_row = r;
       }
       run += total;
     }
   }
   __syncthreads();
-  const long long S0 = sm.ll[0];
+  const long long S0 = sm.first_S;
   const int r0 = sm.first_row;
 
   // the row at stream position S: its blocks [j0, j1) in this CTA's range
@@ -292,6 +293,18 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
 
   if (warp == kQ4ProducerWarp) {
     // ================= producer warp
+    if (lane == 0) {
+      // the second CTA of a cut row notes the row, its first partial slot and their number; every
+      // CTA writes its entry, also one whose range holds no block (per-row units alone)
+      const long long St = S0 + kQ4SegUnits;
+      int4 cut = make_int4(-1, 0, 0, 0);
+      if (St < start && mla_owner(St, T, n_cta) == c - 1) {
+        const int nblk = q4_blocks(q4_len(p, r0));
+        cut = make_int4(r0, static_cast<int>(2 * (c - 1)) + mla_slot(S0, mla_range_start(c - 1, T, n_cta)),
+                        static_cast<int>(mla_owner(St + nblk - 1, T, n_cta) - c + 2), 0);
+      }
+      p.cuts[c] = cut;
+    }
     bool ok = true;
     int seg = 0, st = 0;
     uint32_t round = 0;   // times the ring has been filled
@@ -352,34 +365,6 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
     for (int k = max(0, seg - 2); k < seg; ++k)
       for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sm.q_full[k & 1], static_cast<uint32_t>((k >> 1) & 1)); ++i) {
       }
-    // publish the (at most two) rows this CTA holds a part of
-    if (lane == 0) {
-      int n_pend = 0;
-      S = S0;
-      for (int r = r0; S + kQ4SegUnits < end && r < R; ++r) {
-        const int nblk = q4_blocks(q4_len(p, r));
-        int j0, j1;
-        if (!segment(S, nblk, j0, j1)) {
-          const int slot = mla_slot(S, start);
-          if (q4_wait(&sm.tk_full[slot], 0, s_abort)) {
-            const long long St = S + kQ4SegUnits;
-            const int n_seg = static_cast<int>(mla_owner(St + nblk - 1, T, n_cta) - mla_owner(St, T, n_cta) + 1);
-            __threadfence();   // the partial (written by other warps, ordered by the mbarrier) first
-            if (atomicAdd(&p.row_sync[r], 1) == n_seg - 1) {
-              p.row_sync[r] = 0;
-              __threadfence();
-              sm.pend_row[n_pend] = r;
-              sm.pend_blocks[n_pend] = nblk;
-              sm.ll[2 + n_pend] = S;
-              ++n_pend;
-            }
-          }
-        }
-        S += nblk + kQ4SegUnits;
-      }
-      sm.n_pend = n_pend;
-      mbar_arrive(&sm.tk_done);
-    }
     return;
   }
 
@@ -602,10 +587,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
           }
         }
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sm.fin_full[fb]);
-          if (!complete) mbar_arrive(&sm.tk_full[mla_slot(S, start)]);
-        }
+        if (lane == 0) mbar_arrive(&sm.fin_full[fb]);
       }
       // lsum is written again only after the next row's tile barriers
       S += nblk + kQ4SegUnits;
@@ -710,79 +692,75 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
         }
       }
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.fin_empty[fb]);
-        if (!complete) mbar_arrive(&sm.tk_full[mla_slot(S, start)]);
-      }
+      if (lane == 0) mbar_arrive(&sm.fin_empty[fb]);
       S += nblk + kQ4SegUnits;
     }
   }
+}
 
-  // ================= merges of the rows this CTA published last (all compute warps)
-  q4_wait(&sm.tk_done, 0, s_abort);
-  const int n_pend = min(sm.n_pend, 2);
-  float* s_m = reinterpret_cast<float*>(sm.ring);   // the drained ring
-  for (int pi = 0; pi < n_pend; ++pi) {
-    const int r = sm.pend_row[pi], nblk = sm.pend_blocks[pi];
-    const long long Sb = sm.ll[2 + pi], St = Sb + kQ4SegUnits;
-    const long long c_first = mla_owner(St, T, n_cta), c_last = mla_owner(St + nblk - 1, T, n_cta);
-    const int n_seg = static_cast<int>(c_last - c_first + 1);
-    float* s_l = s_m + kHeads * n_seg;
-    auto part_index = [&](int k) -> long long {
-      const long long cc = c_first + k;
-      return cc * 2 + ((k == 0) ? mla_slot(Sb, mla_range_start(cc, T, n_cta)) : 0);
-    };
-    q4_bar(6, kQ4Compute);   // the ring is drained; the previous merge is done with it
-    for (int i = tid; i < kHeads * n_seg; i += kQ4Compute) {
-      const int h = i / n_seg, k = i % n_seg;
-      const long long pk = part_index(k);
-      s_m[i] = __ldcg(p.ml_part + (pk * kHeads + h) * 2);
-      s_l[i] = __ldcg(p.ml_part + (pk * kHeads + h) * 2 + 1);
+// o_lat[r, h] = sum_k 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k over the partials of a row that was cut.
+// A CTA per cut and head: 4 groups of 64 threads take every fourth partial (a long row alone has one
+// per SM), then meet in shared memory.  A launch of its own:
+// with the merge in the last CTA of a row, 148 partials of 32 KB went through one SM (75 us).
+__global__ __launch_bounds__(256) void mla_q4_merge_kernel(const MlaQ4Params p) {
+  pdl_enter();
+  const int h = blockIdx.y, tid = threadIdx.x;
+  const int4 cut = __ldcg(p.cuts + blockIdx.x);
+  const int r = cut.x, first = cut.y, n = cut.z;
+  if (r < 0) return;
+  if (r >= p.rows || first < 0 || n < 2 || 2 * (first / 2 + n) > p.part_slots || n > kMlaMaxCtas) {
+    if (tid == 0) set_device_error(kErrIndex);   // not what the attention kernel writes
+    return;
+  }
+  __shared__ float s_w[kMlaMaxCtas];
+  __shared__ float s_inv;
+  __shared__ float4 s_o[4][2][64];
+  auto slot = [&](int k) -> long long { return k == 0 ? first : 2LL * (first / 2 + k); };
+  if (tid < 32) {
+    float M = -INFINITY, den = 0.f;
+    for (int k = tid; k < n; k += 32) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml_part + (slot(k) * kHeads + h) * 2));
+      s_w[k] = ml.x;
+      if (ml.y != 0.f) M = fmaxf(M, ml.x);
     }
-    q4_bar(6, kQ4Compute);
-    if (tid < kHeads) {
-      // w_k = 2^(m_k - M) / sum_k 2^(m_k - M) l_k
-      float M = -INFINITY;
-      for (int k = 0; k < n_seg; ++k)
-        if (s_l[tid * n_seg + k] != 0.f) M = fmaxf(M, s_m[tid * n_seg + k]);
-      float den = 0.f;
-      for (int k = 0; k < n_seg; ++k) {
-        const float l = s_l[tid * n_seg + k];
-        const float w = l != 0.f ? exp2f(s_m[tid * n_seg + k] - M) : 0.f;
-        s_m[tid * n_seg + k] = w;
-        den += w * l;
-      }
-      const float inv = den != 0.f ? 1.f / den : 0.f;
-      for (int k = 0; k < n_seg; ++k) s_m[tid * n_seg + k] *= inv;
+    M = warp_max(M);
+    for (int k = tid; k < n; k += 32) {
+      const float l = __ldcg(p.ml_part + (slot(k) * kHeads + h) * 2 + 1);
+      const float w = l != 0.f ? ex2(s_w[k] - M) : 0.f;
+      s_w[k] = w;
+      den += w * l;
     }
-    q4_bar(6, kQ4Compute);
-    constexpr int kItems = kHeads * 512 / 4;
-    constexpr int kPer = (kItems + kQ4Compute - 1) / kQ4Compute;   // 6, the last third of one unused
-    float4 acc[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < n_seg; ++k) {
-      const float4* o = reinterpret_cast<const float4*>(p.o_part + part_index(k) * kHeads * 512);
-      float4 v[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) v[i] = __ldcg(o + min(tid + i * kQ4Compute, kItems - 1));
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const float w = s_m[(min(tid + i * kQ4Compute, kItems - 1) / 128) * n_seg + k];
-        acc[i].x += w * v[i].x;
-        acc[i].y += w * v[i].y;
-        acc[i].z += w * v[i].z;
-        acc[i].w += w * v[i].w;
-      }
-    }
-    bf16* ob = p.o_lat + static_cast<long long>(r) * kHeads * 512;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      uint2 v;
-      v.x = pack_bf16x2(acc[i].x, acc[i].y);
-      v.y = pack_bf16x2(acc[i].z, acc[i].w);
-      if (tid + i * kQ4Compute < kItems) *reinterpret_cast<uint2*>(ob + 4 * (tid + i * kQ4Compute)) = v;
-    }
+    den = warp_sum(den);
+    if (tid == 0) s_inv = den != 0.f ? 1.f / den : 0.f;
+  }
+  __syncthreads();
+  const int g = tid >> 6, d = tid & 63;
+  float4 acc[2];
+  acc[0] = acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = g; k < n; k += 4) {
+    const float4* o = reinterpret_cast<const float4*>(p.o_part + (slot(k) * kHeads + h) * 512) + d;
+    const float4 v = __ldcg(o), u = __ldcg(o + 64);
+    const float w = s_w[k];
+    acc[0].x += w * v.x;
+    acc[0].y += w * v.y;
+    acc[0].z += w * v.z;
+    acc[0].w += w * v.w;
+    acc[1].x += w * u.x;
+    acc[1].y += w * u.y;
+    acc[1].z += w * u.z;
+    acc[1].w += w * u.w;
+  }
+  s_o[g][0][d] = acc[0];
+  s_o[g][1][d] = acc[1];
+  __syncthreads();
+  if (tid < 128) {
+    const float4* o = &s_o[0][0][0] + tid;   // [group][128]
+    const float inv = s_inv;
+    const float4 a = o[0], b = o[128], c = o[256], e = o[384];
+    *reinterpret_cast<uint2*>(p.o_lat + (static_cast<long long>(r) * kHeads + h) * 512 + 4 * tid) =
+        make_uint2(pack_bf16x2((a.x + b.x + c.x + e.x) * inv, (a.y + b.y + c.y + e.y) * inv),
+                   pack_bf16x2((a.z + b.z + c.z + e.z) * inv, (a.w + b.w + c.w + e.w) * inv));
   }
 }
 
@@ -795,6 +773,7 @@ cudaError_t mla_q4_init() {
 cudaError_t launch_mla_q4(const MlaQ4Params& p, int num_sms, cudaStream_t st) {
   const int grid = std::min(std::min(num_sms, kMlaMaxCtas), p.part_slots / 2);
   launch_kernel(mla_q4_kernel, grid, kQ4Threads, sizeof(Q4Smem), st, p);
+  launch_kernel(mla_q4_merge_kernel, dim3(grid, kHeads), 256, 0, st, p);
   return cudaGetLastError();
 }
 

@@ -157,7 +157,7 @@ struct MlaQ4Params {
   float* o_part;               // [part_slots, 16, 512] partials, two slots per CTA
   float* ml_part;              // [part_slots, 16, 2] (m in the log2 domain, l)
   int part_slots;
-  int* row_sync;               // [rows] zero-initialised, left zero
+  int4* cuts;                  // [part_slots / 2] per CTA: {row it cuts or -1, first partial slot, number}
 };
 
 // Low-rank adapters of many requests (lora.cu)

@@ -124,7 +124,7 @@ class MlaDecodeQ4Args(ctypes.Structure):
         ("q_abs", c_vp), ("q_pe", c_vp), ("cache", c_vp), ("n_blocks", c_i64), ("block_table", c_vp),
         ("table_stride", c_i64), ("width", c_i32), ("seqs", c_i32), ("page_size", c_i32), ("rows", c_i32),
         ("positions", c_vp), ("seq_rows", c_vp), ("softmax_scale", c_f32), ("o_lat", c_vp),
-        ("o_part", c_vp), ("ml_part", c_vp), ("row_sync", c_vp), ("part_slots", c_i32),
+        ("o_part", c_vp), ("ml_part", c_vp), ("cuts", c_vp), ("part_slots", c_i32),
     ]
 
 

@@ -610,7 +610,7 @@ class DecodeEngine:
                 raise _lib.Dsv2Error(f"device error {code} in an expert-parallel step: rebuild the engine "
                                      "on every rank")
             s = ops.stream()
-            q4 = (self.q4_ws["row_sync"], self.plan.buf["sync"]) if self.kv_format == "int4" else ()
+            q4 = (self.plan.buf["sync"],) if self.kv_format == "int4" else ()
             for t in (getattr(self, "moe_sync", None), self.mla_sync, *q4):
                 if t is not None:
                     _lib.reset_progress(t.data_ptr(), t.numel(), s)

@@ -655,17 +655,17 @@ def mla_prep_q4(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos:
 
 
 def mla_q4_workspace(rows: int, device) -> dict:
-    """Work buffers of mla_decode_q4 for up to `rows` query rows: partials (two slots per CTA, one
-    CTA per SM) and the zeroed row tickets."""
+    """Work buffers of mla_decode_q4, for any number of query rows: partials (two slots per CTA, one
+    CTA per SM) and the rows that they belong to."""
     slots = 2 * min(torch.cuda.get_device_properties(device).multi_processor_count, MLA_MAX_CTAS)
     return {"o_part": torch.empty((slots, 16, 512), device=device, dtype=torch.float32),
             "ml_part": torch.empty((slots, 16, 2), device=device, dtype=torch.float32),
-            "row_sync": torch.zeros(rows, device=device, dtype=torch.int32)}
+            "cuts": torch.empty((slots // 2, 4), device=device, dtype=torch.int32)}
 
 
 def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                   positions: torch.Tensor, page_size: int, softmax_scale: float, o_lat: torch.Tensor,
-                  o_part: torch.Tensor, ml_part: torch.Tensor, row_sync: torch.Tensor,
+                  o_part: torch.Tensor, ml_part: torch.Tensor, cuts: torch.Tensor,
                   seq_rows: torch.Tensor | None = None) -> torch.Tensor:
     """Latent attention over the paged 4-bit cache (dsv2_mla_decode_q4_args in include/dsv2.h):
     query row r attends positions 0 .. positions[r] of block-table row seq_rows[r] (default r);
@@ -687,7 +687,7 @@ def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tenso
         _need(positions, "positions", torch.int64, rows),
         None if seq_rows is None else _need(seq_rows, "seq_rows", torch.int32, rows), softmax_scale,
         _need(o_lat, "o_lat", torch.bfloat16), _need(o_part, "o_part", torch.float32, slots * 16 * 512),
-        _need(ml_part, "ml_part", torch.float32, slots * 16 * 2), _need(row_sync, "row_sync", torch.int32, rows), slots)
+        _need(ml_part, "ml_part", torch.float32, slots * 16 * 2), _need(cuts, "cuts", torch.int32, slots // 2 * 4), slots)
     _lib.call("dsv2_mla_decode_q4", ctypes.byref(a), _here(q_abs))
     return o_lat
 

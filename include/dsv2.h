@@ -659,7 +659,7 @@ typedef struct dsv2_mla_decode_q4_args {
   void* o_lat;                 /* [rows, 16, 512] bf16 */
   float* o_part;               /* work buffer [part_slots, 16, 512] */
   float* ml_part;              /* work buffer [part_slots, 16, 2] */
-  int32_t* row_sync;           /* [rows], zero before the first call and left zero by every call */
+  int32_t* cuts;               /* work buffer [part_slots / 2, 4] */
   int32_t part_slots;          /* two per CTA: 2 * SMs for the whole GPU, at least 2 */
 } dsv2_mla_decode_q4_args;
 

@@ -147,4 +147,4 @@ def test_python_wrappers_refuse_cpu_tensors_and_wrong_shapes():
 
 
 def _ws(ops):
-    return {"o_part": torch.zeros(2, 16, 512), "ml_part": torch.zeros(2, 16, 2), "row_sync": torch.zeros(2, dtype=torch.int32)}
+    return {"o_part": torch.zeros(2, 16, 512), "ml_part": torch.zeros(2, 16, 2), "cuts": torch.zeros(1, 4, dtype=torch.int32)}
