@@ -17,7 +17,11 @@ constexpr int kQ4ScoreWarps = 8;                             // a block of a til
 constexpr int kQ4PvWarps = 8;                                // 64 latent dims each
 constexpr int kQ4Compute = (kQ4ScoreWarps + kQ4PvWarps) * 32;
 constexpr int kQ4ProducerWarp = kQ4ScoreWarps + kQ4PvWarps;  // warp 16: copies
-constexpr int kQ4Threads = kQ4Compute + 32;
+constexpr int kQ4Threads = kQ4Compute + 128;                 // a whole warpgroup of which one warp works
+// registers a thread: the launch gives 20 warps 96 each; the copy warpgroup hands most of its own on
+constexpr int kQ4LaunchRegs = 96, kQ4CopyRegs = 24, kQ4ScoreRegs = 120, kQ4PvRegs = 104;
+static_assert(4 * kQ4CopyRegs + kQ4ScoreWarps * kQ4ScoreRegs + kQ4PvWarps * kQ4PvRegs <= kQ4Threads / 32 * kQ4LaunchRegs,
+              "register shares exceed the launch's");
 constexpr int kQ4QBytes = kHeads * (1024 + 128);             // a query row: q_abs, then q_pe
 constexpr int kQ4Steps = 32;                                 // k-steps of 16 latent dims; 4 roped ones follow
 constexpr int kQ4PRow = kQ4Pos + 8;                          // row of P
@@ -34,6 +38,10 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 __device__ __forceinline__ void q4_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // barrier 1 over the score warps that also says whether any thread's predicate holds
 __device__ __forceinline__ bool q4_bar_any(bool pred) {
@@ -291,8 +299,10 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
     return St >= start && St + nblk <= end;   // wholly in the range
   };
 
-  if (warp == kQ4ProducerWarp) {
+  if (warp >= kQ4ProducerWarp) {
     // ================= producer warp
+    regs_dec<kQ4CopyRegs>();
+    if (warp > kQ4ProducerWarp) return;
     if (lane == 0) {
       // the second CTA of a cut row notes the row, its first partial slot and their number; every
       // CTA writes its entry, also one whose range holds no block (per-row units alone)
@@ -382,6 +392,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
 
   if (warp < kQ4ScoreWarps) {
     // ================= score warps
+    regs_inc<kQ4ScoreRegs>();
     const uint32_t m1024 = q4_opaque(0x64006400u), m64 = q4_opaque(0x54005400u);
     // B fragment column gq of the 8 positions of half i of a block: token 8 i + (gq >> 1) + 4 (gq & 1);
     // lane tq takes groups 4 gi + tq
@@ -595,6 +606,7 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
   } else {
     // ================= P V warps: latent dims [64 pv, 64 pv + 64); lane gq owns dims 64 pv + 8 gq
     // .. + 8, one word, whose dim t is column gq of n-tile t; lane tq takes tokens tq + 4 i
+    regs_inc<kQ4PvRegs>();
     const uint32_t m128 = q4_opaque(0x43004300u);
     const int pv = warp - kQ4ScoreWarps;
     const int grp = 2 * pv + (gq >> 2);
