@@ -25,6 +25,7 @@ static_assert(4 * kQ4CopyRegs + kQ4ScoreWarps * kQ4ScoreRegs + kQ4PvWarps * kQ4P
 constexpr int kQ4QBytes = kHeads * (1024 + 128);             // a query row: q_abs, then q_pe
 constexpr int kQ4Steps = 32;                                 // k-steps of 16 latent dims; 4 roped ones follow
 constexpr int kQ4PRow = kQ4Pos + 8;                          // row of P
+constexpr float kQ4VUp = 256.f;                              // the P V product's values are v / 256
 constexpr float kQ4Slack = 8.f;                              // log2 growth of a row's maximum left unscaled
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -115,19 +116,27 @@ __device__ __forceinline__ uint32_t q4_lo(uint32_t w, const Q4Scale& c, uint32_t
 __device__ __forceinline__ uint32_t q4_hi(uint32_t w, const Q4Scale& c, uint32_t m64) { return h2fma(q4_under<0x00f000f0u>(w, m64), c.s, c.b4); }
 
 // Nibble pairs to the bf16 pairs of the P V product: P spans more binades than fp16 has (a
-// probability far below the row's largest still decides a dim in which that token is 0).  bf16
-// holds 128 + q for a nibble at bits 3..0 only.  A code in bits 11..4 of a bf16 number is the
-// scale times 2^-112 (subnormals included), so the scale and -136 times it are one product each.
+// probability far below the row's largest still decides a dim in which that token is 0).  A nibble q
+// at bits 3..0 of a half, under the bits of 128, is the bf16 number 128 + q.  One at bits 7..4 alone
+// is q 2^-129: bit 7 is the lowest exponent bit, and subnormals and the first binade have the same
+// spacing.  So one shift serves four nibbles here too.  To keep the factor of the second kind finite
+// all values come out as v 2^-8, made up for at the end.  A code in bits 11..4 of a bf16 number is the
+// scale times 2^-112 (subnormals included); every product and fma below is exact (at most 8 bits).
 struct Q4ScaleB {
-  uint32_t s, b;        // scale pair, -136 s
+  uint32_t m0, b0;      // scale 2^-8 and -136 times it
+  uint32_t m1, b1;      // scale 2^121 and -8 scale 2^-8
 };
 __device__ __forceinline__ Q4ScaleB q4_scale_b(uint32_t codes) {
   Q4ScaleB r;
-  r.s = b2mul(codes << 4, 0x77807780u);   // 2^112
-  r.b = b2mul(codes << 4, 0xfb08fb08u);   // -136 * 2^112
+  const uint32_t raw = codes << 4;
+  r.m0 = b2mul(raw, 0x73807380u);                        // 2^104
+  r.b0 = b2mul(raw, 0xf708f708u);                        // -136 * 2^104
+  r.m1 = b2mul(b2mul(raw, 0x7f007f00u), 0x74807480u);    // 2^127, then 2^106
+  r.b1 = b2mul(raw, 0xf500f500u);                        // -2^107
   return r;
 }
-__device__ __forceinline__ uint32_t q4_b(uint32_t w, const Q4ScaleB& c, uint32_t m128) { return b2fma(q4_under<0x000f000fu>(w, m128), c.s, c.b); }
+__device__ __forceinline__ uint32_t q4_b_lo(uint32_t w, const Q4ScaleB& c, uint32_t m128) { return b2fma(q4_under<0x000f000fu>(w, m128), c.m0, c.b0); }
+__device__ __forceinline__ uint32_t q4_b_hi(uint32_t w, const Q4ScaleB& c) { return b2fma(w & 0x00f000f0u, c.m1, c.b1); }
 
 // Bounded mbarrier wait, a loop of four instructions: the waiting warps share the issue slots with
 // the working ones.  It gives up after 2^24 polls (seconds), and at once when this CTA already has.
@@ -587,8 +596,8 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
             L0 += sm.lsum[w][gq];
             L1 += sm.lsum[w][gq + 8];
           }
-          sm.fin[fb][gq] = L0 > 0.f ? 1.f / L0 : (L0 == 0.f ? 0.f : L0);   // NaN stays NaN
-          sm.fin[fb][gq + 8] = L1 > 0.f ? 1.f / L1 : (L1 == 0.f ? 0.f : L1);
+          sm.fin[fb][gq] = L0 > 0.f ? kQ4VUp / L0 : (L0 == 0.f ? 0.f : L0);   // NaN stays NaN
+          sm.fin[fb][gq + 8] = L1 > 0.f ? kQ4VUp / L1 : (L1 == 0.f ? 0.f : L1);
           if (!complete) {
             float* ml = p.ml_part + (c * 2 + mla_slot(S, start)) * kHeads * 2;
             ml[gq * 2] = m0;
@@ -659,11 +668,15 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
           // even dims of the word are its low half's nibbles, odd ones the high half's
           const uint32_t e01 = __byte_perm(w0, w1, 0x5410), d01 = __byte_perm(w0, w1, 0x7632);
           const uint32_t e23 = __byte_perm(w2, w3, 0x5410), d23 = __byte_perm(w2, w3, 0x7632);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            mma_bf16_16816(o[2 * i], pa, q4_b(e01 >> (4 * i), c01, m128), q4_b(e23 >> (4 * i), c23, m128));
-            mma_bf16_16816(o[2 * i + 1], pa, q4_b(d01 >> (4 * i), c01, m128), q4_b(d23 >> (4 * i), c23, m128));
-          }
+          mma_bf16_16816(o[0], pa, q4_b_lo(e01, c01, m128), q4_b_lo(e23, c23, m128));
+          mma_bf16_16816(o[1], pa, q4_b_lo(d01, c01, m128), q4_b_lo(d23, c23, m128));
+          mma_bf16_16816(o[2], pa, q4_b_hi(e01, c01), q4_b_hi(e23, c23));
+          mma_bf16_16816(o[3], pa, q4_b_hi(d01, c01), q4_b_hi(d23, c23));
+          const uint32_t f01 = e01 >> 8, g01 = d01 >> 8, f23 = e23 >> 8, g23 = d23 >> 8;
+          mma_bf16_16816(o[4], pa, q4_b_lo(f01, c01, m128), q4_b_lo(f23, c23, m128));
+          mma_bf16_16816(o[5], pa, q4_b_lo(g01, c01, m128), q4_b_lo(g23, c23, m128));
+          mma_bf16_16816(o[6], pa, q4_b_hi(f01, c01), q4_b_hi(f23, c23));
+          mma_bf16_16816(o[7], pa, q4_b_hi(g01, c01), q4_b_hi(g23, c23));
         };
         if (jt + kQ4TileBlocks < nblk && nb == kQ4TileBlocks) {   // whole blocks only: no branch between them
 #pragma unroll
@@ -743,7 +756,7 @@ __global__ __launch_bounds__(256) void mla_q4_merge_kernel(const MlaQ4Params p) 
       den += w * l;
     }
     den = warp_sum(den);
-    if (tid == 0) s_inv = den != 0.f ? 1.f / den : 0.f;
+    if (tid == 0) s_inv = den != 0.f ? kQ4VUp / den : 0.f;
   }
   __syncthreads();
   const int g = tid >> 6, d = tid & 63;
