@@ -33,6 +33,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+// (not volatile, unlike mma_bf16_16816: the compiler may move loads and conversions between them)
+__device__ __forceinline__ void q4_mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -508,8 +514,8 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const uint4 u = *reinterpret_cast<const uint4*>(kv + off_r + 1024 * j + 64 * (h ^ (tok >> 2)));
-              mma_bf16_16816(s[j], a0, u.x, u.y);
-              mma_bf16_16816(s[j], a1, u.z, u.w);
+              q4_mma_bf16(s[j], a0, u.x, u.y);
+              q4_mma_bf16(s[j], a1, u.z, u.w);
             }
           }
           const int t0 = (jt + warp) * kL4Tokens + tq;   // columns 2 tq, 2 tq + 1: tokens t0 + 8 j, + 4
@@ -647,43 +653,59 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
         const int nb = min(kQ4TileBlocks, j1 - jt);
         const unsigned char* tile = sm.ring[st];
         const uint32_t p_row = smem_u32(&sm.p[buf][(mi & 1) * 8 + ri][(mi >> 1) * 8]);
-        auto block = [&](int b, bool tail) {
+        // what a lane needs of a block; the next block's is on its way while one is computed
+        struct Part {
+          uint32_t pa[4], w0, w1, w2, w3, sw;
+        };
+        auto load = [&](int b) {
           const unsigned char* kv = tile + b * kL4BlockBytes;
-          uint32_t pa[4];
-          ldmatrix_x4(p_row + 32 * b, pa[0], pa[1], pa[2], pa[3]);
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kv + off0);
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kv + off1);
-          const uint32_t w2 = *reinterpret_cast<const uint32_t*>(kv + off0 + 2048);
-          const uint32_t w3 = *reinterpret_cast<const uint32_t*>(kv + off1 + 2048);
-          uint32_t sw = *reinterpret_cast<const uint32_t*>(kv + off_s);
-          if (tail) {
-            // tokens past the row's length may hold anything, and P = 0 does not cancel an infinity:
-            // give them a finite scale
-            const int rem = len - (jt + b) * kL4Tokens;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (tq + 4 * i >= rem) sw &= ~(0xffu << (8 * i));
-          }
-          const Q4ScaleB c01 = q4_scale_b(__byte_perm(sw, 0, 0x4140)), c23 = q4_scale_b(__byte_perm(sw, 0, 0x4342));
+          Part q;
+          ldmatrix_x4(p_row + 32 * b, q.pa[0], q.pa[1], q.pa[2], q.pa[3]);
+          q.w0 = *reinterpret_cast<const uint32_t*>(kv + off0);
+          q.w1 = *reinterpret_cast<const uint32_t*>(kv + off1);
+          q.w2 = *reinterpret_cast<const uint32_t*>(kv + off0 + 2048);
+          q.w3 = *reinterpret_cast<const uint32_t*>(kv + off1 + 2048);
+          q.sw = *reinterpret_cast<const uint32_t*>(kv + off_s);
+          return q;
+        };
+        auto block = [&](const Part& q) {
+          const Q4ScaleB c01 = q4_scale_b(__byte_perm(q.sw, 0, 0x4140)), c23 = q4_scale_b(__byte_perm(q.sw, 0, 0x4342));
           // even dims of the word are its low half's nibbles, odd ones the high half's
-          const uint32_t e01 = __byte_perm(w0, w1, 0x5410), d01 = __byte_perm(w0, w1, 0x7632);
-          const uint32_t e23 = __byte_perm(w2, w3, 0x5410), d23 = __byte_perm(w2, w3, 0x7632);
-          mma_bf16_16816(o[0], pa, q4_b_lo(e01, c01, m128), q4_b_lo(e23, c23, m128));
-          mma_bf16_16816(o[1], pa, q4_b_lo(d01, c01, m128), q4_b_lo(d23, c23, m128));
-          mma_bf16_16816(o[2], pa, q4_b_hi(e01, c01), q4_b_hi(e23, c23));
-          mma_bf16_16816(o[3], pa, q4_b_hi(d01, c01), q4_b_hi(d23, c23));
+          const uint32_t e01 = __byte_perm(q.w0, q.w1, 0x5410), d01 = __byte_perm(q.w0, q.w1, 0x7632);
+          const uint32_t e23 = __byte_perm(q.w2, q.w3, 0x5410), d23 = __byte_perm(q.w2, q.w3, 0x7632);
+          q4_mma_bf16(o[0], q.pa, q4_b_lo(e01, c01, m128), q4_b_lo(e23, c23, m128));
+          q4_mma_bf16(o[1], q.pa, q4_b_lo(d01, c01, m128), q4_b_lo(d23, c23, m128));
+          q4_mma_bf16(o[2], q.pa, q4_b_hi(e01, c01), q4_b_hi(e23, c23));
+          q4_mma_bf16(o[3], q.pa, q4_b_hi(d01, c01), q4_b_hi(d23, c23));
           const uint32_t f01 = e01 >> 8, g01 = d01 >> 8, f23 = e23 >> 8, g23 = d23 >> 8;
-          mma_bf16_16816(o[4], pa, q4_b_lo(f01, c01, m128), q4_b_lo(f23, c23, m128));
-          mma_bf16_16816(o[5], pa, q4_b_lo(g01, c01, m128), q4_b_lo(g23, c23, m128));
-          mma_bf16_16816(o[6], pa, q4_b_hi(f01, c01), q4_b_hi(f23, c23));
-          mma_bf16_16816(o[7], pa, q4_b_hi(g01, c01), q4_b_hi(g23, c23));
+          q4_mma_bf16(o[4], q.pa, q4_b_lo(f01, c01, m128), q4_b_lo(f23, c23, m128));
+          q4_mma_bf16(o[5], q.pa, q4_b_lo(g01, c01, m128), q4_b_lo(g23, c23, m128));
+          q4_mma_bf16(o[6], q.pa, q4_b_hi(f01, c01), q4_b_hi(f23, c23));
+          q4_mma_bf16(o[7], q.pa, q4_b_hi(g01, c01), q4_b_hi(g23, c23));
         };
         if (jt + kQ4TileBlocks < nblk && nb == kQ4TileBlocks) {   // whole blocks only: no branch between them
+          Part cur = load(0);
 #pragma unroll
-          for (int b = 0; b < kQ4TileBlocks; ++b) block(b, false);
+          for (int b = 0; b < kQ4TileBlocks; ++b) {
+            Part nxt = cur;
+            if (b + 1 < kQ4TileBlocks) nxt = load(b + 1);
+            block(cur);
+            cur = nxt;
+          }
         } else {
 #pragma unroll 1
-          for (int b = 0; b < nb; ++b) block(b, jt + b == nblk - 1);
+          for (int b = 0; b < nb; ++b) {
+            Part q = load(b);
+            if (jt + b == nblk - 1) {
+              // tokens past the row's length may hold anything, and P = 0 does not cancel an infinity:
+              // give them a finite scale
+              const int rem = len - (jt + b) * kL4Tokens;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (tq + 4 * i >= rem) q.sw &= ~(0xffu << (8 * i));
+            }
+            block(q);
+          }
         }
         __syncwarp();
         if (lane == 0) {
