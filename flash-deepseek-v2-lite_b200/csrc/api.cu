@@ -77,6 +77,8 @@ int ensure_init(int* sms_out) {
       return fail(DSV2_ERR_LAUNCH, "mla_tc_init: %s", cudaGetErrorString(e));
     if ((e = mla_q4_init()) != cudaSuccess)
       return fail(DSV2_ERR_LAUNCH, "mla_q4_init: %s", cudaGetErrorString(e));
+    if ((e = lora_gemm_init()) != cudaSuccess)
+      return fail(DSV2_ERR_LAUNCH, "lora_gemm_init: %s", cudaGetErrorString(e));
     if ((e = mla_noalloc_lookup(&g_noalloc_scratch[dev])) != cudaSuccess)
       return fail(DSV2_ERR_LAUNCH, "scratch address of the allocation-free entry point: %s", cudaGetErrorString(e));
     if ((e = router_fused_max_clusters(&g_router_clusters[dev])) != cudaSuccess)

@@ -6,6 +6,12 @@ namespace {
 
 // up to here a shared projection with one partial runs the small (GEMV) family
 constexpr int kLoraGemvTokens = 8;
+// The projection and its adapters are one GEMM above 256 tokens with 16 or more per adapter: it pays a
+// pass that orders the tokens and a step per 64 ranks of every adapter in a tile, and saves the fp32
+// partials.  n 3648, k 2048, rank 32, one GEMM / separate launches: 257 tokens 25 / 29 us with 1 adapter,
+// 30 / 29 with 16, 54 / 35 with 64; 1024 tokens 35 / 39 with 1, 41 / 40 with 64; 768 tokens 42 / 50 with
+// 64.  Up to 256 tokens the projection reads its weights once either way.
+constexpr int kLoraGemmTokens = 256, kLoraGemmPerAdapter = 16;
 constexpr int kQ4MinUnits = 4;   // 64 positions: shorter pieces cost more in merges than they save
 
 // rows of a latent4 call: [n, 576] bf16 with 16-byte aligned rows
@@ -150,7 +156,10 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   if (a->tokens < 0 || a->adapters < 0 || a->n_base < 0 || a->ids_len < 0)
     return fail(DSV2_ERR_INVALID, "lora: tokens %d adapters %d partials %d", a->tokens, a->adapters, a->n_base);
   if (a->tokens == 0) return DSV2_OK;
-  if (a->w && (!a->base || a->n_base < 1)) return fail(DSV2_ERR_INVALID, "lora: w needs base and n_base for its partials");
+  // a long run of tokens: one GEMM over the tokens in adapter order, no partials
+  const bool fused = a->w && a->xs && a->lists && a->tokens > kLoraGemmTokens &&
+                     a->tokens >= static_cast<long long>(kLoraGemmPerAdapter) * a->adapters && a->y_dtype == DSV2_BF16 && a->k % 64 == 0;
+  if (a->w && !fused && (!a->base || a->n_base < 1)) return fail(DSV2_ERR_INVALID, "lora: w needs base and n_base for its partials");
   if (!a->x || !a->ids || !a->y || !a->low || (a->adapters > 0 && (!a->a || !a->b || !a->ranks || !a->scales)) ||
       (a->n_base > 0 && !a->base))
     return fail(DSV2_ERR_INVALID, "lora: null pointer");
@@ -167,7 +176,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
     return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
   int sms = 0;
   if (int rc = ensure_init(&sms)) return rc;
-  if (a->w) {
+  if (a->w && !fused) {
     dsv2_linear_args l = {};
     l.w = a->w;
     l.w_row_stride = a->w_row_stride;
@@ -212,7 +221,22 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   p.y = a->y;
   p.y_f32 = a->y_dtype == DSV2_F32;
   p.y_row_stride = a->y_row_stride;
-  return check_launch(launch_lora(p, sms, static_cast<cudaStream_t>(stream)), "lora");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!fused) return check_launch(launch_lora(p, sms, st), "lora");
+  if (!aligned16(a->w) || !aligned16(a->xs) || !aligned16(a->lists) || a->w_row_stride % 8 || a->w_row_stride < a->k)
+    return fail(DSV2_ERR_INVALID, "lora: w, xs and lists must be 16-byte aligned");
+  p.xs = static_cast<bf16*>(a->xs);
+  p.lists = a->lists;
+  p.base_parts = 0;
+  const int n_tile = lora_gemm_tile(a->tokens, a->n, sms);
+  const uint64_t T = static_cast<uint64_t>(a->tokens), N = static_cast<uint64_t>(a->n), K = static_cast<uint64_t>(a->k);
+  const uint64_t ws = static_cast<uint64_t>(a->w_row_stride) * 2;
+  CUtensorMap tm_x, tm_w;
+  if (int rc = tensor_map_3d(a->xs, K, T, 1, lg_row(a->k, a->rank) * 2, T * lg_row(a->k, a->rank) * 2, kLgRows, &tm_x)) return rc;
+  if (int rc = tensor_map_3d(a->w, K, N, 1, ws, N * ws, static_cast<uint32_t>(n_tile / 2), &tm_w)) return rc;
+  if (int rc = check_launch(launch_lora_low(p, sms, st), "lora: low")) return rc;
+  if (int rc = check_launch(launch_lora_gather(p, st), "lora: gather")) return rc;
+  return check_launch(launch_lora_gemm(p, tm_x, tm_w, n_tile, sms, st), "lora: gemm");
 }
 
 }  // extern "C"

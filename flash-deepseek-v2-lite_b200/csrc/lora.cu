@@ -117,6 +117,22 @@ __device__ __forceinline__ uint4 ld_or_zero(const void* q, bool in) {
   return in ? __ldg(reinterpret_cast<const uint4*>(q)) : make_uint4(0, 0, 0, 0);
 }
 
+// bf16 values that are not finite -> 0
+__device__ __forceinline__ bool drop_nonfinite(uint4& v) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+  __nv_bfloat162 sick = zero;   // 0 * x + 0 is a NaN for those alone
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sick = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(w + i), zero, sick);
+  if (!(__hisnan(__low2bfloat16(sick)) || __hisnan(__high2bfloat16(sick)))) return false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
+  }
+  return true;
+}
+
 // low partials of one tile and k split: low[split, t, j].  NT = rank / 8 n-tiles of 8 ranks.
 template <int NT>
 __global__ __launch_bounds__(kLoraLowWarps * 32) void lora_low_kernel(const LoraParams p) {
@@ -213,7 +229,8 @@ __global__ __launch_bounds__(kLoraOutWarps * 32, 4) void lora_out_kernel(const L
     }
     const uint32_t hi = pack_bf16x2(v0, v1);
     s_hi[r][pair] = hi;
-    s_lo[r][pair] = pack_bf16x2(v0 - bf16lo(hi), v1 - bf16hi(hi));
+    // (an infinite high part is all there is: inf - inf would make it a NaN)
+    s_lo[r][pair] = pack_bf16x2(isinf(bf16lo(hi)) ? 0.f : v0 - bf16lo(hi), isinf(bf16hi(hi)) ? 0.f : v1 - bf16hi(hi));
   }
   __syncthreads();
   const int col = blockIdx.x * (kChunks * kLoraOutCols) + warp * 32;
@@ -289,13 +306,18 @@ __global__ __launch_bounds__(kLoraOutWarps * 32, 4) void lora_out_kernel(const L
         const uint32_t al0[4] = {l0.x, l1.x, l0.y, l1.y}, al1[4] = {l0.z, l1.z, l0.w, l1.w};
         __syncwarp();
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], ah0, b[u].x, b[u].y);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], al0, b[u].x, b[u].y);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], ah1, b[u].z, b[u].w);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mma_bf16_16816(acc[u], al1, b[u].z, b[u].w);
+        for (int u = 0; u < 4; ++u) {
+          float d[4] = {acc[u][0], acc[u][1], acc[u][2], acc[u][3]};
+          mma_bf16_16816(d, ah0, b[u].x, b[u].y);
+          mma_bf16_16816(d, ah1, b[u].z, b[u].w);
+          drop_nonfinite(b[u]);   // the low part may have the other sign or be 0: infinities are the high part's
+          __syncwarp();
+          mma_bf16_16816(d, al0, b[u].x, b[u].y);
+          mma_bf16_16816(d, al1, b[u].z, b[u].w);
+          // other adapters' rows have zeros here, but 0 times an infinity of this B would still reach them
+          if (ad0 == ai) acc[u][0] = d[0], acc[u][1] = d[1];
+          if (ad1 == ai) acc[u][2] = d[2], acc[u][3] = d[3];
+        }
       }
     }
 #pragma unroll
@@ -315,18 +337,27 @@ __global__ __launch_bounds__(kLoraOutWarps * 32, 4) void lora_out_kernel(const L
 
 // Launch shapes.  A tile of few tokens can hold many adapters: with few tiles they are dealt out to
 // 4 CTAs.  With many tiles a CTA of the second product takes 512 columns, which share its set-up.
-cudaError_t launch_lora(const LoraParams& p, int num_sms, cudaStream_t st) {
-  const int tiles = (p.tokens + kLoraTile - 1) / kLoraTile;
-  const int deal = p.tokens > 1 && tiles < num_sms / 4 ? 4 : 1;
+static int lora_deal(const LoraParams& p, int num_sms) {
+  return p.tokens > 1 && (p.tokens + kLoraTile - 1) / kLoraTile < num_sms / 4 ? 4 : 1;
+}
+
+// order (when there is one) and low
+cudaError_t launch_lora_low(const LoraParams& p, int num_sms, cudaStream_t st) {
   if (p.order) launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, kLoraSortThreads, 0, st, p);
-  const dim3 grid(tiles, p.low_parts, deal), block(kLoraLowWarps * 32);
+  const dim3 grid((p.tokens + kLoraTile - 1) / kLoraTile, p.low_parts, lora_deal(p, num_sms)), block(kLoraLowWarps * 32);
   if (p.rank <= 16) launch_kernel(lora_low_kernel<2>, grid, block, 0, st, p);
   else if (p.rank <= 32) launch_kernel(lora_low_kernel<4>, grid, block, 0, st, p);
   else if (p.rank <= 64) launch_kernel(lora_low_kernel<8>, grid, block, 0, st, p);
   else launch_kernel(lora_low_kernel<16>, grid, block, 0, st, p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_lora(const LoraParams& p, int num_sms, cudaStream_t st) {
+  if (cudaError_t e = launch_lora_low(p, num_sms, st)) return e;
+  const int tiles = (p.tokens + kLoraTile - 1) / kLoraTile;
   const unsigned cols = (p.n + kLoraOutCols - 1) / kLoraOutCols;
   if (tiles >= num_sms) launch_kernel(lora_out_kernel<2>, dim3((cols + 1) / 2, tiles), kLoraOutWarps * 32, 0, st, p);
-  else launch_kernel(lora_out_kernel<1>, dim3(cols, tiles, deal), kLoraOutWarps * 32, 0, st, p);
+  else launch_kernel(lora_out_kernel<1>, dim3(cols, tiles, lora_deal(p, num_sms)), kLoraOutWarps * 32, 0, st, p);
   return cudaGetLastError();
 }
 

@@ -181,6 +181,8 @@ struct LoraParams {
   void* y;                     // [tokens, n] bf16 or fp32
   int y_f32;
   long long y_row_stride;
+  bf16* xs;                    // long runs of tokens: [tokens, k + rank rounded up to 64] work buffer, x and low in adapter order
+  int* lists;                  // [ceil(tokens / 256), 2 + 512 ceil(rank / 16)] work buffer, adapters of each token tile
 };
 
 struct MlaDecodeParams {
@@ -250,6 +252,12 @@ cudaError_t launch_page_plan(const PagePlanParams&, int num_sms, cudaStream_t);
 cudaError_t mla_q4_init();
 cudaError_t launch_mla_q4(const MlaQ4Params&, int num_sms, cudaStream_t);
 cudaError_t launch_lora(const LoraParams&, int num_sms, cudaStream_t);
+cudaError_t launch_lora_low(const LoraParams&, int num_sms, cudaStream_t);
+cudaError_t lora_gemm_init();
+int lora_gemm_tile(int tokens, int n, int num_sms);
+cudaError_t launch_lora_gather(const LoraParams&, cudaStream_t);
+cudaError_t launch_lora_gemm(const LoraParams&, const CUtensorMap& tm_x, const CUtensorMap& tm_w, int n_tile, int num_sms,
+                             cudaStream_t);
 cudaError_t mla_decode_init();
 int mla_decode_grid(const MlaDecodeParams&, int num_sms, long long part_slots);
 cudaError_t launch_mla_decode(const MlaDecodeParams&, const CUtensorMap& tm_kv, const CUtensorMap& tm_qa,

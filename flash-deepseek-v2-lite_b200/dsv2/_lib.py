@@ -134,7 +134,7 @@ class LoraArgs(ctypes.Structure):
         ("ranks", c_vp), ("scales", c_vp), ("w", c_vp), ("w_row_stride", c_i64), ("base", c_vp), ("base_part_stride", c_i64),
         ("base_row_stride", c_i64), ("low", c_vp), ("order", c_vp), ("y", c_vp),
         ("y_row_stride", c_i64), ("low_parts", c_i32), ("y_dtype", c_i32), ("n_base", c_i32), ("ids_len", c_i32), ("adapters", c_i32), ("rank", c_i32),
-        ("tokens", c_i32), ("k", c_i32), ("n", c_i32),
+        ("tokens", c_i32), ("k", c_i32), ("n", c_i32), ("xs", c_vp), ("lists", c_vp),
     ]
 
 

@@ -191,7 +191,7 @@ class DecodeEngine:
         if self.adapters is not None:
             self.lora_ws = ops.lora_workspace(B, QKVA_ROWS, HIDDEN, self.adapters.rank, dev)
             if self.split_k:
-                del self.lora_ws["parts"]
+                self.lora_ws = {k: self.lora_ws[k] for k in ("low", "order")}
         self.q_abs = torch.zeros((B, N_HEADS, KV_LORA), device=dev, dtype=bf)
         self.o_lat = torch.zeros((B, N_HEADS, KV_LORA), device=dev, dtype=bf)
         self.attn_o = torch.zeros((B, N_HEADS * V_DIM), device=dev, dtype=bf)

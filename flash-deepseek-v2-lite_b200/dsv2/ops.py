@@ -692,7 +692,7 @@ def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tenso
     return o_lat
 
 
-def _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, base, token_row) -> None:
+def _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, base, token_row, xs=None, lists=None) -> None:
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1 or not x.is_cuda:
         raise NotImplementedError("x must be a CUDA bf16 tensor [tokens, k] with a contiguous last dimension")
     T, K = x.shape
@@ -722,6 +722,9 @@ def _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, base, token_row) -
         _need(low, "low", torch.float32, T * rank), None if order is None else _need(order, "order", torch.int32, 3 * T),
         y.data_ptr(), y.stride(0) if T > 1 else N, max(1, min(low.numel() // max(1, T * rank), 64)), y_dt, n_base,
         ids.numel(), n_ad, rank, T, K, N)
+    if xs is not None and lists is not None:
+        n_xs, n_lists = _lora_gemm_buffers(T, K, rank)
+        args.xs, args.lists = _need(xs, "xs", torch.bfloat16, n_xs[0] * n_xs[1]), _need(lists, "lists", torch.int32, n_lists[0] * n_lists[1])
     _lib.call("dsv2_lora", ctypes.byref(args), _here(x))
 
 
@@ -737,15 +740,27 @@ def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor
     return y
 
 
+def _lora_gemm_buffers(tokens: int, k: int, rank: int) -> tuple:
+    return (tokens, k + (rank + 63) // 64 * 64), ((tokens + 255) // 256, 2 + 512 * ((rank + 15) // 16))
+
+
 def lora_workspace(tokens: int, n: int, k: int, rank: int, device) -> dict:
-    """Work buffers of lora_linear: the shared projection's fp32 partials and the low-rank rows."""
+    """Work buffers of lora_linear: the low-rank rows, the tokens' order by adapter, the shared
+    projection's fp32 partials and, above 256 tokens, the activations in that order with the
+    adapters of each tile of tokens (xs, lists: the projection and the adapters are then one
+    GEMM if there are at least 16 tokens per adapter)."""
     sms = torch.cuda.get_device_properties(device).multi_processor_count
     splits = 1
-    if LORA_GEMV_TOKENS < tokens <= 256:   # decode batches: K split over the SMs, as the engine's projections
+    if LORA_GEMV_TOKENS < tokens <= LORA_GEMM_TOKENS:   # decode batches: K split over the SMs, as the engine's projections
         splits = max(1, min(sms // ((n + 127) // 128), k // 64, 5))
-    return {"parts": torch.empty((splits, tokens, n), device=device, dtype=torch.float32),
-            "low": torch.empty((lora_splits(tokens, k, sms), tokens, rank), device=device, dtype=torch.float32),
-            "order": torch.empty((3, tokens), device=device, dtype=torch.int32)}
+    ws = {"low": torch.empty((lora_splits(tokens, k, sms), tokens, rank), device=device, dtype=torch.float32),
+          "order": torch.empty((3, tokens), device=device, dtype=torch.int32),
+          "parts": torch.empty((splits, tokens, n), device=device, dtype=torch.float32)}
+    if tokens > LORA_GEMM_TOKENS and k % 64 == 0:
+        xs, lists = _lora_gemm_buffers(tokens, k, rank)
+        ws["xs"] = torch.empty(xs, device=device, dtype=torch.bfloat16)
+        ws["lists"] = torch.empty(lists, device=device, dtype=torch.int32)
+    return ws
 
 
 def lora_splits(tokens: int, k: int, num_sms: int) -> int:
@@ -755,12 +770,14 @@ def lora_splits(tokens: int, k: int, num_sms: int) -> int:
     return max(1, min(6 * num_sms // max(1, (tokens + 15) // 16), k // 256, 16))
 
 
-LORA_GEMV_TOKENS = 8   # up to here lora_linear's shared projection runs the small (GEMV) family
+LORA_GEMV_TOKENS = 8     # up to here lora_linear's shared projection runs the small (GEMV) family
+LORA_GEMM_TOKENS = 256   # above, the projection and its adapters can be one GEMM
 
 
 def lora_linear(*, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
                 ranks: torch.Tensor, scales: torch.Tensor, y: torch.Tensor, parts: torch.Tensor, low: torch.Tensor,
-                order: torch.Tensor | None = None, token_row: torch.Tensor | None = None) -> torch.Tensor:
+                order: torch.Tensor | None = None, xs: torch.Tensor | None = None, lists: torch.Tensor | None = None,
+                token_row: torch.Tensor | None = None) -> torch.Tensor:
     """The shared projection x @ w.T (w bf16 [N, K]) plus every token's low-rank adapter, rounded
     once to y's dtype: y[t] = w x[t] + scales[i] * b[i] (a[i] x[t]); see lora and
     lora_workspace."""
@@ -768,5 +785,5 @@ def lora_linear(*, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         raise NotImplementedError("lora_linear supports a CUDA bf16 w [N, K] with contiguous rows")
     if w.shape[1] != x.shape[-1] or w.shape[0] != y.shape[-1]:
         raise ValueError("lora_linear: inconsistent shapes of x, w and y")
-    _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, parts, token_row)
+    _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, parts, token_row, xs, lists)
     return y

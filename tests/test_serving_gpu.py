@@ -425,7 +425,7 @@ def test_attention_flags_pages_and_rows_out_of_range(D):
 
 
 # ------------------------------------------------------------------ adapters
-def lora_case(T, n_ad, rank, K, N, seed, none=0.2):
+def lora_case(T, n_ad, rank, K, N, seed, none=0.2, ranks=None):
     g = torch.Generator().manual_seed(seed)
 
     def bf(*shape, std=1.0):
@@ -436,6 +436,8 @@ def lora_case(T, n_ad, rank, K, N, seed, none=0.2):
          "scales": torch.rand(n_ad, generator=g) * 3 - 1}
     c["ids"][torch.rand(T, generator=g) < none] = -1
     c["ranks"][0] = rank
+    if ranks:
+        c["ranks"] = torch.tensor(ranks, dtype=torch.int32)
     # rows past an adapter's rank are not part of it, whatever they hold
     for i, r in enumerate(c["ranks"].tolist()):
         c["a"][i, r:] = math.nan
@@ -453,6 +455,7 @@ def check_lora(got, c, w=True, out_bits=8):
 @pytest.mark.parametrize("T,n_ad,rank,K,N", [
     (1, 1, 8, 64, 8), (1, 5, 16, 2048, 3648), (2, 3, 8, 128, 72), (7, 2, 64, 2048, 2048), (8, 9, 24, 192, 136),
     (9, 4, 16, 2048, 3648), (33, 33, 40, 256, 520), (100, 1, 128, 320, 264), (257, 7, 64, 2048, 1000),
+    (300, 33, 16, 128, 96), (1030, 64, 128, 128, 136), (2049, 1, 24, 64, 1288),
     (700, 20, 32, 2048, 512), (129, 3, 56, 10944, 128), (1100, 2, 8, 64, 40)])
 def test_lora_linear(D, T, n_ad, rank, K, N):
     c = lora_case(T, n_ad, rank, K, N, seed=T + N)
@@ -495,6 +498,27 @@ def test_lora_rows_without_adapter_keep_the_projection(D):
     y = torch.empty(50, 96, dtype=torch.bfloat16, device=DEV)
     D.lora_linear(**d, y=y, **D.lora_workspace(50, 96, 512, 8, DEV))
     check_lora(y, c)
+
+
+@pytest.mark.parametrize("T,rank,N", [(1, 8, 64), (6, 16, 72), (16, 40, 200), (100, 16, 264), (300, 24, 520), (520, 64, 104)])
+def test_lora_infinities_stay_with_their_adapter(D, T, rank, N):
+    c = lora_case(T, 3, rank, 256, N, seed=T, ranks=[rank, rank - 1, rank - 5])
+    c["ids"][0] = 1
+
+    def run():
+        y = torch.empty(T, N, dtype=torch.bfloat16, device=DEV)
+        D.lora_linear(**{k: v.to(DEV) for k, v in c.items()}, y=y, **D.lora_workspace(T, N, 256, rank, DEV))
+        return y.cpu()
+    clean = run()
+    c["b"][1, 3, 2], c["b"][1, N - 1, 0], c["b"][1, 17, rank - 2] = math.inf, math.nan, -math.inf
+    got = run()
+    own = c["ids"] == 1
+    assert torch.equal(got[~own], clean[~own])            # other adapters' tokens do not see them
+    keep = [n for n in range(N) if n not in (3, 17, N - 1)]
+    assert torch.equal(got[own][:, keep], clean[own][:, keep])
+    want, _, _ = S.lora(c["x"], c["w"], c["a"], c["b"], c["ids"].tolist(), c["ranks"], c["scales"])
+    assert torch.equal(got[own][:, [3, 17]].double(), want[own][:, [3, 17]])
+    assert bool(got[own][:, N - 1].isnan().all())
 
 
 def test_lora_flags_ids_out_of_range(D):
