@@ -6,12 +6,12 @@ namespace {
 
 // up to here a shared projection with one partial runs the small (GEMV) family
 constexpr int kLoraGemvTokens = 8;
-// The projection and its adapters are one GEMM above 256 tokens with 16 or more per adapter: it pays a
+// The projection and its adapters are one GEMM above 256 tokens with 12 or more per adapter: it pays a
 // pass that orders the tokens and a step per 64 ranks of every adapter in a tile, and saves the fp32
-// partials.  n 3648, k 2048, rank 32, one GEMM / separate launches: 257 tokens 25 / 29 us with 1 adapter,
-// 30 / 29 with 16, 54 / 35 with 64; 1024 tokens 35 / 39 with 1, 41 / 40 with 64; 768 tokens 42 / 50 with
-// 64.  Up to 256 tokens the projection reads its weights once either way.
-constexpr int kLoraGemmTokens = 256, kLoraGemmPerAdapter = 16;
+// partials.  n 3648, k 2048, rank 32, one GEMM / separate launches: 257 tokens 22 / 28 us with 1 adapter,
+// 27 / 29 with 16, 33 / 31 with 32; 1024 tokens 32 / 39 with 1, 38 / 40 with 64; 4001 with 6 74 / 134.
+// Up to 256 tokens the projection reads its weights once either way.
+constexpr int kLoraGemmTokens = 256, kLoraGemmPerAdapter = 12;
 constexpr int kQ4MinUnits = 4;   // 64 positions: shorter pieces cost more in merges than they save
 
 // rows of a latent4 call: [n, 576] bf16 with 16-byte aligned rows
@@ -234,8 +234,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   CUtensorMap tm_x, tm_w;
   if (int rc = tensor_map_3d(a->xs, K, T, 1, lg_row(a->k, a->rank) * 2, T * lg_row(a->k, a->rank) * 2, kLgRows, &tm_x)) return rc;
   if (int rc = tensor_map_3d(a->w, K, N, 1, ws, N * ws, static_cast<uint32_t>(n_tile / 2), &tm_w)) return rc;
-  if (int rc = check_launch(launch_lora_low(p, sms, st), "lora: low")) return rc;
-  if (int rc = check_launch(launch_lora_gather(p, st), "lora: gather")) return rc;
+  if (int rc = check_launch(launch_lora_rows(p, sms, st), "lora: rows")) return rc;
   return check_launch(launch_lora_gemm(p, tm_x, tm_w, n_tile, sms, st), "lora: gemm");
 }
 

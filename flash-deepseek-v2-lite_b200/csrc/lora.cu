@@ -117,6 +117,46 @@ __device__ __forceinline__ uint4 ld_or_zero(const void* q, bool in) {
   return in ? __ldg(reinterpret_cast<const uint4*>(q)) : make_uint4(0, 0, 0, 0);
 }
 
+// Tiles of the GEMM of lora_gemm.cu.
+constexpr int kLgRows = 128;          // tokens of a CTA's half of a tile
+constexpr int kLgM = 2 * kLgRows;     // tokens of a tile
+constexpr int kLgPiece = 16;          // ranks of a piece, the k of one tcgen05.mma
+// ints of a tile's list: the number of pieces, one unused, then (adapter, first rank | ranks << 16) each
+__host__ __device__ constexpr long long lg_list_ints(int rank) {
+  return 2 + 2LL * kLgM * ((rank + kLgPiece - 1) / kLgPiece);
+}
+// elements of a row of xs, x and then low as bf16 (of a token without an adapter: nothing): whole
+// 128-byte lines, which is what the GEMM's copies take
+__host__ __device__ constexpr long long lg_row(int k, int rank) { return k + (rank + 63LL) / 64 * 64; }
+
+// The pieces of a tile, by one warp.
+__device__ __forceinline__ void lora_list_pieces(const LoraParams& p, int tile) {
+  const int lane = threadIdx.x & 31;
+  int* list = p.lists + tile * lg_list_ints(p.rank);
+  int n = 0;
+  for (int q = 0; q < kLgM; q += 32) {
+    const int pos = tile * kLgM + q + lane;
+    const int a = pos < p.tokens ? p.order[p.tokens + pos] : -1;
+    // tokens are in adapter order: the first of each adapter lists its pieces
+    const bool first = a >= 0 && (q + lane == 0 || p.order[p.tokens + pos - 1] != a);
+    const int rank = first ? p.order[2 * p.tokens + pos] : 0, mine = (rank + kLgPiece - 1) / kLgPiece;
+    int at = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int u = __shfl_up_sync(0xffffffffu, at, d);
+      if (lane >= d) at += u;
+    }
+    const int sum = __shfl_sync(0xffffffffu, at, 31);
+    at += n - mine;
+    for (int c = 0; c < mine; ++c) {
+      list[2 + 2 * (at + c)] = a;
+      list[2 + 2 * (at + c) + 1] = c * kLgPiece | min(rank - c * kLgPiece, kLgPiece) << 16;
+    }
+    n += sum;
+  }
+  if (lane == 0) list[0] = n;
+}
+
 // bf16 values that are not finite -> 0
 __device__ __forceinline__ bool drop_nonfinite(uint4& v) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&v);
@@ -133,21 +173,48 @@ __device__ __forceinline__ bool drop_nonfinite(uint4& v) {
   return true;
 }
 
-// low partials of one tile and k split: low[split, t, j].  NT = rank / 8 n-tiles of 8 ranks.
-template <int NT>
-__global__ __launch_bounds__(kLoraLowWarps * 32) void lora_low_kernel(const LoraParams p) {
+__device__ __forceinline__ float ld_cluster_f32(const float* local, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(local, rank)) : "memory");
+  return v;
+}
+
+// low partials of one tile and k split: low[split, t, j].  NT = rank / 8 n-tiles of 8 ranks.  For the
+// GEMM of lora_gemm.cu (kSorted) the tile's rows of xs instead: x and the whole low as bf16, and the
+// pieces of each tile of that GEMM: one pass over x where a low of its own and a gather take two
+// (4001 tokens, k 2048, rank 32: 16 us for both, 16 + 10 us apart).  The k splits are then the CTAs of
+// a cluster, which sum through each other's shared memory.
+template <int NT, int kWarps, bool kSorted>
+__global__ __launch_bounds__(kWarps * 32) void lora_low_kernel(const LoraParams p) {
   pdl_enter();
   __shared__ LoraTile s;
-  __shared__ float s_sum[kLoraLowWarps][kLoraTile][8 * NT + 4];
+  __shared__ float s_sum[kWarps][kLoraTile][8 * NT + 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
   lora_tile(p, blockIdx.x, s);
+  if (kSorted) {
+    if (blockIdx.x % (kLgM / kLoraTile) == 0 && blockIdx.y == 0 && warp == kWarps - 1) lora_list_pieces(p, blockIdx.x / (kLgM / kLoraTile));
+    for (int r = blockIdx.y * kWarps + warp; r < kLoraTile && s.tok[r] >= 0; r += gridDim.y * kWarps) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.x + s.tok[r] * p.x_row_stride);
+      uint4* dst = reinterpret_cast<uint4*>(p.xs + (blockIdx.x * kLoraTile + r) * lg_row(p.k, p.rank));
+#pragma unroll 8
+      for (int j = lane; j < p.k / 8; j += 32) dst[j] = __ldg(src + j);
+    }
+  }
   // this CTA's k range, in steps of 32, and this warp's part of it
-  const int steps = (p.k + 31) / 32, splits = gridDim.y * kLoraLowWarps, part = blockIdx.y * kLoraLowWarps + warp;
+  const int steps = (p.k + 31) / 32, splits = gridDim.y * kWarps, part = blockIdx.y * kWarps + warp;
   const int k0 = static_cast<int>(static_cast<long long>(steps) * part / splits) * 32;
   const int k1 = static_cast<int>(static_cast<long long>(steps) * (part + 1) / splits) * 32;
   const int t0 = s.tok[gq], t1 = s.tok[gq + 8];
   const bf16* x0 = p.x + (t0 >= 0 ? t0 : 0) * p.x_row_stride;
   const bf16* x1 = p.x + (t1 >= 0 ? t1 : 0) * p.x_row_stride;
+  auto sync = [&]() {   // of those that share the sums
+    if (kSorted && gridDim.y > 1) {
+      cluster_arrive_release();
+      cluster_wait_acquire();
+    } else {
+      __syncthreads();
+    }
+  };
   // the adapters of a tile are dealt out to the CTAs that share it
   for (int ai = blockIdx.z; ai < s.n; ai += gridDim.z) {
     const int a = s.list[ai], rank = s.rank[ai], nt = (rank + 7) / 8;
@@ -173,7 +240,7 @@ __global__ __launch_bounds__(kLoraLowWarps * 32) void lora_low_kernel(const Lora
         }
       }
     }
-    __syncthreads();   // the previous adapter's sums have been read
+    sync();   // the previous adapter's sums have been read
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       s_sum[warp][gq][8 * n + 2 * tq] = acc[n][0];
@@ -181,17 +248,28 @@ __global__ __launch_bounds__(kLoraLowWarps * 32) void lora_low_kernel(const Lora
       s_sum[warp][gq + 8][8 * n + 2 * tq] = acc[n][2];
       s_sum[warp][gq + 8][8 * n + 2 * tq + 1] = acc[n][3];
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kLoraTile * 8 * NT; i += kLoraLowWarps * 32) {
+    sync();
+    const int part0 = kSorted ? blockIdx.y * kWarps * 32 : 0, parts = kSorted ? gridDim.y * kWarps * 32 : kWarps * 32;
+    for (int i = part0 + threadIdx.x; i < kLoraTile * 8 * NT; i += parts) {
       const int r = i / (8 * NT), j = i % (8 * NT);
       if (s.which[r] != ai || j >= p.rank) continue;
       float v = 0.f;
+      if (kSorted && gridDim.y > 1) {
+        for (uint32_t c = 0; c < gridDim.y; ++c) {
 #pragma unroll
-      for (int q = 0; q < kLoraLowWarps; ++q) v += s_sum[q][r][j];
+          for (int q = 0; q < kWarps; ++q) v += ld_cluster_f32(&s_sum[q][r][j], c);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kWarps; ++q) v += s_sum[q][r][j];
+      }
       // columns past the adapter's rank hold whatever its padding holds
-      p.low[(static_cast<long long>(blockIdx.y) * p.tokens + s.tok[r]) * p.rank + j] = j < rank ? v * scale : 0.f;
+      v = j < rank ? v * scale : 0.f;
+      if (kSorted) p.xs[(blockIdx.x * kLoraTile + r) * lg_row(p.k, p.rank) + p.k + j] = __float2bfloat16(v);
+      else p.low[(static_cast<long long>(blockIdx.y) * p.tokens + s.tok[r]) * p.rank + j] = v;
     }
   }
+  if (kSorted && gridDim.y > 1) sync();   // nobody reads this CTA's sums any more
 }
 
 // y: a tile of 16 tokens x kChunks blocks of 256 columns.  A warp takes 32 columns as two pairs of
@@ -200,7 +278,7 @@ __global__ __launch_bounds__(kLoraLowWarps * 32) void lora_low_kernel(const Lora
 // two bf16 numbers (16 significant bits), so that it adds no rounding of its own to y.  A CTA writes
 // the rows of its adapters (blockIdx.z 0 also those of none).
 template <int kChunks>
-__global__ __launch_bounds__(kLoraOutWarps * 32, 4) void lora_out_kernel(const LoraParams p) {
+__global__ __launch_bounds__(kLoraOutWarps * 32, 3) void lora_out_kernel(const LoraParams p) {
   pdl_enter();
   __shared__ LoraTile s;
   __shared__ __align__(16) uint32_t s_hi[kLoraTile][68], s_lo[kLoraTile][68];   // bf16 pairs, up to 128 ranks
@@ -341,23 +419,57 @@ static int lora_deal(const LoraParams& p, int num_sms) {
   return p.tokens > 1 && (p.tokens + kLoraTile - 1) / kLoraTile < num_sms / 4 ? 4 : 1;
 }
 
-// order (when there is one) and low
-cudaError_t launch_lora_low(const LoraParams& p, int num_sms, cudaStream_t st) {
-  if (p.order) launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, kLoraSortThreads, 0, st, p);
-  const dim3 grid((p.tokens + kLoraTile - 1) / kLoraTile, p.low_parts, lora_deal(p, num_sms)), block(kLoraLowWarps * 32);
-  if (p.rank <= 16) launch_kernel(lora_low_kernel<2>, grid, block, 0, st, p);
-  else if (p.rank <= 32) launch_kernel(lora_low_kernel<4>, grid, block, 0, st, p);
-  else if (p.rank <= 64) launch_kernel(lora_low_kernel<8>, grid, block, 0, st, p);
-  else launch_kernel(lora_low_kernel<16>, grid, block, 0, st, p);
-  return cudaGetLastError();
+template <int NT>
+static void launch_low(const LoraParams& p, int deal, cudaStream_t st) {
+  launch_kernel(lora_low_kernel<NT, kLoraLowWarps, false>, dim3((p.tokens + kLoraTile - 1) / kLoraTile, p.low_parts, deal), kLoraLowWarps * 32,
+                0, st, p);
+}
+
+template <int NT, int kWarps>
+static cudaError_t launch_rows(const LoraParams& p, int num_sms, cudaStream_t st) {
+  // CTAs that share a tile: while the GPU has room for more (three per SM) and each warp keeps 64 of k
+  const int tiles = (p.tokens + kLoraTile - 1) / kLoraTile;
+  unsigned share = 1;
+  while (share < 8 && 2 * share * tiles <= 3u * num_sms && 2 * share * kWarps * 64 <= static_cast<unsigned>(p.k)) share *= 2;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = g_pdl_enabled ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = share;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles, share);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  return cudaLaunchKernelEx(&cfg, lora_low_kernel<NT, kWarps, true>, p);
+}
+
+// the order of the tokens, then the rows of xs and the lists
+cudaError_t launch_lora_rows(const LoraParams& p, int num_sms, cudaStream_t st) {
+  launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, kLoraSortThreads, 0, st, p);
+  cudaError_t e;
+  if (p.rank <= 16) e = launch_rows<2, 8>(p, num_sms, st);
+  else if (p.rank <= 32) e = launch_rows<4, 8>(p, num_sms, st);
+  else if (p.rank <= 64) e = launch_rows<8, 8>(p, num_sms, st);
+  else e = launch_rows<16, 4>(p, num_sms, st);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 cudaError_t launch_lora(const LoraParams& p, int num_sms, cudaStream_t st) {
-  if (cudaError_t e = launch_lora_low(p, num_sms, st)) return e;
+  const int deal = lora_deal(p, num_sms);
+  if (p.order) launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, kLoraSortThreads, 0, st, p);
+  if (p.rank <= 16) launch_low<2>(p, deal, st);
+  else if (p.rank <= 32) launch_low<4>(p, deal, st);
+  else if (p.rank <= 64) launch_low<8>(p, deal, st);
+  else launch_low<16>(p, deal, st);
   const int tiles = (p.tokens + kLoraTile - 1) / kLoraTile;
   const unsigned cols = (p.n + kLoraOutCols - 1) / kLoraOutCols;
   if (tiles >= num_sms) launch_kernel(lora_out_kernel<2>, dim3((cols + 1) / 2, tiles), kLoraOutWarps * 32, 0, st, p);
-  else launch_kernel(lora_out_kernel<1>, dim3(cols, tiles, lora_deal(p, num_sms)), kLoraOutWarps * 32, 0, st, p);
+  else launch_kernel(lora_out_kernel<1>, dim3(cols, tiles, deal), kLoraOutWarps * 32, 0, st, p);
   return cudaGetLastError();
 }
 

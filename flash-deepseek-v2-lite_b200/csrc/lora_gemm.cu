@@ -10,27 +10,29 @@
 // the ones before it are multiplied.
 //
 // A pair of SMs has a tile of 256 tokens x n_tile columns (tcgen05.mma on cta_group::2): each holds the
-// operands and accumulators of 128 of the tokens and the operand of half of the columns.  The operands'
-// way from L2 is what bounds this product; a pair brings in 128 + n_tile / 2 rows per SM and step
-// where single SMs with 128 x n_tile tiles bring in 128 + n_tile.  Both operands K-major with the
-// 128-byte swizzle, accumulators fp32 in TMEM, two of them.  Persistent, one CTA per SM, 14 warps:
+// operands and accumulators of 128 of the tokens and the operand of half of the columns, so that an SM
+// brings in 128 + n_tile / 2 rows per step where a single SM with a 128 x n_tile tile brings in 128 +
+// n_tile (all of the call 73 us, single SMs 75 us).  The issuing lanes are chosen by elect.sync: chosen
+// by their number, each tcgen05.mma took some 200 clocks to issue and the GEMM 65 us instead of 46.
+// Both operands K-major with the 128-byte swizzle, accumulators fp32 in TMEM, two of them.
+// Persistent, one CTA per SM, 14 warps:
 //  - warp 0 (one lane): TMA of this CTA's projection operands into a ring of 6 stages;
 //  - warp 1 (one lane, of the pair's first CTA): tcgen05.mma for both;
 //  - warps 2-5: accumulators to bf16 rows of y, while the next tile is multiplied;
 //  - warps 6-13, in two groups that take the adapters' steps in turn: their operands, from global
-//    memory through registers into ring stages; the loads are on their way before the stage is free.  A plain copy will not do: what an adapter's
+//    memory through registers into ring stages; the loads are on their way before the stage is free.
+//    (One group: 1024 tokens with 64 adapters 45 us, two: 41.)  A plain copy will not do: what an adapter's
 //    padding past its rank holds must not be multiplied, nor may an infinity or a NaN of one adapter
 //    meet the zeros that other adapters' tokens have in its columns.  Such values enter as zeros, and
 //    the epilogue adds their products to the rows of their own adapter.
 // low enters as bf16: its rounding (2^-9 of the adapters' part) is below that of y.
-// 4001 tokens, 6 adapters of rank 32, 2048 -> 3648: 46 of the 81 us that the order (9 us), low (15), the
-// gather (10) and this take together, 1.3 PFLOP/s; with one SM per tile of 128 x 224 it took 65 us.
+// 4001 tokens, 6 adapters of rank 32, 2048 -> 3648: 46 of the 73 us that the order (9 us), the rows
+// (16) and this take together; 1.3 PFLOP/s.  Bound by the multiplications with what the last tiles
+// leave idle: 16 x 17 tiles are 3.7 rounds of 74 pairs.
 #include "params.cuh"
 
 namespace dsv2 {
 
-constexpr int kLgRows = 128;          // tokens of a CTA's half of a tile
-constexpr int kLgM = 2 * kLgRows;     // tokens of a tile
 constexpr int kLgK = 64;              // k of a ring stage
 constexpr int kLgStages = 6;
 constexpr int kLgABytes = kLgRows * kLgK * 2;
@@ -41,65 +43,6 @@ constexpr int kLgGroups = 2;
 constexpr int kLgThreads = 6 * 32 + kLgGroups * kLgLoaders;
 constexpr size_t kLgSmem = kLgStages * kLgStageBytes + 1024 + 256;
 static_assert(kLgSmem <= 232448, "adapter GEMM: shared memory exceeds 227 KB");
-
-constexpr int kLgPiece = 16;          // ranks of a piece, the k of one tcgen05.mma
-
-// ints of a tile's list: the number of pieces, one unused, then (adapter, first rank | ranks << 16) each
-__host__ __device__ constexpr long long lg_list_ints(int rank) {
-  return 2 + 2LL * kLgM * ((rank + kLgPiece - 1) / kLgPiece);
-}
-
-// elements of a row of xs: whole 128-byte lines, which is what the GEMM's copies take
-__host__ __device__ constexpr long long lg_row(int k, int rank) { return k + (rank + 63LL) / 64 * 64; }
-
-// xs[i] = x[order[i]], then that token's low as bf16 (0 past its adapter's rank; rows of tokens without
-// an adapter hold nothing), one warp per row; every 32nd CTA also lists the pieces of its 256-token tile.
-__global__ __launch_bounds__(256) void lora_gather_kernel(const LoraParams p) {
-  pdl_enter();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 8 + warp;
-  if (i < p.tokens) {
-    const uint4* src = reinterpret_cast<const uint4*>(p.x + p.order[i] * p.x_row_stride);
-    uint4* dst = reinterpret_cast<uint4*>(p.xs + i * lg_row(p.k, p.rank));
-    if (lane < p.rank / 4 && p.order[p.tokens + i] >= 0) {
-      const float* low = p.low + static_cast<long long>(p.order[i]) * p.rank + 4 * lane;
-      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < p.low_parts; ++q, low += static_cast<long long>(p.tokens) * p.rank) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(low));
-        f = make_float4(f.x + v.x, f.y + v.y, f.z + v.z, f.w + v.w);
-      }
-      reinterpret_cast<uint2*>(dst + p.k / 8)[lane] = make_uint2(pack_bf16x2(f.x, f.y), pack_bf16x2(f.z, f.w));
-    }
-#pragma unroll 8
-    for (int j = lane; j < p.k / 8; j += 32) dst[j] = __ldg(src + j);
-  }
-  if (blockIdx.x % (kLgM / 8) == 0 && warp == 0) {
-    const int tile = blockIdx.x / (kLgM / 8);
-    int* list = p.lists + tile * lg_list_ints(p.rank);
-    int n = 0;
-    for (int q = 0; q < kLgM; q += 32) {
-      const int pos = tile * kLgM + q + lane;
-      const int a = pos < p.tokens ? p.order[p.tokens + pos] : -1;
-      // tokens are in adapter order: the first of each adapter lists its pieces
-      const bool first = a >= 0 && (q + lane == 0 || p.order[p.tokens + pos - 1] != a);
-      const int rank = first ? p.order[2 * p.tokens + pos] : 0, mine = (rank + kLgPiece - 1) / kLgPiece;
-      int at = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int u = __shfl_up_sync(0xffffffffu, at, d);
-        if (lane >= d) at += u;
-      }
-      const int sum = __shfl_sync(0xffffffffu, at, 31);
-      at += n - mine;
-      for (int c = 0; c < mine; ++c) {
-        list[2 + 2 * (at + c)] = a;
-        list[2 + 2 * (at + c) + 1] = c * kLgPiece | min(rank - c * kLgPiece, kLgPiece) << 16;
-      }
-      n += sum;
-    }
-    if (lane == 0) list[0] = n;
-  }
-}
 
 // The steps of an item: nkb of the projection and extra = ceil(pieces / 4) of the adapters, of which
 // number e comes after (e + 1) nkb / (extra + 1) of the projection's.
@@ -178,8 +121,6 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* odd_flag = abort_flag + 1;        // an adapter's B held an infinity or a NaN
-  // (uniform roles and elect.sync for the issuing lane: with a lane number the operands of an issue are
-  // not known to be uniform)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t half = cluster_ctarank();        // of the pair
   const int pair = cluster_id_x(), pairs = n_clusters_x();
@@ -341,15 +282,13 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
       if (*odd_flag && live && p.order[p.tokens + pos] >= 0) {
         // the products that were left out, into this thread's own elements of y (rare: any speed will do)
         const int a = p.order[p.tokens + pos], rank = p.order[2 * p.tokens + pos];
-        const float* low = p.low + static_cast<long long>(p.order[pos]) * p.rank;
+        const bf16* low = p.xs + pos * lg_row(p.k, p.rank) + p.k;
         const bf16* b = p.b + (static_cast<long long>(a) * p.n + nt * n_tile) * p.rank;
         for (int c = 0; c < cols; ++c, b += p.rank)
           for (int j = 0; j < rank; ++j) {
             const float w = __bfloat162float(b[j]);
             if (isfinite(w)) continue;
-            float u = 0.f;
-            for (int q = 0; q < p.low_parts; ++q) u += low[static_cast<long long>(q) * p.tokens * p.rank + j];
-            y[c] = __float2bfloat16(__bfloat162float(y[c]) + u * w);
+            y[c] = __float2bfloat16(__bfloat162float(y[c]) + __bfloat162float(low[j]) * w);
           }
       }
     }
@@ -458,11 +397,6 @@ int lora_gemm_tile(int tokens, int n, int num_sms) {
     }
   }
   return tile;
-}
-
-cudaError_t launch_lora_gather(const LoraParams& p, cudaStream_t st) {
-  launch_kernel(lora_gather_kernel, (p.tokens + 7) / 8, 256, 0, st, p);
-  return cudaGetLastError();
 }
 
 cudaError_t launch_lora_gemm(const LoraParams& p, const CUtensorMap& tm_x, const CUtensorMap& tm_w, int n_tile, int num_sms,

@@ -252,10 +252,9 @@ cudaError_t launch_page_plan(const PagePlanParams&, int num_sms, cudaStream_t);
 cudaError_t mla_q4_init();
 cudaError_t launch_mla_q4(const MlaQ4Params&, int num_sms, cudaStream_t);
 cudaError_t launch_lora(const LoraParams&, int num_sms, cudaStream_t);
-cudaError_t launch_lora_low(const LoraParams&, int num_sms, cudaStream_t);
+cudaError_t launch_lora_rows(const LoraParams&, int num_sms, cudaStream_t);
 cudaError_t lora_gemm_init();
 int lora_gemm_tile(int tokens, int n, int num_sms);
-cudaError_t launch_lora_gather(const LoraParams&, cudaStream_t);
 cudaError_t launch_lora_gemm(const LoraParams&, const CUtensorMap& tm_x, const CUtensorMap& tm_w, int n_tile, int num_sms,
                              cudaStream_t);
 cudaError_t mla_decode_init();

@@ -748,7 +748,7 @@ def lora_workspace(tokens: int, n: int, k: int, rank: int, device) -> dict:
     """Work buffers of lora_linear: the low-rank rows, the tokens' order by adapter, the shared
     projection's fp32 partials and, above 256 tokens, the activations in that order with the
     adapters of each tile of tokens (xs, lists: the projection and the adapters are then one
-    GEMM if there are at least 16 tokens per adapter)."""
+    GEMM if there are at least 12 tokens per adapter)."""
     sms = torch.cuda.get_device_properties(device).multi_processor_count
     splits = 1
     if LORA_GEMV_TOKENS < tokens <= LORA_GEMM_TOKENS:   # decode batches: K split over the SMs, as the engine's projections

@@ -678,7 +678,7 @@ DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* strea
  * order: int32 work buffer [3 * tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128.
  * xs, lists: work buffers, may be NULL: bf16 [tokens, k + rank rounded up to 64] and int32
  * [ceil(tokens / 256), 2 + 512 * ceil(rank / 16)].  With them and w, a long run of tokens (more than 256
- * and at least 16 per adapter, bf16 y, k % 64 == 0) is one GEMM over the tokens in adapter order. */
+ * and at least 12 per adapter, bf16 y, k % 64 == 0) is one GEMM over the tokens in adapter order. */
 typedef struct dsv2_lora_args {
   const void* x;
   int64_t x_row_stride;
