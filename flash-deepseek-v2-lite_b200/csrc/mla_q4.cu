@@ -12,7 +12,10 @@ constexpr int kQ4Pos = 128;                                  // positions of a t
 constexpr int kQ4TileBlocks = kQ4Pos / kL4Tokens;
 constexpr int kQ4Stages = 3;
 constexpr int kQ4StageBytes = kQ4TileBlocks * kL4BlockBytes; // 51200
-constexpr int kQ4SegUnits = 4;                               // per-row cost in blocks (work balance)
+// per-row cost in blocks, for the work balance: 4 / 8 / 16 / 32 give 17.3 / 16.1 / 16.0 / 16.9 us for 32
+// rows of 512, 41.9 / 40.9 / 42.1 / 45.1 for 256 ragged ones, 41.3 / 36.9 / 36.4 / 37.8 for 9 x 3 long ones,
+// 57.8 / 55.7 / 58.1 / 62.7 for 100 x 2 of 50 .. 2500
+constexpr int kQ4SegUnits = 8;
 constexpr int kQ4ScoreWarps = 8;                             // a block of a tile each
 constexpr int kQ4PvWarps = 8;                                // 64 latent dims each
 constexpr int kQ4Compute = (kQ4ScoreWarps + kQ4PvWarps) * 32;
