@@ -4,7 +4,8 @@
 
 namespace {
 
-// up to here a shared projection with one partial runs the small (GEMV) family
+// up to here a shared projection with one partial runs the small (GEMV) family (n 3648, k 2048, with
+// adapters: 1 / 8 tokens 9.1 / 10.2 us; the batch family in 4 pieces of k 13.5 / 14.6)
 constexpr int kLoraGemvTokens = 8;
 // The projection and its adapters are one GEMM above 256 tokens with 12 or more per adapter: it pays a
 // pass that orders the tokens and a step per 64 ranks of every adapter in a tile, and saves the fp32

@@ -214,6 +214,12 @@ static_assert(sizeof(Q4Smem) <= 232448, "4-bit latent attention: shared memory e
 //  - warp 16: copies blocks (looked up 32 at a time) and query rows, and notes each row's partials.
 // The maximum that P is taken against is kept until a score exceeds it by 2^kQ4Slack: the score
 // warps then agree on a new one and the P V warps rescale.
+//
+// With the merge launch: 64 rows of 8192 tokens 89 us (212 MB, 2.4 TB/s), 64 x 2048 36 us, 256 ragged rows
+// of 1 .. 1900 58 us, one row of 512 12 us.  The copies alone take 49 us of the 89, scores without P V 66,
+// P V without scores 56: about 33 us of products and as much of conversions on each side (34.8 kFLOP and
+// 1024 nibble conversions a token, for 400 bytes) overlap with each other and with the copies only in
+// part.  Tiles of 64 positions (7 stages) and conversions taken out on one side changed nothing.
 __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Q4Smem& sm = *reinterpret_cast<Q4Smem*>(smem_raw);

@@ -12,6 +12,9 @@
 // short computation per token and per moved page.  Every CTA runs the prefix sums over all
 // requests, 1024 at a time, and takes every gridDim-th group of 1024 tokens and pages, which it
 // finds by bisection in the prefix sums of the chunk: no second launch and no wait between CTAs.
+//
+// Bound by latency, a chain of dependent loads and barriers per chunk: 256 decoding requests 7.3 us;
+// 1500 requests with 16381 tokens of prompts, two chunks, 23 us (0.5 MB).
 #include "params.cuh"
 
 namespace dsv2 {
