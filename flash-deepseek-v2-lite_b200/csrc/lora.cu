@@ -68,11 +68,19 @@ __global__ __launch_bounds__(kLoraSortThreads) void lora_sort_kernel(const LoraP
     const int n = min(kLoraSortChunk, p.tokens - u0);
     const int4* q = reinterpret_cast<const int4*>(s_id);
     const int rel = t - u0;
+    // w < mine, or equal and earlier: an equal one counts when its index is below this token's.  The
+    // CTA's tokens are 32 in a row, so only the quads among them need a look at each index
+    const int r0 = rel - lane;
+#pragma unroll 4
     for (int i = warp; i < (n + 3) / 4; i += kLoraSortThreads / 32) {
       const int4 w = q[i];
-      // w < mine, or equal and earlier: equal counts when the index is below this token's
-      before += (w.x < mine + (4 * i < rel)) + (w.y < mine + (4 * i + 1 < rel)) + (w.z < mine + (4 * i + 2 < rel)) +
-                (w.w < mine + (4 * i + 3 < rel));
+      if (4 * i >= r0 && 4 * i < r0 + 32) {
+        before += (w.x < mine + (4 * i < rel)) + (w.y < mine + (4 * i + 1 < rel)) + (w.z < mine + (4 * i + 2 < rel)) +
+                  (w.w < mine + (4 * i + 3 < rel));
+      } else {
+        const int m = mine + (4 * i < r0);
+        before += (w.x < m) + (w.y < m) + (w.z < m) + (w.w < m);
+      }
     }
   }
   s_before[threadIdx.x] = before;
@@ -137,13 +145,19 @@ __host__ __device__ constexpr long long lg_row(int k, int rank) { return k + (ra
 __device__ __forceinline__ void lora_list_pieces(const LoraParams& p, int tile) {
   const int lane = threadIdx.x & 31;
   int* list = p.lists + tile * lg_list_ints(p.rank);
+  int ad[kLgM / 32], before[kLgM / 32], ranks[kLgM / 32];   // all loads under way together
+#pragma unroll
+  for (int q = 0; q < kLgM / 32; ++q) {
+    const int pos = tile * kLgM + q * 32 + lane;
+    ad[q] = pos < p.tokens ? p.order[p.tokens + pos] : -1;
+    before[q] = pos < p.tokens && q * 32 + lane > 0 ? p.order[p.tokens + pos - 1] : -1;
+    ranks[q] = pos < p.tokens ? p.order[2 * p.tokens + pos] : 0;
+  }
   int n = 0;
-  for (int q = 0; q < kLgM; q += 32) {
-    const int pos = tile * kLgM + q + lane;
-    const int a = pos < p.tokens ? p.order[p.tokens + pos] : -1;
+#pragma unroll
+  for (int q = 0; q < kLgM / 32; ++q) {
     // tokens are in adapter order: the first of each adapter lists its pieces
-    const bool first = a >= 0 && (q + lane == 0 || p.order[p.tokens + pos - 1] != a);
-    const int rank = first ? p.order[2 * p.tokens + pos] : 0, mine = (rank + kLgPiece - 1) / kLgPiece;
+    const int a = ad[q], rank = a >= 0 && a != before[q] ? ranks[q] : 0, mine = (rank + kLgPiece - 1) / kLgPiece;
     int at = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
