@@ -10,8 +10,8 @@ constexpr int kLoraGemvTokens = 8;
 // The projection and its adapters are one GEMM above 256 tokens with 12 or more per adapter: it pays a
 // pass that orders the tokens and a step per 64 ranks of every adapter in a tile, and saves the fp32
 // partials.  n 3648, k 2048, rank 32, one GEMM / separate launches: 257 tokens 22 / 28 us with 1 adapter,
-// 27 / 29 with 16, 33 / 31 with 32; 1024 tokens 32 / 39 with 1, 38 / 40 with 64; 4001 with 6 74 / 134.
-// Up to 256 tokens the projection reads its weights once either way.
+// 27.5 / 29 with 16, 37 / 31 with 32, 56 / 34 with 64; 768 tokens 37 / 48 with 64; 1024 tokens 29 / 39 with
+// 1, 35 / 40 with 64; 4001 with 6 71 / 133.  Up to 256 tokens the projection reads its weights once either way.
 constexpr int kLoraGemmTokens = 256, kLoraGemmPerAdapter = 12;
 // fewest units of a CTA (64 positions): one row of 512 with 1 / 4 / 16: 13.9 / 13.6 / 14.8 us, of 64:
 // 11.7 / 10.3 / 10.3

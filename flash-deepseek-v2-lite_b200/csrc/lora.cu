@@ -434,7 +434,7 @@ __global__ __launch_bounds__(kLoraOutWarps * 32, 3) void lora_out_kernel(const L
 // Launch shapes.  A tile of few tokens can hold many adapters: with few tiles they are dealt out to
 // 4 CTAs (dealt / not: 64 tokens with 60 adapters 26 / 46 us, 200 with 40 30 / 33, 500 with 60 39 / 35).
 // With many tiles a CTA of the second product takes 512 columns, which share its set-up (4001 tokens
-// 135 us, with 256 columns 141).
+// 133 us, with 256 columns 140).
 static int lora_deal(const LoraParams& p, int num_sms) {
   return p.tokens > 1 && (p.tokens + kLoraTile - 1) / kLoraTile < num_sms / 8 ? 4 : 1;
 }

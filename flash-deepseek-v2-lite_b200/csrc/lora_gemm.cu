@@ -26,9 +26,9 @@
 //    meet the zeros that other adapters' tokens have in its columns.  Such values enter as zeros, and
 //    the epilogue adds their products to the rows of their own adapter.
 // low enters as bf16: its rounding (2^-9 of the adapters' part) is below that of y.
-// 4001 tokens, 6 adapters of rank 32, 2048 -> 3648: 46 of the 73 us that the order (9 us), the rows
-// (16) and this take together; 1.3 PFLOP/s.  Bound by the multiplications with what the last tiles
-// leave idle: 16 x 17 tiles are 3.7 rounds of 74 pairs.
+// 4001 tokens, 6 adapters of rank 32, 2048 -> 3648: about 46 of the 71 us that the order, the rows and
+// this take together; 1.3 PFLOP/s.  Bound by the multiplications with what the last tiles leave idle:
+// 16 x 17 tiles are 3.7 rounds of 74 pairs.
 #include "params.cuh"
 
 namespace dsv2 {

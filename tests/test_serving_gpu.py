@@ -521,6 +521,59 @@ def test_lora_infinities_stay_with_their_adapter(D, T, rank, N):
     assert bool(got[own][:, N - 1].isnan().all())
 
 
+@pytest.mark.parametrize("T,rank", [(300, 16), (777, 40)])
+def test_lora_long_runs_strided_by_request_in_a_graph(D, T, rank):
+    K, N = 192, 328
+    c = lora_case(T, 5, rank, K, N, seed=T)
+    g = torch.Generator().manual_seed(T)
+    req = torch.randperm(T, generator=g)
+    token_row = req.to(torch.int32)
+    token_row[T - 20:] = -1                               # padding rows: the projection alone
+    by_req = torch.empty_like(c["ids"])
+    by_req[req] = c["ids"]
+    c["ids"] = torch.where(token_row < 0, torch.tensor(-1, dtype=torch.int32), c["ids"])
+    x = torch.full((T, K + 40), math.nan, dtype=torch.bfloat16, device=DEV)
+    x[:, 8:8 + K] = c["x"].to(DEV)
+    w = torch.full((N, K + 16), math.nan, dtype=torch.bfloat16, device=DEV)
+    w[:, :K] = c["w"].to(DEV)
+    y = torch.full((T, N + 24), 5.0, dtype=torch.bfloat16, device=DEV)
+    d = {k: c[k].to(DEV) for k in ("a", "b", "ranks", "scales")}
+    ids, token_row = by_req.to(DEV), token_row.to(DEV)
+    ws = D.lora_workspace(T, N, K, rank, DEV)
+    ws["xs"].fill_(math.nan)                              # work buffers may hold anything
+    ws["lists"].fill_(-7)
+
+    def run():
+        D.lora_linear(x=x[:, 8:8 + K], w=w[:, :K], ids=ids, token_row=token_row, y=y[:, :N], **d, **ws)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    s.synchronize()
+    check_lora(y[:, :N], c)
+    first = y.clone()
+    assert bool((y[:, N:] == 5).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    y[:, :N] = 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, first)
+
+
+def test_lora_refuses_short_gemm_buffers(D):
+    c = lora_case(300, 2, 16, 64, 64, seed=3)
+    d = {k: v.to(DEV) for k, v in c.items()}
+    y = torch.empty(300, 64, dtype=torch.bfloat16, device=DEV)
+    ws = D.lora_workspace(300, 64, 64, 16, DEV)
+    for name in ("xs", "lists"):
+        with pytest.raises(ValueError):
+            D.lora_linear(**d, y=y, **dict(ws, **{name: ws[name].view(-1)[:-1]}))
+    with pytest.raises(ValueError):                       # not on a 16-byte boundary
+        D.lora_linear(**d, y=y, **dict(ws, xs=torch.empty(ws["xs"].numel() + 1, dtype=torch.bfloat16, device=DEV)[1:]))
+
+
 def test_lora_flags_ids_out_of_range(D):
     c = lora_case(20, 2, 8, 64, 16, seed=2, none=0)
     good = c["ids"].clone()
