@@ -4,8 +4,8 @@
 
 namespace {
 
-// up to here a shared projection with one partial runs the small (GEMV) family (n 3648, k 2048, with
-// adapters: 1 / 8 tokens 9.1 / 10.2 us; the batch family in 4 pieces of k 13.5 / 14.6)
+// up to here a shared projection with one partial shares a launch with the second product (n 3648, k 2048:
+// 1 / 8 tokens 7.3 / 9.3 us; the batch projection in 4 pieces of k with the two products 13.5 / 14.6)
 constexpr int kLoraGemvTokens = 8;
 // The projection and its adapters are one GEMM above 256 tokens with 12 or more per adapter: it pays a
 // pass that orders the tokens and a step per 64 ranks of every adapter in a tile, and saves the fp32
@@ -179,7 +179,10 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
     return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
   int sms = 0;
   if (int rc = ensure_init(&sms)) return rc;
-  if (a->w && !fused) {
+  const bool few = a->w && a->tokens <= kLoraGemvTokens && a->n_base == 1;
+  if ((few || fused) && (!aligned16(a->w) || a->w_row_stride % 8 || a->w_row_stride < a->k))
+    return fail(DSV2_ERR_INVALID, "lora: w must be 16-byte aligned rows");
+  if (a->w && !fused && !few) {
     dsv2_linear_args l = {};
     l.w = a->w;
     l.w_row_stride = a->w_row_stride;
@@ -196,8 +199,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
     l.x_group_rows = a->tokens;
     l.k_splits = a->n_base;
     l.y_split_stride = a->base_part_stride;
-    const bool small = a->tokens <= kLoraGemvTokens && a->n_base == 1;
-    if (int rc = dsv2_linear(&l, small ? DSV2_FAMILY_SMALL : DSV2_FAMILY_BATCH, stream)) return rc;
+    if (int rc = dsv2_linear(&l, DSV2_FAMILY_BATCH, stream)) return rc;
   }
   LoraParams p = {};
   p.x = static_cast<const bf16*>(a->x);
@@ -225,9 +227,13 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   p.y_f32 = a->y_dtype == DSV2_F32;
   p.y_row_stride = a->y_row_stride;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (few) {
+    p.w = static_cast<const bf16*>(a->w);
+    p.w_row_stride = a->w_row_stride;
+    p.base_parts = 0;
+  }
   if (!fused) return check_launch(launch_lora(p, sms, st), "lora");
-  if (!aligned16(a->w) || !aligned16(a->xs) || !aligned16(a->lists) || a->w_row_stride % 8 || a->w_row_stride < a->k)
-    return fail(DSV2_ERR_INVALID, "lora: w, xs and lists must be 16-byte aligned");
+  if (!aligned16(a->xs) || !aligned16(a->lists)) return fail(DSV2_ERR_INVALID, "lora: xs and lists must be 16-byte aligned");
   p.xs = static_cast<bf16*>(a->xs);
   p.lists = a->lists;
   p.base_parts = 0;

@@ -11,7 +11,7 @@
 // 16 bytes a lane: which k the lanes of a quad hold is free as long as both operands agree, so
 // lane tq of a quad takes 8 consecutive k of every 32.
 //
-// With the shared projection (2048 -> 3648): 1 token 8.8 us, 16.7 MB of weights and three launches; 200
+// With the shared projection (2048 -> 3648): 1 token 7.3 us, 15 MB and two launches (lora_few_kernel); 200
 // tokens of 40 adapters of rank 64 29.6 us, 43 MB, of which the projection takes about 9 and the rest is
 // latency of the order, first and second product.  Long runs of tokens: lora_gemm.cu.
 #include "params.cuh"
@@ -431,6 +431,101 @@ __global__ __launch_bounds__(kLoraOutWarps * 32, 3) void lora_out_kernel(const L
   }
 }
 
+// Up to 8 tokens: the shared projection and the second product in one launch, 16 columns of y a CTA.
+// Eight warps take a part of k each, W as the mma's 16 rows and the tokens as its 8 columns; the first
+// 256 of each part of W are requested before the wait for the first product's launch.  Then a thread adds
+// half of the ranks for one of the 16 x 8 results.  Bound by reading W (15 MB) and the chain of two launches:
+// 1
+// token of rank 16, 2048 -> 3648: 7.3 us (2.1 TB/s), 8 of rank 32: 9.3; as projection, first and second
+// product 9.2 and 12.8.
+constexpr int kLoraFewTokens = 8, kLoraFewCols = 16, kLoraFewWarps = 8, kLoraFewAhead = 8;
+__global__ __launch_bounds__(kLoraFewWarps * 32, 2) void lora_few_kernel(const LoraParams p) {
+  __shared__ float s_red[kLoraFewWarps][kLoraFewTokens][kLoraFewCols + 1];
+  __shared__ float s_low[kLoraFewTokens][128];
+  __shared__ float s_half[kLoraFewTokens][kLoraFewCols];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  const int n0 = blockIdx.x * kLoraFewCols;
+  const int steps = (p.k + 31) / 32;
+  const int k0 = steps * warp / kLoraFewWarps * 32, k1 = steps * (warp + 1) / kLoraFewWarps * 32;
+  const bool in0 = n0 + gq < p.n, in1 = n0 + gq + 8 < p.n;
+  const bf16* w0 = p.w + (in0 ? n0 + gq : 0) * p.w_row_stride;
+  const bf16* w1 = p.w + (in1 ? n0 + gq + 8 : 0) * p.w_row_stride;
+  uint4 a0[kLoraFewAhead], a1[kLoraFewAhead];
+  auto load_w = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < kLoraFewAhead; ++i) {
+      const int kk = k + 32 * i + 8 * tq;
+      const bool in = kk < k1 && kk < p.k;
+      a0[i] = ld_or_zero(w0 + kk, in && in0);
+      a1[i] = ld_or_zero(w1 + kk, in && in1);
+    }
+  };
+  load_w(k0);
+  pdl_enter();
+  // low of the tokens, its pieces summed in order
+  for (int i = threadIdx.x; i < p.tokens * p.rank; i += kLoraFewWarps * 32) {
+    const int t = i / p.rank;
+    const int id = lora_id(p, t);
+    float v = 0.f;
+    if (id >= 0) {
+#pragma unroll 8
+      for (int q = 0; q < p.low_parts; ++q) v += __ldcg(p.low + static_cast<long long>(q) * p.tokens * p.rank + i);
+    }
+    s_low[t][i % p.rank] = v;
+  }
+  const bf16* x = p.x + (gq < p.tokens ? gq : 0) * p.x_row_stride;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = k0; k < k1; k += 32 * kLoraFewAhead) {
+    if (k > k0) load_w(k);
+    uint4 u[kLoraFewAhead];
+#pragma unroll
+    for (int i = 0; i < kLoraFewAhead; ++i) {
+      const int kk = k + 32 * i + 8 * tq;
+      u[i] = ld_or_zero(x + kk, kk < k1 && kk < p.k && gq < p.tokens);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoraFewAhead; ++i) {
+      const uint32_t f0[4] = {a0[i].x, a1[i].x, a0[i].y, a1[i].y}, f1[4] = {a0[i].z, a1[i].z, a0[i].w, a1[i].w};
+      mma_bf16_16816(acc, f0, u[i].x, u[i].y);
+      mma_bf16_16816(acc, f1, u[i].z, u[i].w);
+    }
+  }
+  s_red[warp][2 * tq][gq] = acc[0];
+  s_red[warp][2 * tq + 1][gq] = acc[1];
+  s_red[warp][2 * tq][gq + 8] = acc[2];
+  s_red[warp][2 * tq + 1][gq + 8] = acc[3];
+  // this thread's result and half of the ranks
+  const int col = threadIdx.x % kLoraFewCols, t = threadIdx.x / kLoraFewCols % kLoraFewTokens;
+  const bool upper = threadIdx.x >= kLoraFewCols * kLoraFewTokens;
+  const bool mine = t < p.tokens && n0 + col < p.n;
+  const int id = mine ? lora_id(p, t) : -1;
+  const int rank = id >= 0 ? min(max(p.ranks[id], 0), p.rank) : 0;
+  __syncthreads();
+  float v = 0.f;
+  const int mid = p.rank / 16 * 8, j0 = upper ? mid : 0, j1 = min(upper ? p.rank : mid, rank);
+  const bf16* b = p.b + (static_cast<long long>(max(id, 0)) * p.n + (mine ? n0 + col : 0)) * p.rank;
+#pragma unroll 4
+  for (int j = j0; j < j1; j += 8) {
+    const uint4 c = __ldg(reinterpret_cast<const uint4*>(b + j));
+    const uint32_t wd[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // what lies past the rank may be anything
+      if (j + 2 * i < j1) v += s_low[t][j + 2 * i] * bf16lo(wd[i]);
+      if (j + 2 * i + 1 < j1) v += s_low[t][j + 2 * i + 1] * bf16hi(wd[i]);
+    }
+  }
+  if (upper) s_half[t][col] = v;
+  __syncthreads();
+  if (upper || !mine) return;
+  float base = 0.f;
+#pragma unroll
+  for (int q = 0; q < kLoraFewWarps; ++q) base += s_red[q][t][col];
+  v = base + (v + s_half[t][col]);
+  const long long at = t * p.y_row_stride + n0 + col;
+  if (p.y_f32) reinterpret_cast<float*>(p.y)[at] = v;
+  else reinterpret_cast<bf16*>(p.y)[at] = __float2bfloat16(v);
+}
+
 // Launch shapes.  A tile of few tokens can hold many adapters: with few tiles they are dealt out to
 // 4 CTAs (dealt / not: 64 tokens with 60 adapters 26 / 46 us, 200 with 40 30 / 33, 500 with 60 39 / 35).
 // With many tiles a CTA of the second product takes 512 columns, which share its set-up (4001 tokens
@@ -481,11 +576,15 @@ cudaError_t launch_lora_rows(const LoraParams& p, int num_sms, cudaStream_t st) 
 
 cudaError_t launch_lora(const LoraParams& p, int num_sms, cudaStream_t st) {
   const int deal = lora_deal(p, num_sms);
-  if (p.order) launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, kLoraSortThreads, 0, st, p);
+  if (p.order && !p.w) launch_kernel(lora_sort_kernel, (p.tokens + 31) / 32, kLoraSortThreads, 0, st, p);
   if (p.rank <= 16) launch_low<2>(p, deal, st);
   else if (p.rank <= 32) launch_low<4>(p, deal, st);
   else if (p.rank <= 64) launch_low<8>(p, deal, st);
   else launch_low<16>(p, deal, st);
+  if (p.w) {   // few tokens
+    launch_kernel(lora_few_kernel, (p.n + kLoraFewCols - 1) / kLoraFewCols, kLoraFewWarps * 32, 0, st, p);
+    return cudaGetLastError();
+  }
   const int tiles = (p.tokens + kLoraTile - 1) / kLoraTile;
   const unsigned cols = (p.n + kLoraOutCols - 1) / kLoraOutCols;
   if (tiles >= num_sms) launch_kernel(lora_out_kernel<2>, dim3((cols + 1) / 2, tiles), kLoraOutWarps * 32, 0, st, p);

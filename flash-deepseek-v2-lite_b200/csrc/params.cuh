@@ -181,6 +181,8 @@ struct LoraParams {
   void* y;                     // [tokens, n] bf16 or fp32
   int y_f32;
   long long y_row_stride;
+  const bf16* w;               // few tokens: the shared projection's weights, [n, k] (else null)
+  long long w_row_stride;
   bf16* xs;                    // long runs of tokens: [tokens, k + rank rounded up to 64] work buffer, x and low in adapter order
   int* lists;                  // [ceil(tokens / 256), 2 + 512 ceil(rank / 16)] work buffer, adapters of each token tile
 };

@@ -768,12 +768,12 @@ def lora_workspace(tokens: int, n: int, k: int, rank: int, device) -> dict:
 def lora_splits(tokens: int, k: int, num_sms: int) -> int:
     """Pieces of k that the adapters' first product runs side by side: about six CTAs (of a tile
     of 16 tokens) per SM, each with at least 256 of k, at most 16 pieces for the second product
-    to sum.  (k 2048, pieces 1 / 4 / 8 / 16: 1 token 12.5 / 9.2 / 8.8 / 9.3 us, 200 tokens of 40 adapters
-    35 / 29 / 29 / 33.)"""
+    to sum.  (k 2048, pieces 1 / 4 / 8 / 16: 64 tokens of 16 adapters 21 / 18 / 18 / 19 us, 200 tokens of
+    40 35 / 29 / 29 / 33.)"""
     return max(1, min(6 * num_sms // max(1, (tokens + 15) // 16), k // 256, 16))
 
 
-LORA_GEMV_TOKENS = 8     # up to here lora_linear's shared projection runs the small (GEMV) family
+LORA_GEMV_TOKENS = 8     # up to here lora_linear's shared projection and the adapters' second product are one launch
 LORA_GEMM_TOKENS = 256   # above, the projection and its adapters can be one GEMM
 
 
