@@ -4,9 +4,10 @@
 
 namespace {
 
-// up to here a shared projection with one partial shares a launch with the second product (n 3648, k 2048:
-// 1 / 8 tokens 7.3 / 9.3 us; the batch projection in 4 pieces of k with the two products 13.5 / 14.6)
-constexpr int kLoraGemvTokens = 8;
+// up to here a shared projection with one partial shares a launch with the second product (n 3648, k 2048,
+// shared / separate: 1 token 7.3 / 9.2 us, 9 of rank 16 8.1 / 15.4, 16 of rank 32 11.5 / 17.8, 16 of rank
+// 64 18.8 / 27.8; 32 of rank 32 15.8 / 16.2, of rank 128 36 / 23)
+constexpr int kLoraGemvTokens = 16;
 // The projection and its adapters are one GEMM above 256 tokens with 12 or more per adapter: it pays a
 // pass that orders the tokens and a step per 64 ranks of every adapter in a tile, and saves the fp32
 // partials.  n 3648, k 2048, rank 32, one GEMM / separate launches: 257 tokens 22 / 28 us with 1 adapter,

@@ -431,18 +431,19 @@ __global__ __launch_bounds__(kLoraOutWarps * 32, 3) void lora_out_kernel(const L
   }
 }
 
-// Up to 8 tokens: the shared projection and the second product in one launch, 16 columns of y a CTA.
-// Eight warps take a part of k each, W as the mma's 16 rows and the tokens as its 8 columns; the first
+// Few tokens (kGroups x 8): the shared projection and the second product in one launch, 16 columns of y
+// a CTA.  Eight warps take a part of k each, W as the mma's 16 rows and tokens as its 8 columns; the first
 // 256 of each part of W are requested before the wait for the first product's launch.  Then a thread adds
-// half of the ranks for one of the 16 x 8 results.  Bound by reading W (15 MB) and the chain of two launches:
-// 1
-// token of rank 16, 2048 -> 3648: 7.3 us (2.1 TB/s), 8 of rank 32: 9.3; as projection, first and second
-// product 9.2 and 12.8.
-constexpr int kLoraFewTokens = 8, kLoraFewCols = 16, kLoraFewWarps = 8, kLoraFewAhead = 8;
+// the ranks (with 8 tokens: half of them) of one of the 16 x tokens results.  Bound by reading W (15 MB)
+// and the chain of two launches: 1 token of rank 16, 2048 -> 3648, 7.3 us (2.1 TB/s); 8 of rank 32 9.4; as
+// projection, first and second product 9.2 and 12.8.
+constexpr int kLoraFewCols = 16, kLoraFewWarps = 8, kLoraFewAhead = 8;
+template <int kGroups>
 __global__ __launch_bounds__(kLoraFewWarps * 32, 2) void lora_few_kernel(const LoraParams p) {
-  __shared__ float s_red[kLoraFewWarps][kLoraFewTokens][kLoraFewCols + 1];
-  __shared__ float s_low[kLoraFewTokens][128];
-  __shared__ float s_half[kLoraFewTokens][kLoraFewCols];
+  constexpr int kTok = 8 * kGroups, kHalves = kGroups == 1 ? 2 : 1;
+  __shared__ float s_red[kLoraFewWarps][kTok][kLoraFewCols + 1];
+  __shared__ float s_low[kTok][128];
+  __shared__ float s_half[8][kLoraFewCols];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
   const int n0 = blockIdx.x * kLoraFewCols;
   const int steps = (p.k + 31) / 32;
@@ -465,65 +466,77 @@ __global__ __launch_bounds__(kLoraFewWarps * 32, 2) void lora_few_kernel(const L
   // low of the tokens, its pieces summed in order
   for (int i = threadIdx.x; i < p.tokens * p.rank; i += kLoraFewWarps * 32) {
     const int t = i / p.rank;
-    const int id = lora_id(p, t);
     float v = 0.f;
-    if (id >= 0) {
+    if (lora_id(p, t) >= 0) {
 #pragma unroll 8
       for (int q = 0; q < p.low_parts; ++q) v += __ldcg(p.low + static_cast<long long>(q) * p.tokens * p.rank + i);
     }
     s_low[t][i % p.rank] = v;
   }
-  const bf16* x = p.x + (gq < p.tokens ? gq : 0) * p.x_row_stride;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  float acc[kGroups][4];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.f;
   for (int k = k0; k < k1; k += 32 * kLoraFewAhead) {
     if (k > k0) load_w(k);
-    uint4 u[kLoraFewAhead];
 #pragma unroll
-    for (int i = 0; i < kLoraFewAhead; ++i) {
-      const int kk = k + 32 * i + 8 * tq;
-      u[i] = ld_or_zero(x + kk, kk < k1 && kk < p.k && gq < p.tokens);
-    }
+    for (int g = 0; g < kGroups; ++g) {
+      const int t = 8 * g + gq;
+      const bf16* x = p.x + (t < p.tokens ? t : 0) * p.x_row_stride;
+      uint4 u[kLoraFewAhead];
 #pragma unroll
-    for (int i = 0; i < kLoraFewAhead; ++i) {
-      const uint32_t f0[4] = {a0[i].x, a1[i].x, a0[i].y, a1[i].y}, f1[4] = {a0[i].z, a1[i].z, a0[i].w, a1[i].w};
-      mma_bf16_16816(acc, f0, u[i].x, u[i].y);
-      mma_bf16_16816(acc, f1, u[i].z, u[i].w);
+      for (int i = 0; i < kLoraFewAhead; ++i) {
+        const int kk = k + 32 * i + 8 * tq;
+        u[i] = ld_or_zero(x + kk, kk < k1 && kk < p.k && t < p.tokens);
+      }
+#pragma unroll
+      for (int i = 0; i < kLoraFewAhead; ++i) {
+        const uint32_t f0[4] = {a0[i].x, a1[i].x, a0[i].y, a1[i].y}, f1[4] = {a0[i].z, a1[i].z, a0[i].w, a1[i].w};
+        mma_bf16_16816(acc[g], f0, u[i].x, u[i].y);
+        mma_bf16_16816(acc[g], f1, u[i].z, u[i].w);
+      }
     }
   }
-  s_red[warp][2 * tq][gq] = acc[0];
-  s_red[warp][2 * tq + 1][gq] = acc[1];
-  s_red[warp][2 * tq][gq + 8] = acc[2];
-  s_red[warp][2 * tq + 1][gq + 8] = acc[3];
-  // this thread's result and half of the ranks
-  const int col = threadIdx.x % kLoraFewCols, t = threadIdx.x / kLoraFewCols % kLoraFewTokens;
-  const bool upper = threadIdx.x >= kLoraFewCols * kLoraFewTokens;
-  const bool mine = t < p.tokens && n0 + col < p.n;
-  const int id = mine ? lora_id(p, t) : -1;
-  const int rank = id >= 0 ? min(max(p.ranks[id], 0), p.rank) : 0;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    s_red[warp][8 * g + 2 * tq][gq] = acc[g][0];
+    s_red[warp][8 * g + 2 * tq + 1][gq] = acc[g][1];
+    s_red[warp][8 * g + 2 * tq][gq + 8] = acc[g][2];
+    s_red[warp][8 * g + 2 * tq + 1][gq + 8] = acc[g][3];
+  }
   __syncthreads();
-  float v = 0.f;
-  const int mid = p.rank / 16 * 8, j0 = upper ? mid : 0, j1 = min(upper ? p.rank : mid, rank);
-  const bf16* b = p.b + (static_cast<long long>(max(id, 0)) * p.n + (mine ? n0 + col : 0)) * p.rank;
+#pragma unroll
+  for (int o = threadIdx.x; o < kLoraFewCols * kTok * kHalves; o += kLoraFewWarps * 32) {
+    const int col = o % kLoraFewCols, t = o / kLoraFewCols % kTok;
+    const bool upper = o >= kLoraFewCols * kTok, mine = t < p.tokens && n0 + col < p.n;
+    const int id = mine ? lora_id(p, t) : -1;
+    const int rank = id >= 0 ? min(max(p.ranks[id], 0), p.rank) : 0;
+    const int mid = kHalves == 2 ? p.rank / 16 * 8 : p.rank, j0 = upper ? mid : 0, j1 = min(upper ? p.rank : mid, rank);
+    const bf16* b = p.b + (static_cast<long long>(max(id, 0)) * p.n + (mine ? n0 + col : 0)) * p.rank;
+    float v = 0.f;
 #pragma unroll 4
-  for (int j = j0; j < j1; j += 8) {
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(b + j));
-    const uint32_t wd[4] = {c.x, c.y, c.z, c.w};
+    for (int j = j0; j < j1; j += 8) {
+      const uint4 c = __ldg(reinterpret_cast<const uint4*>(b + j));
+      const uint32_t wd[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {   // what lies past the rank may be anything
-      if (j + 2 * i < j1) v += s_low[t][j + 2 * i] * bf16lo(wd[i]);
-      if (j + 2 * i + 1 < j1) v += s_low[t][j + 2 * i + 1] * bf16hi(wd[i]);
+      for (int i = 0; i < 4; ++i) {   // what lies past the rank may be anything
+        if (j + 2 * i < j1) v += s_low[t][j + 2 * i] * bf16lo(wd[i]);
+        if (j + 2 * i + 1 < j1) v += s_low[t][j + 2 * i + 1] * bf16hi(wd[i]);
+      }
     }
-  }
-  if (upper) s_half[t][col] = v;
-  __syncthreads();
-  if (upper || !mine) return;
-  float base = 0.f;
+    if (kHalves == 2) {   // one round, of all threads
+      if (upper) s_half[t][col] = v;
+      __syncthreads();
+      if (!upper) v += s_half[t][col];
+    }
+    if (upper || !mine) continue;
+    float base = 0.f;
 #pragma unroll
-  for (int q = 0; q < kLoraFewWarps; ++q) base += s_red[q][t][col];
-  v = base + (v + s_half[t][col]);
-  const long long at = t * p.y_row_stride + n0 + col;
-  if (p.y_f32) reinterpret_cast<float*>(p.y)[at] = v;
-  else reinterpret_cast<bf16*>(p.y)[at] = __float2bfloat16(v);
+    for (int q = 0; q < kLoraFewWarps; ++q) base += s_red[q][t][col];
+    v += base;
+    const long long at = t * p.y_row_stride + n0 + col;
+    if (p.y_f32) reinterpret_cast<float*>(p.y)[at] = v;
+    else reinterpret_cast<bf16*>(p.y)[at] = __float2bfloat16(v);
+  }
 }
 
 // Launch shapes.  A tile of few tokens can hold many adapters: with few tiles they are dealt out to
@@ -582,7 +595,9 @@ cudaError_t launch_lora(const LoraParams& p, int num_sms, cudaStream_t st) {
   else if (p.rank <= 64) launch_low<8>(p, deal, st);
   else launch_low<16>(p, deal, st);
   if (p.w) {   // few tokens
-    launch_kernel(lora_few_kernel, (p.n + kLoraFewCols - 1) / kLoraFewCols, kLoraFewWarps * 32, 0, st, p);
+    const unsigned grid = (p.n + kLoraFewCols - 1) / kLoraFewCols;
+    if (p.tokens <= 8) launch_kernel(lora_few_kernel<1>, grid, kLoraFewWarps * 32, 0, st, p);
+    else launch_kernel(lora_few_kernel<2>, grid, kLoraFewWarps * 32, 0, st, p);
     return cudaGetLastError();
   }
   const int tiles = (p.tokens + kLoraTile - 1) / kLoraTile;

@@ -773,7 +773,7 @@ def lora_splits(tokens: int, k: int, num_sms: int) -> int:
     return max(1, min(6 * num_sms // max(1, (tokens + 15) // 16), k // 256, 16))
 
 
-LORA_GEMV_TOKENS = 8     # up to here lora_linear's shared projection and the adapters' second product are one launch
+LORA_GEMV_TOKENS = 16    # up to here lora_linear's shared projection and the adapters' second product are one launch
 LORA_GEMM_TOKENS = 256   # above, the projection and its adapters can be one GEMM
 
 

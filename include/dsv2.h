@@ -671,7 +671,7 @@ DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* strea
  * ranks[a] of its `rank` rows are used (the rest are not read into the result).  A negative id
  * or token row: no adapter.  base: n_base fp32 partials of the shared projection, 0 = none; with w
  * ([n, k] bf16 rows at w_row_stride) they are computed here (base is then a work buffer and n_base
- * the number of pieces of k, as dsv2_linear's k_splits; one piece and up to 8 tokens: not written), else they are the caller's (dsv2_linear
+ * the number of pieces of k, as dsv2_linear's k_splits; one piece and up to 16 tokens: not written), else they are the caller's (dsv2_linear
  * with DSV2_EPI_STORE_F32).  y: y_dtype DSV2_BF16 (one rounding of the fp32 sum) or
  * DSV2_F32 (with n_base = 0 the adapters' part alone, e.g. one more partial of the projection).
  * low: fp32 work buffer [low_parts, tokens, rank] (low_parts >= 1 pieces of k run side by side);
