@@ -488,10 +488,11 @@ int dsv2_linear(const dsv2_linear_args* a, int family, void* stream) {
   return linear_impl(a, family, stream, false);
 }
 
-int dsv2_lm_head_argmax(const void* w, int vocab, int hidden, const void* x, int64_t x_row_stride,
-                        int n_tokens, uint64_t* keys, int64_t keys_capacity, int64_t* next_ids,
-                        int64_t* input_ids, int64_t* positions, int pos_numel, int64_t* step_counter,
-                        int family, void* stream) {
+// served != nullptr: rows with served[t] < 0 keep their token and position and are counted in *missed
+static int lm_head_argmax_impl(const void* w, int vocab, int hidden, const void* x, int64_t x_row_stride,
+                               int n_tokens, uint64_t* keys, int64_t keys_capacity, int64_t* next_ids,
+                               int64_t* input_ids, int64_t* positions, int pos_numel, int64_t* step_counter,
+                               const int64_t* served, int32_t* missed, int family, void* stream) {
   if (!w || !x || !keys || !next_ids) return fail(DSV2_ERR_INVALID, "lm_head_argmax: null pointer");
   if (vocab <= 0 || hidden <= 0 || n_tokens < 0)
     return fail(DSV2_ERR_INVALID, "lm_head_argmax: vocab %d hidden %d tokens %d", vocab, hidden, n_tokens);
@@ -525,8 +526,28 @@ int dsv2_lm_head_argmax(const void* w, int vocab, int hidden, const void* x, int
                                              reinterpret_cast<long long*>(input_ids),
                                              reinterpret_cast<long long*>(positions), pos_numel,
                                              reinterpret_cast<long long*>(step_counter),
+                                             reinterpret_cast<const long long*>(served), missed,
                                              static_cast<cudaStream_t>(stream)),
                       "lm_head_argmax: finalize");
+}
+
+int dsv2_lm_head_argmax(const void* w, int vocab, int hidden, const void* x, int64_t x_row_stride,
+                        int n_tokens, uint64_t* keys, int64_t keys_capacity, int64_t* next_ids,
+                        int64_t* input_ids, int64_t* positions, int pos_numel, int64_t* step_counter,
+                        int family, void* stream) {
+  return lm_head_argmax_impl(w, vocab, hidden, x, x_row_stride, n_tokens, keys, keys_capacity, next_ids, input_ids,
+                             positions, pos_numel, step_counter, nullptr, nullptr, family, stream);
+}
+
+int dsv2_lm_head_argmax_served(const void* w, int vocab, int hidden, const void* x, int64_t x_row_stride,
+                               int n_tokens, uint64_t* keys, int64_t keys_capacity, int64_t* next_ids,
+                               int64_t* input_ids, int64_t* positions, int pos_numel, int64_t* step_counter,
+                               const int64_t* served, int32_t* missed, int family, void* stream) {
+  if (!served || !missed) return fail(DSV2_ERR_INVALID, "lm_head_argmax_served: null pointer");
+  if (positions && pos_numel != n_tokens)
+    return fail(DSV2_ERR_INVALID, "lm_head_argmax_served: %d positions for %d tokens", pos_numel, n_tokens);
+  return lm_head_argmax_impl(w, vocab, hidden, x, x_row_stride, n_tokens, keys, keys_capacity, next_ids, input_ids,
+                             positions, pos_numel, step_counter, served, missed, family, stream);
 }
 
 static int linear_impl(const dsv2_linear_args* a, int family, void* stream, bool argmax) {

@@ -318,13 +318,16 @@ __global__ void sum_partials_kernel(const float* __restrict__ part, int n_parts,
 
 // Greedy token per row from the per-block arg-max keys [n_blocks][key_stride] (largest
 // key = largest bf16 logit, lowest vocabulary index on ties): next_ids[t] = index; also
-// input_ids[t] = index and positions[t] += 1 when given (the end of a decode step).
+// input_ids[t] = index and positions[t] += 1 when given (the end of a decode step).  With `served` a row
+// with served[t] < 0 had no place in the cache: it keeps its token and position, next_ids[t] = -1, and *missed
+// counts it.
 __global__ __launch_bounds__(256) void argmax_finalize_kernel(const unsigned long long* __restrict__ keys,
                                                               int n_blocks, long long key_stride,
                                                               long long* __restrict__ next_ids,
                                                               long long* __restrict__ input_ids,
                                                               long long* __restrict__ positions,
-                                                              int pos_numel, long long* step_counter) {
+                                                              int pos_numel, long long* step_counter,
+                                                              const long long* __restrict__ served, int* missed) {
   pdl_enter();
   if (step_counter && blockIdx.x == 0 && threadIdx.x == 0) *step_counter += 1;
   __shared__ unsigned long long s_best[8];
@@ -339,6 +342,11 @@ __global__ __launch_bounds__(256) void argmax_finalize_kernel(const unsigned lon
     for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) best = max(best, s_best[w]);
     best = max(best, s_best[0]);
     const long long idx = static_cast<long long>(0xffffffffu - static_cast<uint32_t>(best & 0xffffffffu));
+    if (served && served[t] < 0) {
+      next_ids[t] = -1;
+      atomicAdd(missed, 1);
+      return;
+    }
     next_ids[t] = idx;
     if (input_ids) input_ids[t] = idx;
     if (positions && (pos_numel != 1 || t == 0)) positions[pos_numel == 1 ? 0 : t] += 1;
@@ -468,9 +476,9 @@ cudaError_t launch_sum_partials(const float* part, int n_parts, long long ps, lo
 cudaError_t launch_argmax_finalize(const unsigned long long* keys, int n_blocks, long long key_stride,
                                    int n_tokens, long long* next_ids, long long* input_ids,
                                    long long* positions, int pos_numel, long long* step_counter,
-                                   cudaStream_t st) {
+                                   const long long* served, int* missed, cudaStream_t st) {
   launch_kernel(argmax_finalize_kernel, n_tokens, 256, 0, st, keys, n_blocks, key_stride, next_ids, input_ids,
-                positions, pos_numel, step_counter);
+                positions, pos_numel, step_counter, served, missed);
   return cudaGetLastError();
 }
 

@@ -233,7 +233,7 @@ cudaError_t launch_advance_positions(long long*, int, cudaStream_t);
 cudaError_t launch_argmax_finalize(const unsigned long long* keys, int n_blocks, long long key_stride,
                                    int n_tokens, long long* next_ids, long long* input_ids,
                                    long long* positions, int pos_numel, long long* step_counter,
-                                   cudaStream_t st);
+                                   const long long* served, int* missed, cudaStream_t st);
 // router.cu
 cudaError_t launch_router(const RouterParams&, int max_clusters, int num_sms, cudaStream_t);
 cudaError_t router_fused_max_clusters(int* n);

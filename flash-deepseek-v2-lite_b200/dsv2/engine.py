@@ -17,8 +17,10 @@ all-gathered and the expert outputs reduce-scattered with NCCL inside the graph.
 
 kv_format="int4" keeps the latent cache in 4 bits in pages (dsv2.serving.PagedCache4): every
 step first plans its pages and slots on the device, then quantises the new rows into them and
-attends over the pages.  adapters= adds each request's low-rank adapter to the query + latent
-and the output projection.  Both are for one rank.
+attends over the pages.  A request that gets no page keeps its length and token, and goes on once
+pages are free again; plan.check() raises if there was one.  plan.new stays as it is (one token of
+every request: rows are requests).  adapters= adds each request's low-rank adapter to the query +
+latent and the output projection.  Both are for one rank.
 """
 from __future__ import annotations
 
@@ -539,7 +541,8 @@ class DecodeEngine:
         # advances the positions (src/run.py:585-588)
         ops.lm_head_argmax(w=self.lm_head, x=self.x, keys=self.argmax_keys, next_ids=self.next_ids,
                            family=self.family, input_ids=self.input_ids, positions=self.positions,
-                           step_counter=self.step_count)
+                           step_counter=self.step_count,
+                           **(dict(served=self.plan.positions, missed=self.plan.missed) if self.kv_format == "int4" else {}))
 
     def _add_rmsnorm(self, delta, w, eps) -> None:
         """Residual add of the previous sublayer's output + the next RMSNorm; an expert-parallel
@@ -554,20 +557,23 @@ class DecodeEngine:
     def set_state(self, positions: torch.Tensor, input_ids: torch.Tensor) -> None:
         self.positions.copy_(positions.to(self.positions))
         self.input_ids.copy_(input_ids.to(self.input_ids).view(-1))
-        # the ring of free pages goes back with the positions: the steps after restore() take the
-        # same pages again
-        self._saved = (self.positions.clone(), self.input_ids.clone(),
-                       self.paged.ring.clone() if self.kv_format == "int4" else None)
+        self._saved = (self.positions.clone(), self.input_ids.clone())
+        if self.kv_format == "int4":
+            # the ring of free pages goes back with the positions: the steps after restore() take the
+            # same pages again
+            self.plan.clear()
+            self._saved += (self.paged.ring.clone(),)
 
     def restore(self) -> None:
         """Roll back positions / next tokens to the post-prefill state.  Cache rows at or
         beyond a row's position are never read before being rewritten, so the latent cache
         needs no snapshot (unlike the expanded cache of src/run.py:161-217)."""
-        pos, ids, ring = self._saved
+        pos, ids, *ring = self._saved
         self.positions.copy_(pos)
         self.input_ids.copy_(ids)
-        if ring is not None:
-            self.paged.ring.copy_(ring)
+        if ring:
+            self.paged.ring.copy_(ring[0])
+            self.plan.clear()
 
     def capture(self, warmup: int = 3) -> None:
         """Warm up eagerly (rolled back), then capture one decode step in a CUDA graph."""

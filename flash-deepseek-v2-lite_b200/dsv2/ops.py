@@ -266,10 +266,13 @@ def moe(*, gate_up: torch.Tensor, down: torch.Tensor, x_sorted: torch.Tensor, h:
 
 def lm_head_argmax(*, w: torch.Tensor, x: torch.Tensor, keys: torch.Tensor, next_ids: torch.Tensor,
                    family: int, input_ids: torch.Tensor | None = None,
-                   positions: torch.Tensor | None = None, step_counter: torch.Tensor | None = None) -> None:
+                   positions: torch.Tensor | None = None, step_counter: torch.Tensor | None = None,
+                   served: torch.Tensor | None = None, missed: torch.Tensor | None = None) -> None:
     """next_ids[t] = argmax over the vocabulary of bf16(x[t] @ w^T) (lowest index on ties),
     without materialising the logits; optionally input_ids = next_ids and positions += 1.
-    keys: uint64 (int64) work buffer of at least ceil(vocab / 16) * tokens entries."""
+    keys: uint64 (int64) work buffer of at least ceil(vocab / 16) * tokens entries.
+    served (int64 [T], e.g. a page plan's positions): a row with served[t] < 0 keeps its token and
+    position, next_ids[t] = -1, and missed (int32 [1]) counts it."""
     _cuda(x, "x")
     if w.dtype != torch.bfloat16 or x.dtype != torch.bfloat16 or w.stride(1) != 1 or x.stride(1) != 1:
         raise NotImplementedError("lm_head_argmax supports bf16 weights/activations with contiguous rows")
@@ -277,9 +280,15 @@ def lm_head_argmax(*, w: torch.Tensor, x: torch.Tensor, keys: torch.Tensor, next
         raise ValueError("next_ids must be int64 and keys 64-bit")
     vocab, hidden = w.shape
     n = x.shape[0]
-    _lib.call("dsv2_lm_head_argmax", w.data_ptr(), vocab, hidden, x.data_ptr(), x.stride(0), n, keys.data_ptr(),
-              keys.numel(), next_ids.data_ptr(), _ptr(input_ids), _ptr(positions),
-              positions.numel() if positions is not None else 0, _ptr(step_counter), family, stream())
+    args = (w.data_ptr(), vocab, hidden, x.data_ptr(), x.stride(0), n, keys.data_ptr(), keys.numel(), next_ids.data_ptr(),
+            _ptr(input_ids), _ptr(positions), positions.numel() if positions is not None else 0, _ptr(step_counter))
+    if served is None:
+        _lib.call("dsv2_lm_head_argmax", *args, family, stream())
+        return
+    if missed is None:
+        raise ValueError("lm_head_argmax: served needs missed, which counts the other rows")
+    _lib.call("dsv2_lm_head_argmax_served", *args, _need(served, "served", torch.int64, n),
+              _need(missed, "missed", torch.int32, 1), family, stream())
 
 
 def router(*, x: torch.Tensor, w: torch.Tensor, scaling: float, logits: torch.Tensor,

@@ -149,6 +149,8 @@ def run_graph_decode(model, prompt: torch.Tensor, batch: int, max_new_tokens: in
             add_trace(step, toks, prompt_len + step)
     torch.cuda.synchronize(dev)
     decode_s = time.perf_counter() - t0
+    if kv_cache == "int4":
+        eng.plan.check()
     eng.release()
     decode_tokens = batch * max(max_new_tokens - 1, 0)
     out = {"batch_size": batch, "path": f"dsv2_{family}_graph", "ttft_ms": prefill_s * 1000.0,

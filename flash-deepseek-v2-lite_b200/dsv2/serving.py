@@ -32,7 +32,8 @@ class PagedCache4:
         if self.pages <= 0:
             raise ValueError("the pool needs at least one page")
         self.cache = ops.latent4_cache(self.pages, page_size, device, layers=layers)
-        self.block_table = torch.zeros((requests, self.width), device=device, dtype=torch.int32)
+        # an entry that was never given names no page: a length that claims it is flagged, not served from page 0
+        self.block_table = torch.full((requests, self.width), -1, device=device, dtype=torch.int32)
         self.free_ring = torch.arange(self.pages, device=device, dtype=torch.int32)
         self.ring = torch.tensor([0, self.pages], device=device, dtype=torch.int64)
 
@@ -40,10 +41,13 @@ class PagedCache4:
         """Give every page back (all requests start over)."""
         self.free_ring.copy_(torch.arange(self.pages, device=self.free_ring.device, dtype=torch.int32))
         self.ring.copy_(torch.tensor([0, self.pages], dtype=torch.int64))
+        self.block_table.fill_(-1)
 
 
 class PagePlan:
-    """Buffers of a step's page plan: `capacity` token rows over the cache's requests."""
+    """Buffers of a step's page plan: `capacity` token rows over the cache's requests.  missed counts
+    the rows that an engine's steps could not serve since clear(): they have kept their length and
+    token (dsv2.ops.lm_head_argmax), also in steps replayed from a graph."""
 
     def __init__(self, paged: PagedCache4, capacity: int, new: torch.Tensor | None = None):
         dev = paged.block_table.device
@@ -51,6 +55,7 @@ class PagePlan:
         self.new = torch.ones(paged.requests, device=dev, dtype=torch.int32) if new is None else new
         self.buf = ops.page_plan_buffers(paged.requests, capacity, dev)
         self.buf["ring_out"] = paged.ring           # the ring advances in place
+        self.missed = torch.zeros(1, device=dev, dtype=torch.int32)
 
     def run(self, cached: torch.Tensor) -> None:
         """Append `new` tokens to the requests that hold `cached` ones (int32 / int64 [requests])."""
@@ -71,11 +76,17 @@ class PagePlan:
         return self.buf["token_row"]
 
     def check(self) -> None:
-        """Raise if the last step could not serve every request (synchronises)."""
-        n = int(self.buf["counts"][3])
-        if n:
-            raise RuntimeError(f"page plan: {n} request(s) got no pages ({self.paged.pages} pages of "
-                               f"{self.paged.page_size} tokens)")
+        """Raise if the last step, or an engine's step since clear(), could not serve every request
+        (synchronises)."""
+        n, m = int(self.buf["counts"][3]), int(self.missed)
+        if n or m:
+            raise RuntimeError(f"page plan: {n} request(s) got no pages in the last step, {m} token row(s) since the count "
+                               f"was cleared ({self.paged.pages} pages of {self.paged.page_size} tokens)")
+
+    def clear(self) -> None:
+        """Forget the steps that could not serve every request."""
+        self.missed.zero_()
+        self.buf["counts"].zero_()
 
 
 @dataclass

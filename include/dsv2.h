@@ -341,6 +341,15 @@ DSV2_API int dsv2_lm_head_argmax(const void* w, int vocab, int hidden, const voi
                                  int64_t keys_capacity, int64_t* next_ids, int64_t* input_ids,
                                  int64_t* positions, int pos_numel, int64_t* step_counter,
                                  int family, void* stream);
+/* dsv2_lm_head_argmax where not every row had a place in the cache (dsv2_page_plan): a row with
+ * served[t] < 0 (int64 [n_tokens], e.g. the plan's positions) keeps input_ids[t] and
+ * positions[t], next_ids[t] = -1, and missed[0] (int32) grows by one.  positions, when given,
+ * holds one entry per token. */
+DSV2_API int dsv2_lm_head_argmax_served(const void* w, int vocab, int hidden, const void* x,
+                                        int64_t x_row_stride, int n_tokens, uint64_t* keys,
+                                        int64_t keys_capacity, int64_t* next_ids, int64_t* input_ids,
+                                        int64_t* positions, int pos_numel, int64_t* step_counter,
+                                        const int64_t* served, int32_t* missed, int family, void* stream);
 
 /* ---- MoE routing ------------------------------------------------------------ */
 /* Gate GEMV (fp32 over bf16 activations) + softmax + top-6, then bucketing.
