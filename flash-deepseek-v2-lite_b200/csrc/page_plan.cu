@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(const PagePlanP
     const int n = min(kPlanThreads, p.requests - r0), r = r0 + tid;
     // --- this chunk's requests
     PlanScan v = {0, 0, 0};
-    int cached = 0, fresh = 0;
+    int cached = 0, fresh = 0, kept = 0;   // kept: the length that a request which is not served keeps
     bool finished = false, fits = false;
     if (tid < n) {
       const long long c = p.cached64 ? reinterpret_cast<const long long*>(p.cached)[r] : reinterpret_cast<const int*>(p.cached)[r];
@@ -76,6 +76,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(const PagePlanP
       const bool ok = c >= 0 && c <= most && nw >= -1;
       finished = ok && nw < 0;
       cached = ok ? static_cast<int>(c) : 0;
+      kept = static_cast<int>(min(max(c, -0x80000000LL), 0x7fffffffLL));
       fresh = ok ? max(nw, 0) : 0;
       fits = ok && nw >= 0 && c + fresh <= most;
       if (!ok || (nw >= 0 && !fits)) set_device_error(kErrIndex);
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(const PagePlanP
     const long long upto = served && mine.need > 0 ? base.need + v.need : 0;
     if (tid < n && !served && !finished) atomicAdd(&s_deferred, 1);
     if (cta == (r0 / kPlanThreads) % grid && tid < n) {
-      p.lens[r] = finished ? 0 : (served ? cached + fresh : cached);
+      p.lens[r] = finished ? 0 : (served ? cached + fresh : kept);
       p.cu_new[r + 1] = static_cast<int>(min(base.tok + v.tok, 0x7fffffffLL));
     }
     // pages taken: the largest U_r of a served request (served requests that need pages come first)

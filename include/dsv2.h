@@ -603,8 +603,8 @@ DSV2_API int dsv2_mla_decode_noalloc(const void* q_abs, const void* q_pe, const 
  *     for, pages taken, pages put, requests not served}.
  * lens must not overlap cached.  sync: one int32, zero before the first call and left zero;
  * calls that share it must not overlap on the GPU.  A negative or too long request (more than
- * width pages) is not served and sets DSV2_DEVERR_INDEX, as does a ring whose counters are
- * impossible. */
+ * width pages) or fresh[r] below -1 is not served (lens[r] = cached[r], within int32's range) and sets
+ * DSV2_DEVERR_INDEX, as does a ring whose counters are impossible. */
 typedef struct dsv2_page_plan_args {
   const void* cached;        /* [requests] int32, or int64 when cached_is64 */
   const int32_t* fresh;      /* [requests] */
