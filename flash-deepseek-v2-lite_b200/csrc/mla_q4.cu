@@ -573,12 +573,16 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
         if (g >= 2) q4_wait(&sm.p_empty[buf], ((g >> 1) - 1) & 1, s_abort);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float p0 = ex2(s[j][0] - u0), p1 = ex2(s[j][1] - u0), p2 = ex2(s[j][2] - u1), p3 = ex2(s[j][3] - u1);
-          l0 += p0 + p1;
-          l1 += p2 + p3;
+          // P is bf16 (2^-8; another bf16 part of it would double the P V product, which bounds long rows).  l sums
+          // what is stored: the weights that are used add up to 1, and a token that decides the row alone comes out
+          // as it is in the cache
+          const uint32_t w0 = pack_bf16x2(ex2(s[j][0] - u0), ex2(s[j][1] - u0));
+          const uint32_t w1 = pack_bf16x2(ex2(s[j][2] - u1), ex2(s[j][3] - u1));
+          l0 += bf16lo(w0) + bf16hi(w0);
+          l1 += bf16lo(w1) + bf16hi(w1);
           const int col = 16 * warp + 8 * j + 2 * tq;
-          *reinterpret_cast<uint32_t*>(&sm.p[buf][gq][col]) = pack_bf16x2(p0, p1);
-          *reinterpret_cast<uint32_t*>(&sm.p[buf][gq + 8][col]) = pack_bf16x2(p2, p3);
+          *reinterpret_cast<uint32_t*>(&sm.p[buf][gq][col]) = w0;
+          *reinterpret_cast<uint32_t*>(&sm.p[buf][gq + 8][col]) = w1;
         }
         if (warp == 0) {
           if (tq == 0) {

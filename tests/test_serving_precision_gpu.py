@@ -1,0 +1,139 @@
+"""What the serving operators keep of their inputs' precision, with bounds for each path of the adapters and
+rows of attention that one token decides."""
+import math
+
+import pytest
+import torch
+
+from oracle import serving as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def D():
+    from dsv2 import _lib, ops
+    _lib.load()
+    _lib.device_error(clear=True)
+    return ops
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    from dsv2 import _lib
+    _lib.device_error(clear=True)
+    yield
+    assert _lib.device_error(clear=True) == 0
+
+
+# ------------------------------------------------------------------ attention
+SCALE = 192 ** -0.5
+
+
+class Pages:
+    """Sequences of given lengths in shuffled pages (values of few distinct rows: quick to make)."""
+
+    def __init__(self, D, lens, page, seed):
+        g = torch.Generator().manual_seed(seed)
+        self.page, self.lens = page, lens
+        held = [-(-n // page) for n in lens]
+        order = torch.randperm(sum(held) + 3, generator=g)
+        self.table = torch.full((len(lens), max(held) + 2), -1, dtype=torch.int32)
+        self.cache = torch.randint(0, 256, (sum(held) + 3, page // 16 * 6400), generator=g, dtype=torch.uint8).to(DEV)
+        self.rows, at = [], 0
+        for i, n in enumerate(lens):
+            pages = order[at:at + held[i]]
+            at += held[i]
+            self.table[i, :held[i]] = pages.to(torch.int32)
+            rows = torch.randn(n, 576, generator=g).to(torch.bfloat16)
+            t = torch.arange(n)
+            D.latent4_write(rows=rows.to(DEV), slots=(pages[t // page] * page + t % page).to(DEV), cache=self.cache)
+            self.rows.append(S.values(rows))
+
+    def run(self, D, q_abs, q_pe, positions, seq_rows=None, scale=SCALE, table=None):
+        n = q_abs.shape[0]
+        out = torch.full((n, 16, 512), math.nan, dtype=torch.bfloat16, device=DEV)
+        D.mla_decode_q4(q_abs=q_abs.to(DEV), q_pe=q_pe.to(DEV), cache=self.cache,
+                        block_table=self.table.to(DEV) if table is None else table,
+                        positions=torch.tensor(positions, device=DEV), page_size=self.page, softmax_scale=scale, o_lat=out,
+                        seq_rows=None if seq_rows is None else torch.tensor(seq_rows, dtype=torch.int32, device=DEV),
+                        **D.mla_q4_workspace(n, DEV))
+        return out.cpu().double()
+
+
+@pytest.mark.parametrize("n,page", [(1, 16), (70, 16), (513, 48), (3000, 64), (9001, 64)])
+def test_attention_counts_every_token_once(D, n, page):
+    """Head h sees eight tokens alone (at block, tile and page edges, the first and the last among them), all with the same
+    score: its result is the mean of their rows.  A token lost or counted twice moves it by a tenth of a row."""
+    pg = Pages(D, [n], page, seed=n)
+    g = torch.Generator().manual_seed(n + 1)
+    edges = torch.tensor(sorted({t for b in range(0, n, 16) for t in (b, b + 15) if t < n} | {n - 1}))
+    q_pe = torch.zeros(1, 16, 64)
+    q_pe[0, torch.arange(16), torch.arange(16)] = 16.0
+    for batch in range(3):
+        rows = pg.rows[0].to(torch.bfloat16)              # (exact: quantised values are bf16 numbers)
+        rows[:, 512:] = 0
+        groups = []
+        for h in range(16):
+            pick = edges[torch.randperm(len(edges), generator=g)[:8]]
+            if h < 4:
+                pick[0] = n - 1 if h % 2 else 0
+            groups.append(pick.unique())
+            rows[groups[-1], 512 + h] = 16.0              # score 256 against 0
+        t = torch.arange(n)
+        slots = pg.table[0].long()[t // page] * page + t % page
+        D.latent4_write(rows=rows.to(DEV), slots=slots.to(DEV), cache=pg.cache)
+        val = S.values(rows)[:, :512]
+        got = pg.run(D, torch.zeros(1, 16, 512, dtype=torch.bfloat16), q_pe.to(torch.bfloat16), [n - 1], scale=1.0)[0]
+        for h, grp in enumerate(groups):
+            want, mag = val[grp].mean(0), val[grp].abs().mean(0)
+            # the result's bf16 rounding; sums of at most 8 products of 8-bit numbers, in fp32
+            assert float(((got[h] - want).abs() - 2.0 ** -8 * want.abs() - 2.0 ** -18 * mag - 1e-30).max()) <= 0, (batch, h)
+
+
+def test_attention_divides_by_the_probabilities_that_it_multiplies(D):
+    """Every token holds the same latent row, so the result is that row, a bf16 number, whatever the probabilities are
+    rounded to, if their sum is that of the rounded ones.  Token 130 has 128.05 .. 128.95 times the probability of token 0,
+    in a later tile (where the maximum is not taken anew: it would round by up to 2^-8); the others have none."""
+    n, R = 144, 2000
+    pg = Pages(D, [n], 16, seed=1)
+    rows = torch.randn(1, 576, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).repeat(n, 1)
+    rows[:, 512:] = 0
+    rows[130, 512], rows[130, 513] = 1, 1
+    rows[:, 514] = 1
+    rows[0, 514] = rows[130, 514] = 0
+    t = torch.arange(n)
+    D.latent4_write(rows=rows.to(DEV), slots=(pg.table[0].long()[t // 16] * 16 + t % 16).to(DEV), cache=pg.cache)
+    q_pe = torch.zeros(16, 64)
+    q_pe[:, 0] = 7.0
+    q_pe[:, 1] = torch.log2(1 + torch.linspace(0.05, 0.95, 16) / 128)
+    q_pe[:, 2] = -1000.0
+    got = pg.run(D, torch.zeros(R, 16, 512, dtype=torch.bfloat16), q_pe.to(torch.bfloat16).expand(R, 16, 64).contiguous(),
+                 [n - 1] * R, [0] * R, scale=math.log(2))
+    want = S.values(rows[:1])[:, :512].expand(R, 16, 512)
+    assert torch.equal(got, want), int((got != want).sum())
+
+
+@pytest.mark.parametrize("R", [639, 640, 641, 1290])
+def test_attention_of_many_rows(D, R):
+    """Prompt rows: more query rows than the launch has threads, several sequences, tables with wide rows."""
+    lens = [211, 90, 330, 17]
+    pg = Pages(D, lens, 32, seed=R)
+    g = torch.Generator().manual_seed(R)
+    seq = torch.randint(-1, len(lens), (R,), generator=g).tolist()
+    pos = [int(torch.randint(0, lens[s], (1,), generator=g)) if s >= 0 else 3 for s in seq]
+    q_abs = torch.randn(R, 16, 512, generator=g).to(torch.bfloat16)
+    q_pe = torch.randn(R, 16, 64, generator=g).to(torch.bfloat16)
+    wide = torch.full((len(lens), pg.table.shape[1] + 5), 10 ** 6, dtype=torch.int32)
+    wide[:, :pg.table.shape[1]] = pg.table
+    got = pg.run(D, q_abs, q_pe, pos, seq, table=wide.to(DEV)[:, :pg.table.shape[1]])
+    for r in sorted({0, 1, R // 2, 638, R - 2, R - 1} | set(range(5, R, 37))):
+        m = 0 if seq[r] < 0 else pos[r] + 1
+        v = pg.rows[seq[r]][:m] if m else torch.zeros(0, 576).double()
+        want, mag, terms = S.attention(q_abs[r].double(), q_pe[r].double(), v[:, :512], v[:, 512:], SCALE)
+        # the stored probabilities and the result in bf16, scores off by d in the exponent
+        d = 576 * 2.0 ** -24 * terms
+        assert float(((got[r] - want).abs() - (2.0 ** -7 + 2 * d) * mag - 1e-30).max()) <= 0, r
+        if m == 0:
+            assert not bool(got[r].any())
