@@ -23,8 +23,9 @@
 //    memory through registers into ring stages; the loads are on their way before the stage is free.
 //    (One group: 1024 tokens with 64 adapters 45 us, two: 41.)  A plain copy will not do: what an adapter's
 //    padding past its rank holds must not be multiplied, nor may an infinity or a NaN of one adapter
-//    meet the zeros that other adapters' tokens have in its columns.  Such values enter as zeros, and
-//    the epilogue adds their products to the rows of their own adapter.
+//    meet the zeros that other adapters' tokens have in its columns.  Such values, and those of low, which would
+//    meet the zeros that stand for them, enter as zeros, and the epilogue adds their products to the rows of
+//    their own adapter.
 // low enters as bf16: its rounding (2^-9 of the adapters' part) is below that of y.
 // 4001 tokens, 6 adapters of rank 32, 2048 -> 3648: about 46 of the 71 us that the order, the rows and
 // this take together; 1.3 PFLOP/s.  Bound by the multiplications with what the last tiles leave idle:
@@ -120,7 +121,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
   uint64_t* tempty_bar = tfull_bar + 2;           // [2] (the first CTA's)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* odd_flag = abort_flag + 1;        // an adapter's B held an infinity or a NaN
+  volatile int* odd_flag = abort_flag + 1;        // an adapter's B or low held an infinity or a NaN
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t half = cluster_ctarank();        // of the pair
   const int pair = cluster_id_x(), pairs = n_clusters_x();
@@ -286,9 +287,9 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
         const bf16* b = p.b + (static_cast<long long>(a) * p.n + nt * n_tile) * p.rank;
         for (int c = 0; c < cols; ++c, b += p.rank)
           for (int j = 0; j < rank; ++j) {
-            const float w = __bfloat162float(b[j]);
-            if (isfinite(w)) continue;
-            y[c] = __float2bfloat16(__bfloat162float(y[c]) + __bfloat162float(low[j]) * w);
+            const float w = __bfloat162float(b[j]), l = __bfloat162float(low[j]);
+            if (isfinite(w) && isfinite(l)) continue;
+            y[c] = __float2bfloat16(__bfloat162float(y[c]) + l * w);
           }
       }
     }
@@ -346,7 +347,10 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
         }
         bool odd = false;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) odd |= drop_nonfinite(rb[c]);
+        for (int c = 0; c < 8; ++c) {
+          odd |= drop_nonfinite(ra[c]);
+          odd |= drop_nonfinite(rb[c]);
+        }
         if (odd)
           for (uint32_t r = 0; r < 2; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(const_cast<int*>(odd_flag), r)), "r"(1) : "memory");
         if (mbar_wait(&go_bar[group * kLgStages + st_i], parity)) {

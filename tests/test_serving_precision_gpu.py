@@ -27,6 +27,59 @@ def no_device_error():
     assert _lib.device_error(clear=True) == 0
 
 
+# ------------------------------------------------------------------ adapters
+def lora_case(T, n_ad, rank, K, N, seed, cancel=False):
+    g = torch.Generator().manual_seed(seed)
+
+    def bf(*shape, std=1.0):
+        return (torch.randn(*shape, generator=g) * std).to(torch.bfloat16)
+    c = {"x": bf(T, K), "w": bf(N, K, std=0.02), "a": bf(n_ad, rank, K, std=K ** -0.5), "b": bf(n_ad, N, rank, std=0.5),
+         "ids": torch.randint(-1, n_ad, (T,), generator=g, dtype=torch.int32),
+         "ranks": torch.randint(max(2, rank - 7), rank + 1, (n_ad,), generator=g, dtype=torch.int32),
+         "scales": torch.rand(n_ad, generator=g) + 0.5}
+    if cancel:
+        # ranks 0 and 1 cancel, 48 low_0 - 64 (3 / 4 low_0), and are far larger than what is left; x in 16ths up to 4 and
+        # powers of two in A make both sums exact in fp32
+        c["x"] = (torch.randn(T, K, generator=g) * 16).round().clamp(-64, 64).div(16).to(torch.bfloat16)
+        e = torch.randint(0, 2, (n_ad, K), generator=g) - round(math.log2(K) / 2)
+        c["a"][:, 0] = (torch.exp2(e.float()) * (torch.randint(0, 2, (n_ad, K), generator=g) * 2 - 1)).to(torch.bfloat16)
+        c["a"][:, 1] = 0.75 * c["a"][:, 0]
+        c["b"] *= 0.01
+        c["b"][:, :, 0] = 48.0
+        c["b"][:, :, 1] = -64.0
+        c["w"] *= 0.05
+    for i, r in enumerate(c["ranks"].tolist()):
+        c["a"][i, r:] = math.nan
+        c["b"][i, :, r:] = math.nan
+    return c
+
+
+@pytest.mark.parametrize("T", [6, 40, 300])
+def test_lora_infinities_on_both_sides(D, T):
+    """An infinite low-rank activation that meets an infinity of B is an infinity (or, of opposite
+    signs, a NaN), as in 64 bits, whatever the number of tokens."""
+    K, N, rank = 256, 72, 24
+    c = lora_case(T, 2, rank, K, N, seed=T)
+    c["ranks"][:] = rank
+    g = torch.Generator().manual_seed(7)
+    c["a"] = (torch.randn(2, rank, K, generator=g) * K ** -0.5).to(torch.bfloat16)
+    c["b"] = (torch.rand(2, N, rank, generator=g) + 0.25).to(torch.bfloat16)       # no zeros
+    c["ids"][:] = torch.arange(T) % 3 - 1
+    c["x"][:, 0] = 1.0
+    c["a"][1, 3, 0] = math.inf                           # low[:, 3] of every token of adapter 1
+    c["b"][1, 5, 3], c["b"][1, 9, 3], c["b"][1, 11, 6] = math.inf, -math.inf, math.inf
+    c["b"][1, 13, 3] = -0.5
+    y = torch.empty(T, N, dtype=torch.bfloat16, device=DEV)
+    D.lora_linear(**{k: v.to(DEV) for k, v in c.items()}, y=y, **D.lora_workspace(T, N, K, rank, DEV))
+    want = S.lora(c["x"], c["w"], c["a"], c["b"], c["ids"].tolist(), c["ranks"], c["scales"])[0]
+    y = y.cpu().double()
+    own = c["ids"] == 1
+    sane = want.isfinite()
+    assert torch.equal(y.isnan(), want.isnan())
+    assert torch.equal(y[~sane & ~want.isnan()], want[~sane & ~want.isnan()])
+    assert bool((~sane)[own].any()) and bool(sane[~own].all())
+
+
 # ------------------------------------------------------------------ attention
 SCALE = 192 ** -0.5
 
