@@ -8,12 +8,23 @@ namespace {
 // shared / separate: 1 token 7.3 / 9.2 us, 9 of rank 16 8.1 / 15.4, 16 of rank 32 11.5 / 17.8, 16 of rank
 // 64 18.8 / 27.8; 32 of rank 32 15.8 / 16.2, of rank 128 36 / 23)
 constexpr int kLoraGemvTokens = 16;
-// The projection and its adapters are one GEMM above 256 tokens with 12 or more per adapter: it pays a
-// pass that orders the tokens and a step per 64 ranks of every adapter in a tile, and saves the fp32
-// partials.  n 3648, k 2048, rank 32, one GEMM / separate launches: 257 tokens 22 / 28 us with 1 adapter,
-// 27.5 / 29 with 16, 37 / 31 with 32, 56 / 34 with 64; 768 tokens 37 / 48 with 64; 1024 tokens 29 / 39 with
-// 1, 35 / 40 with 64; 4001 with 6 71 / 133.  Up to 256 tokens the projection reads its weights once either way.
-constexpr int kLoraGemmTokens = 256, kLoraGemmPerAdapter = 12;
+// The projection and its adapters are one GEMM above 256 tokens where the adapters' steps are few beside the
+// projection's: it pays a pass that orders the tokens and a step for every two pieces of 16 ranks in a tile, and
+// saves the fp32 partials.  The limit is 16 + k / 128 pieces up to 512 tokens and half as many again above, where the
+// partials weigh more.  One GEMM / separate launches, us, (pieces):
+//   k 2048, n 3648: 257 tokens of rank 32 with 10 adapters 29.2 / 29.3 (20), with 16 30.9 / 29.6 (32), with 42 54 / 32 (84);
+//     400 of rank 64 with 10 33 / 35 (28), with 25 45 / 37 (68); 768 of rank 64 with 32 46 / 54 (44), with 64 62 / 59 (88);
+//     1024 of rank 32 with 64 37 / 39 (34), with 128 52 / 45 (66); 4001 with 6 71 / 133 (2)
+//   k 256, n 3648: 300 of rank 16 with 18 19.6 / 19.9 (16), with 30 24.6 / 21.0 (26); 1024 with 102 31 / 34 (26), with 170
+//     40.0 / 38.6 (43)
+//   k 10944, n 2048, rank 128: 300 with 12 102 / 152 (88), with 37 191 / 187 (256)
+// Up to 256 tokens the projection reads its weights once either way.
+constexpr int kLoraGemmTokens = 256;
+bool lora_one_gemm(long long tokens, long long adapters, long long rank, long long k) {
+  // adapters of a tile, if the tokens are spread over them evenly, and their pieces
+  const long long in_tile = std::min(adapters, adapters * kLgM / tokens + 1), pieces = in_tile * ((rank + kLgPiece - 1) / kLgPiece);
+  return tokens > kLoraGemmTokens && k % 64 == 0 && 2 * pieces < (tokens > 2 * kLoraGemmTokens ? 3 : 2) * (16 + k / 128);
+}
 // fewest units of a CTA (64 positions): one row of 512 with 1 / 4 / 16: 13.9 / 13.6 / 14.8 us, of 64:
 // 11.7 / 10.3 / 10.3
 constexpr int kQ4MinUnits = 4;
@@ -161,8 +172,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
     return fail(DSV2_ERR_INVALID, "lora: tokens %d adapters %d partials %d", a->tokens, a->adapters, a->n_base);
   if (a->tokens == 0) return DSV2_OK;
   // a long run of tokens: one GEMM over the tokens in adapter order, no partials
-  const bool fused = a->w && a->xs && a->lists && a->tokens > kLoraGemmTokens &&
-                     a->tokens >= static_cast<long long>(kLoraGemmPerAdapter) * a->adapters && a->y_dtype == DSV2_BF16 && a->k % 64 == 0;
+  const bool fused = a->w && a->xs && a->lists && a->y_dtype == DSV2_BF16 && lora_one_gemm(a->tokens, a->adapters, a->rank, a->k);
   if (a->w && !fused && (!a->base || a->n_base < 1)) return fail(DSV2_ERR_INVALID, "lora: w needs base and n_base for its partials");
   if (!a->x || !a->ids || !a->y || !a->low || (a->adapters > 0 && (!a->a || !a->b || !a->ranks || !a->scales)) ||
       (a->n_base > 0 && !a->base))
@@ -178,6 +188,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
       !aligned16(a->order) || !aligned16(a->y) || a->x_row_stride % 8 || a->base_part_stride % 4 || a->base_row_stride % 4 ||
       a->y_row_stride % (a->y_dtype == DSV2_F32 ? 4 : 8))
     return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
+  if (!aligned16(a->xs) || !aligned16(a->lists)) return fail(DSV2_ERR_INVALID, "lora: xs and lists must be 16-byte aligned");
   int sms = 0;
   if (int rc = ensure_init(&sms)) return rc;
   const bool few = a->w && a->tokens <= kLoraGemvTokens && a->n_base == 1;
@@ -234,7 +245,6 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
     p.base_parts = 0;
   }
   if (!fused) return check_launch(launch_lora(p, sms, st), "lora");
-  if (!aligned16(a->xs) || !aligned16(a->lists)) return fail(DSV2_ERR_INVALID, "lora: xs and lists must be 16-byte aligned");
   p.xs = static_cast<bf16*>(a->xs);
   p.lists = a->lists;
   p.base_parts = 0;
@@ -242,7 +252,7 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
   const uint64_t T = static_cast<uint64_t>(a->tokens), N = static_cast<uint64_t>(a->n), K = static_cast<uint64_t>(a->k);
   const uint64_t ws = static_cast<uint64_t>(a->w_row_stride) * 2;
   CUtensorMap tm_x, tm_w;
-  if (int rc = tensor_map_3d(a->xs, K, T, 1, lg_row(a->k, a->rank) * 2, T * lg_row(a->k, a->rank) * 2, kLgRows, &tm_x)) return rc;
+  if (int rc = tensor_map_3d(a->xs, K, T, 1, K * 2, T * K * 2, kLgRows, &tm_x)) return rc;
   if (int rc = tensor_map_3d(a->w, K, N, 1, ws, N * ws, static_cast<uint32_t>(n_tile / 2), &tm_w)) return rc;
   if (int rc = check_launch(launch_lora_rows(p, sms, st), "lora: rows")) return rc;
   return check_launch(launch_lora_gemm(p, tm_x, tm_w, n_tile, sms, st), "lora: gemm");

@@ -137,10 +137,6 @@ constexpr int kLgPiece = 16;          // ranks of a piece, the k of one tcgen05.
 __host__ __device__ constexpr long long lg_list_ints(int rank) {
   return 2 + 2LL * kLgM * ((rank + kLgPiece - 1) / kLgPiece);
 }
-// elements of a row of xs, x and then low as bf16 (of a token without an adapter: nothing): whole
-// 128-byte lines, which is what the GEMM's copies take
-__host__ __device__ constexpr long long lg_row(int k, int rank) { return k + (rank + 63LL) / 64 * 64; }
-
 // The pieces of a tile, by one warp.
 __device__ __forceinline__ void lora_list_pieces(const LoraParams& p, int tile) {
   const int lane = threadIdx.x & 31;
@@ -198,12 +194,13 @@ __device__ __forceinline__ float ld_cluster_f32(const float* local, uint32_t ran
 }
 
 // low partials of one tile and k split: low[split, t, j].  NT = rank / 8 n-tiles of 8 ranks.  For the
-// GEMM of lora_gemm.cu (kSorted) the tile's rows of xs instead: x and the whole low as bf16, and the
+// GEMM of lora_gemm.cu (kSorted) the tile's rows of xs and the whole low, both in adapter order, and the
 // pieces of each tile of that GEMM: one pass over x where a low of its own and a gather take two
-// (4001 tokens, k 2048, rank 32: 16 us for both, 16 + 10 us apart).  The k splits are then the CTAs of
+// (4001 tokens, k 2048, rank 32: 16 us for both, 16 + 10 us apart).  (Two CTAs an SM: at rank 64 the compiler
+// otherwise keeps fewer loads under way, 3800 tokens 53 us against 31.)  The k splits are then the CTAs of
 // a cluster, which sum through each other's shared memory.
 template <int NT, int kWarps, bool kSorted>
-__global__ __launch_bounds__(kWarps * 32) void lora_low_kernel(const LoraParams p) {
+__global__ __launch_bounds__(kWarps * 32, kSorted && NT == 8 ? 2 : 0) void lora_low_kernel(const LoraParams p) {
   pdl_enter();
   __shared__ LoraTile s;
   __shared__ float s_sum[kWarps][kLoraTile][8 * NT + 4];
@@ -213,7 +210,7 @@ __global__ __launch_bounds__(kWarps * 32) void lora_low_kernel(const LoraParams 
     if (blockIdx.x % (kLgM / kLoraTile) == 0 && blockIdx.y == 0 && warp == kWarps - 1) lora_list_pieces(p, blockIdx.x / (kLgM / kLoraTile));
     for (int r = blockIdx.y * kWarps + warp; r < kLoraTile && s.tok[r] >= 0; r += gridDim.y * kWarps) {
       const uint4* src = reinterpret_cast<const uint4*>(p.x + s.tok[r] * p.x_row_stride);
-      uint4* dst = reinterpret_cast<uint4*>(p.xs + (blockIdx.x * kLoraTile + r) * lg_row(p.k, p.rank));
+      uint4* dst = reinterpret_cast<uint4*>(p.xs + (blockIdx.x * kLoraTile + r) * static_cast<long long>(p.k));
 #pragma unroll 8
       for (int j = lane; j < p.k / 8; j += 32) dst[j] = __ldg(src + j);
     }
@@ -283,8 +280,8 @@ __global__ __launch_bounds__(kWarps * 32) void lora_low_kernel(const LoraParams 
       }
       // columns past the adapter's rank hold whatever its padding holds
       v = j < rank ? v * scale : 0.f;
-      if (kSorted) p.xs[(blockIdx.x * kLoraTile + r) * lg_row(p.k, p.rank) + p.k + j] = __float2bfloat16(v);
-      else p.low[(static_cast<long long>(blockIdx.y) * p.tokens + s.tok[r]) * p.rank + j] = v;
+      const long long row = kSorted ? blockIdx.x * kLoraTile + r : static_cast<long long>(blockIdx.y) * p.tokens + s.tok[r];
+      p.low[row * p.rank + j] = v;
     }
   }
   if (kSorted && gridDim.y > 1) sync();   // nobody reads this CTA's sums any more

@@ -1,13 +1,16 @@
 // Shared projection and adapters of a long run of tokens (a prompt chunk) in one tcgen05 GEMM:
 //   y[order[i], n] = bf16( sum_k xs[i, k] W[n, k] + sum_a sum_j L_a[i, j] B_a[n, j] )
 // over tokens in adapter order (lora_sort_kernel): xs = the rows of x in that order, and
-// L_a[i, j] = low[order[i], j] where token i has adapter a, else 0.  A tile of 256 tokens holds few
-// adapters, so their products are a few more steps of 64 k on the same accumulator (two or three
-// against 32 at k = 2048 with five adapters of rank 32), and neither the projection's fp32 sums nor
+// L_a[i, j] = low[i, j] (fp32, in that order) where token i has adapter a, else 0.  A tile of 256 tokens holds few
+// adapters, so their products are a few more steps of 64 k on the same accumulator (five against
+// 32 at k = 2048 with five adapters of rank 32 in a tile), and neither the projection's fp32 sums nor
 // the adapters' part ever reach memory: with separate launches those are 8 bytes written and read
-// per output element.  The adapters' ranks are cut into pieces of 16, four to a step whatever
+// per output element.  The adapters' ranks are cut into pieces of 16, two to a step whatever
 // adapters they belong to, and the steps stand evenly among the projection's: each is loaded while
 // the ones before it are multiplied.
+// low enters as the sum of two bf16 numbers (columns of their own against the same B), as in
+// lora_out_kernel: 2^-16 of it is lost.  As one number it would lose 2^-8 of sum_j |low_j B_j|, far more than y's
+// own rounding where terms cancel, and a token's precision would depend on how many share its call.
 //
 // A pair of SMs has a tile of 256 tokens x n_tile columns (tcgen05.mma on cta_group::2): each holds the
 // operands and accumulators of 128 of the tokens and the operand of half of the columns, so that an SM
@@ -15,18 +18,18 @@
 // n_tile (all of the call 73 us, single SMs 75 us).  The issuing lanes are chosen by elect.sync: chosen
 // by their number, each tcgen05.mma took some 200 clocks to issue and the GEMM 65 us instead of 46.
 // Both operands K-major with the 128-byte swizzle, accumulators fp32 in TMEM, two of them.
-// Persistent, one CTA per SM, 14 warps:
+// Persistent, one CTA per SM, 22 warps:
 //  - warp 0 (one lane): TMA of this CTA's projection operands into a ring of 6 stages;
 //  - warp 1 (one lane, of the pair's first CTA): tcgen05.mma for both;
 //  - warps 2-5: accumulators to bf16 rows of y, while the next tile is multiplied;
-//  - warps 6-13, in two groups that take the adapters' steps in turn: their operands, from global
+//  - warps 6-21, in four groups that take the adapters' steps in turn: their operands, from global
 //    memory through registers into ring stages; the loads are on their way before the stage is free.
-//    (One group: 1024 tokens with 64 adapters 45 us, two: 41.)  A plain copy will not do: what an adapter's
+//    (2 / 3 / 4 groups: 768 tokens with 64 adapters 47 / 44 / 40 us, 4001 with 6 71.4 / 72.0 / 72.2.  Rows of low and
+//    B shared out over neighbouring lanes were slower: 52 / 49 / 47.)  A plain copy will not do: what an adapter's
 //    padding past its rank holds must not be multiplied, nor may an infinity or a NaN of one adapter
 //    meet the zeros that other adapters' tokens have in its columns.  Such values, and those of low, which would
 //    meet the zeros that stand for them, enter as zeros, and the epilogue adds their products to the rows of
 //    their own adapter.
-// low enters as bf16: its rounding (2^-9 of the adapters' part) is below that of y.
 // 4001 tokens, 6 adapters of rank 32, 2048 -> 3648: about 46 of the 71 us that the order, the rows and
 // this take together; 1.3 PFLOP/s.  Bound by the multiplications with what the last tiles leave idle:
 // 16 x 17 tiles are 3.7 rounds of 74 pairs.
@@ -36,21 +39,22 @@ namespace dsv2 {
 
 constexpr int kLgK = 64;              // k of a ring stage
 constexpr int kLgStages = 6;
+constexpr int kLgStepPieces = kLgK / (2 * kLgPiece);   // pieces of an adapters' step, each with both parts of low
 constexpr int kLgABytes = kLgRows * kLgK * 2;
 constexpr int kLgMaxN = 256;
 constexpr int kLgStageBytes = kLgABytes + kLgMaxN / 2 * kLgK * 2;
 constexpr int kLgLoaders = 128;       // threads of a group that brings in the adapters' operands
-constexpr int kLgGroups = 2;
+constexpr int kLgGroups = 4;
 constexpr int kLgThreads = 6 * 32 + kLgGroups * kLgLoaders;
-constexpr size_t kLgSmem = kLgStages * kLgStageBytes + 1024 + 256;
+constexpr size_t kLgSmem = kLgStages * kLgStageBytes + 1024 + 512;
 static_assert(kLgSmem <= 232448, "adapter GEMM: shared memory exceeds 227 KB");
 
-// The steps of an item: nkb of the projection and extra = ceil(pieces / 4) of the adapters, of which
+// The steps of an item: nkb of the projection and extra = ceil(pieces / 2) of the adapters, of which
 // number e comes after (e + 1) nkb / (extra + 1) of the projection's.
 struct LgSteps {
   int nkb, extra, kb, e, next;
   __device__ __forceinline__ LgSteps(int nkb_, int pieces)
-      : nkb(nkb_), extra((pieces + kLgK / kLgPiece - 1) / (kLgK / kLgPiece)), kb(0), e(0), next(before(0)) {}
+      : nkb(nkb_), extra((pieces + kLgStepPieces - 1) / kLgStepPieces), kb(0), e(0), next(before(0)) {}
   __device__ __forceinline__ int before(int i) const { return static_cast<unsigned>((i + 1) * nkb) / static_cast<unsigned>(extra + 1); }
   __device__ __forceinline__ bool more() const { return kb < nkb || e < extra; }
   __device__ __forceinline__ bool adapters() const { return kb >= next && e < extra; }   // of the next step
@@ -221,13 +225,17 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
           }
           tc_fence_after();
           const bool ad = q.adapters();
-          const int k16 = ad ? min(pieces - q.e * (kLgK / kLgPiece), kLgK / kLgPiece) : kLgK / kLgPiece;
+          const int k16 = ad ? 2 * min(pieces - q.e * kLgStepPieces, kLgStepPieces) : kLgK / kLgPiece;
           unsigned char* st = smem + stage * kLgStageBytes;
           const uint64_t da = sw128_kmajor_desc(smem_u32(st)), db = sw128_kmajor_desc(smem_u32(st + kLgABytes));
+          // adapters: columns 0-15 and 16-31 of A are a piece's high and low parts, both against columns 0-15 of B
+          const int b1 = ad ? 0 : 2, b2 = ad ? 2 : 4, b3 = ad ? 2 : 6;
           lg_mma(dacc, da, db, idesc, first ? 0u : 1u);
-          if (k16 > 1) lg_mma(dacc, da + 2, db + 2, idesc, 1);
-          if (k16 > 2) lg_mma(dacc, da + 4, db + 4, idesc, 1);
-          if (k16 > 3) lg_mma(dacc, da + 6, db + 6, idesc, 1);
+          lg_mma(dacc, da + 2, db + b1, idesc, 1);
+          if (k16 > 2) {
+            lg_mma(dacc, da + 4, db + b2, idesc, 1);
+            lg_mma(dacc, da + 6, db + b3, idesc, 1);
+          }
           first = false;
           lg_commit(&empty_bar[stage]);
           if (++stage == kLgStages) {
@@ -283,12 +291,12 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
       if (*odd_flag && live && p.order[p.tokens + pos] >= 0) {
         // the products that were left out, into this thread's own elements of y (rare: any speed will do)
         const int a = p.order[p.tokens + pos], rank = p.order[2 * p.tokens + pos];
-        const bf16* low = p.xs + pos * lg_row(p.k, p.rank) + p.k;
+        const float* low = p.low + static_cast<long long>(pos) * p.rank;
         const bf16* b = p.b + (static_cast<long long>(a) * p.n + nt * n_tile) * p.rank;
         for (int c = 0; c < cols; ++c, b += p.rank)
           for (int j = 0; j < rank; ++j) {
-            const float w = __bfloat162float(b[j]), l = __bfloat162float(low[j]);
-            if (isfinite(w) && isfinite(l)) continue;
+            const float w = __bfloat162float(b[j]), l = low[j];
+            if (isfinite(w) && isfinite(__bfloat162float(__float2bfloat16(l)))) continue;
             y[c] = __float2bfloat16(__bfloat162float(y[c]) + l * w);
           }
       }
@@ -304,7 +312,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
       const int mt = it % m_tiles, nt = it / m_tiles;
       const int pos = mt * kLgM + half * kLgRows + t;
       const int mine = pos < p.tokens ? p.order[p.tokens + pos] : -1;
-      const bf16* low = p.xs + min(pos, p.tokens - 1) * lg_row(p.k, p.rank) + p.k;
+      const float* low = p.low + static_cast<long long>(min(pos, p.tokens - 1)) * p.rank;
       const int* list = list_of(mt);
       const int n = nt * n_tile + half * n_half + t;
       const bool in = t < n_half && n < p.n;
@@ -317,25 +325,27 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
         done = at + 1;
         const int st_i = stage;
         stage = (stage + 1) % kLgStages;
-        if (q.e % kLgGroups != group) continue;   // the other group's
+        if (q.e % kLgGroups != group) continue;   // another group's
         const uint32_t parity = (go_phase >> st_i) & 1;
         go_phase ^= 1u << st_i;
-        uint4 ra[8], rb[8];
-        int2 u[4];   // this step's pieces; none: no ranks
+        constexpr int kChunks = 2 * kLgStepPieces;   // of 8 ranks
+        uint4 ra[kChunks], rl[kChunks], rb[kChunks];   // low's two parts (at first its 8 fp32 numbers), B
+        int2 u[kLgStepPieces];   // this step's pieces; none: no ranks
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int piece = q.e * (kLgK / kLgPiece) + g;
+        for (int g = 0; g < kLgStepPieces; ++g) {
+          const int piece = q.e * kLgStepPieces + g;
           u[g] = piece < pieces ? __ldg(reinterpret_cast<const int2*>(list + 2 + 2 * piece)) : make_int2(0, 0);
         }
         // no branches here: all of a step's loads are under way together
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           const int a = u[c >> 1].x, j = (u[c >> 1].y & 0xffff) + 8 * (c & 1), left = (u[c >> 1].y >> 16) - 8 * (c & 1);
           ra[c] = ld_or_zero(low + j, mine == a && left > 0);
+          rl[c] = ld_or_zero(low + j + 4, mine == a && left > 0);
           rb[c] = ld_or_zero(p.b + (static_cast<long long>(a) * p.n + n) * p.rank + j, in && left > 0);
         }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           const int left = (u[c >> 1].y >> 16) - 8 * (c & 1);
           if (left <= 0 || left >= 8) continue;
           // padding past the rank may be anything, and 0 * NaN is not 0
@@ -347,17 +357,32 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kLgThreads, 1) void lora_
         }
         bool odd = false;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          odd |= drop_nonfinite(ra[c]);
+        for (int c = 0; c < kChunks; ++c) {
           odd |= drop_nonfinite(rb[c]);
+          const uint32_t w[8] = {ra[c].x, ra[c].y, ra[c].z, ra[c].w, rl[c].x, rl[c].y, rl[c].z, rl[c].w};
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v0 = __uint_as_float(w[2 * i]), v1 = __uint_as_float(w[2 * i + 1]);
+            hi[i] = pack_bf16x2(v0, v1);
+            lo[i] = pack_bf16x2(v0 - bf16lo(hi[i]), v1 - bf16hi(hi[i]));
+          }
+          ra[c] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          rl[c] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (drop_nonfinite(ra[c])) {   // (what is left of an infinity or a NaN is not finite either)
+            drop_nonfinite(rl[c]);
+            odd = true;
+          }
         }
         if (odd)
           for (uint32_t r = 0; r < 2; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(const_cast<int*>(odd_flag), r)), "r"(1) : "memory");
         if (mbar_wait(&go_bar[group * kLgStages + st_i], parity)) {
           unsigned char* st = smem + st_i * kLgStageBytes;
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            *reinterpret_cast<uint4*>(st + swz(t, c)) = ra[c];
+          for (int c = 0; c < kChunks; ++c) {
+            const int at = 4 * (c >> 1) + (c & 1);
+            *reinterpret_cast<uint4*>(st + swz(t, at)) = ra[c];
+            *reinterpret_cast<uint4*>(st + swz(t, at + 2)) = rl[c];
             if (t < n_half) *reinterpret_cast<uint4*>(st + kLgABytes + swz(t, c)) = rb[c];
           }
           fence_proxy_async_smem();

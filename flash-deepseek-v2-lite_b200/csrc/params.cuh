@@ -172,7 +172,7 @@ struct LoraParams {
   const float* scales;         // [adapters]
   int adapters, rank, tokens, k, n;
   int ids_len;
-  float* low;                  // [low_parts, tokens, rank] work buffer
+  float* low;                  // [low_parts, tokens, rank] work buffer (long runs: the first part, in adapter order)
   int low_parts;               // k splits of the first product
   int* order;                  // [3, tokens] work buffer: tokens by adapter, adapters, ranks (nullptr: as they come)
   const float* base;           // optional fp32 partials of the shared projection, summed in order
@@ -183,7 +183,7 @@ struct LoraParams {
   long long y_row_stride;
   const bf16* w;               // few tokens: the shared projection's weights, [n, k] (else null)
   long long w_row_stride;
-  bf16* xs;                    // long runs of tokens: [tokens, k + rank rounded up to 64] work buffer, x and low in adapter order
+  bf16* xs;                    // long runs of tokens: [tokens, k] work buffer, x in adapter order
   int* lists;                  // [ceil(tokens / 256), 2 + 512 ceil(rank / 16)] work buffer, adapters of each token tile
 };
 

@@ -750,14 +750,14 @@ def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor
 
 
 def _lora_gemm_buffers(tokens: int, k: int, rank: int) -> tuple:
-    return (tokens, k + (rank + 63) // 64 * 64), ((tokens + 255) // 256, 2 + 512 * ((rank + 15) // 16))
+    return (tokens, k), ((tokens + 255) // 256, 2 + 512 * ((rank + 15) // 16))
 
 
 def lora_workspace(tokens: int, n: int, k: int, rank: int, device) -> dict:
     """Work buffers of lora_linear: the low-rank rows, the tokens' order by adapter, the shared
     projection's fp32 partials and, above 256 tokens, the activations in that order with the
     adapters of each tile of tokens (xs, lists: the projection and the adapters are then one
-    GEMM if there are at least 12 tokens per adapter)."""
+    GEMM if y is bf16 and the ranks that 256 tokens use are few beside k)."""
     sms = torch.cuda.get_device_properties(device).multi_processor_count
     splits = 1
     # decode batches: K split over the SMs, as the engine's projections (1 / 5 pieces: 64 tokens 24 / 18 us,

@@ -685,9 +685,10 @@ DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* strea
  * DSV2_F32 (with n_base = 0 the adapters' part alone, e.g. one more partial of the projection).
  * low: fp32 work buffer [low_parts, tokens, rank] (low_parts >= 1 pieces of k run side by side);
  * order: int32 work buffer [3 * tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128.
- * xs, lists: work buffers, may be NULL: bf16 [tokens, k + rank rounded up to 64] and int32
- * [ceil(tokens / 256), 2 + 512 * ceil(rank / 16)].  With them and w, a long run of tokens (more than 256
- * and at least 12 per adapter, bf16 y, k % 64 == 0) is one GEMM over the tokens in adapter order. */
+ * xs, lists: work buffers, may be NULL: bf16 [tokens, k] and int32
+ * [ceil(tokens / 256), 2 + 512 * ceil(rank / 16)].  With them and w, a long run of tokens (more than 256,
+ * bf16 y, k % 64 == 0, the ranks that 256 of them use few beside k) is one GEMM over the tokens in adapter
+ * order.  A_a x enters the second product with 16 significant bits or more, whatever the number of tokens. */
 typedef struct dsv2_lora_args {
   const void* x;
   int64_t x_row_stride;

@@ -28,6 +28,17 @@ def no_device_error():
 
 
 # ------------------------------------------------------------------ adapters
+# Bounds, from the roundings of each path: low is an fp32 sum; up to 16 tokens of lora_linear it is used as it is,
+# elsewhere as the sum of two bf16 numbers, each within 2^-8 of what it stands for: 2^-16 of low is lost.  The
+# fp32 sums of the K products of W x and of low are off by at most (K + 512) 2^-24 of the sum of their
+# magnitudes, the sum over the ranks (two products each, truncated) by (2 rank + 64) 2^-23, and the result's own
+# rounding is 2^-8 (bf16) or 2^-24 (fp32) of it.
+def lora_tol(c, y, low, mag, split, f32):
+    k, rank = c["x"].shape[1] + 512, c["a"].shape[1]
+    return ((2.0 ** -24 if f32 else 2.0 ** -8) * y.abs() + (2.0 ** -16 if split else 0.0) * low * (1 + 2.0 ** -7) +
+            (2 * rank + 64) * 2.0 ** -23 * low + k * 2.0 ** -24 * mag + 1e-30)
+
+
 def lora_case(T, n_ad, rank, K, N, seed, cancel=False):
     g = torch.Generator().manual_seed(seed)
 
@@ -54,6 +65,47 @@ def lora_case(T, n_ad, rank, K, N, seed, cancel=False):
     return c
 
 
+def lora_want(c, w=True, cancel=False):
+    """(y, sum |low B|, the magnitudes of the sums over k that are not exact)."""
+    ids = c["ids"].tolist()
+    y, low, mag = S.lora(c["x"], c["w"] if w else None, c["a"], c["b"], ids, c["ranks"], c["scales"])
+    if cancel:
+        b = c["b"].clone()
+        b[:, :, :2] = 0
+        mag = S.lora(c["x"], c["w"] if w else None, c["a"], b, ids, c["ranks"], c["scales"])[2]
+    return y, low, mag
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("cancel", [False, True])
+@pytest.mark.parametrize("T,n_ad,rank,K,N", [
+    (1, 2, 8, 2048, 256), (5, 3, 48, 256, 72), (8, 2, 128, 192, 136), (16, 5, 96, 320, 200), (13, 4, 64, 1024, 264),
+    (3, 2, 16, 72, 40), (16, 3, 72, 584, 48), (17, 3, 16, 256, 200), (64, 20, 40, 2048, 264), (200, 9, 64, 512, 328),
+    (257, 3, 16, 2048, 264), (400, 5, 40, 256, 520), (700, 30, 128, 192, 136), (300, 40, 24, 128, 72),
+    (1030, 8, 128, 512, 264), (900, 12, 128, 2048, 136)])
+def test_lora_linear_keeps_the_adapters_precision(D, T, n_ad, rank, K, N, cancel, f32):
+    c = lora_case(T, n_ad, rank, K, N, seed=T + rank, cancel=cancel)
+    y = torch.full((T, N), math.nan, dtype=torch.float32 if f32 else torch.bfloat16, device=DEV)
+    D.lora_linear(**{k: v.to(DEV) for k, v in c.items()}, y=y, **D.lora_workspace(T, N, K, rank, DEV))
+    want, low, mag = lora_want(c, cancel=cancel)
+    bad = (y.cpu().double() - want).abs() / lora_tol(c, want, low, mag, split=T > 16, f32=f32)
+    assert not bool(y.isnan().any()) and float(bad.max()) <= 1, float(bad.max())
+
+
+@pytest.mark.parametrize("T,n_ad,rank,K,N", [(1, 2, 16, 72, 40), (9, 3, 128, 1096, 136), (40, 7, 56, 264, 328), (600, 12, 32, 520, 200)])
+def test_lora_alone_keeps_precision_at_any_k(D, T, n_ad, rank, K, N):
+    c = lora_case(T, n_ad, rank, K, N, seed=K)
+    g = torch.Generator().manual_seed(1)
+    base = torch.randn(3, T, N, generator=g)
+    y = torch.empty(T, N, device=DEV)
+    ws = D.lora_workspace(T, N, K, rank, DEV)
+    D.lora(**{k: v.to(DEV) for k, v in c.items() if k != "w"}, y=y, base=base.to(DEV), low=ws["low"], order=ws["order"])
+    want, low, mag = lora_want(c, w=False)
+    want, mag = want + base.double().sum(0), mag + base.double().abs().sum(0)
+    bad = (y.cpu().double() - want).abs() / lora_tol(c, want, low, mag, split=True, f32=True)
+    assert float(bad.max()) <= 1, float(bad.max())
+
+
 @pytest.mark.parametrize("T", [6, 40, 300])
 def test_lora_infinities_on_both_sides(D, T):
     """An infinite low-rank activation that meets an infinity of B is an infinity (or, of opposite
@@ -71,13 +123,15 @@ def test_lora_infinities_on_both_sides(D, T):
     c["b"][1, 13, 3] = -0.5
     y = torch.empty(T, N, dtype=torch.bfloat16, device=DEV)
     D.lora_linear(**{k: v.to(DEV) for k, v in c.items()}, y=y, **D.lora_workspace(T, N, K, rank, DEV))
-    want = S.lora(c["x"], c["w"], c["a"], c["b"], c["ids"].tolist(), c["ranks"], c["scales"])[0]
+    want, low, mag = lora_want(c)
     y = y.cpu().double()
     own = c["ids"] == 1
     sane = want.isfinite()
     assert torch.equal(y.isnan(), want.isnan())
     assert torch.equal(y[~sane & ~want.isnan()], want[~sane & ~want.isnan()])
     assert bool((~sane)[own].any()) and bool(sane[~own].all())
+    tol = lora_tol(c, want, low, mag, split=T > 16, f32=False)
+    assert float(((y - want).abs() / tol)[sane].max()) <= 1
 
 
 # ------------------------------------------------------------------ attention
