@@ -189,9 +189,12 @@ int dsv2_lora(const dsv2_lora_args* a, void* stream) {
       a->y_row_stride % (a->y_dtype == DSV2_F32 ? 4 : 8))
     return fail(DSV2_ERR_INVALID, "lora: operands must be 16-byte aligned rows");
   if (!aligned16(a->xs) || !aligned16(a->lists)) return fail(DSV2_ERR_INVALID, "lora: xs and lists must be 16-byte aligned");
+  const bool few = a->w && a->tokens <= kLoraGemvTokens && a->n_base == 1;
+  if (a->w && !few && a->k % 64)   // dsv2_linear's condition, told before anything is launched
+    return fail(DSV2_ERR_UNSUPPORTED, "lora: k %d: with w and more than %d tokens or pieces of k, a multiple of 64", a->k,
+                kLoraGemvTokens);
   int sms = 0;
   if (int rc = ensure_init(&sms)) return rc;
-  const bool few = a->w && a->tokens <= kLoraGemvTokens && a->n_base == 1;
   if ((few || fused) && (!aligned16(a->w) || a->w_row_stride % 8 || a->w_row_stride < a->k))
     return fail(DSV2_ERR_INVALID, "lora: w must be 16-byte aligned rows");
   if (a->w && !fused && !few) {

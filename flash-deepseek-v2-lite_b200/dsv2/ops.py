@@ -792,7 +792,7 @@ def lora_linear(*, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
                 token_row: torch.Tensor | None = None) -> torch.Tensor:
     """The shared projection x @ w.T (w bf16 [N, K]) plus every token's low-rank adapter, rounded
     once to y's dtype: y[t] = w x[t] + scales[i] * b[i] (a[i] x[t]); see lora and
-    lora_workspace."""
+    lora_workspace.  K is a multiple of 8 (above 16 tokens of 64)."""
     if w.dim() != 2 or w.dtype != torch.bfloat16 or w.stride(1) != 1 or not w.is_cuda:
         raise NotImplementedError("lora_linear supports a CUDA bf16 w [N, K] with contiguous rows")
     if w.shape[1] != x.shape[-1] or w.shape[0] != y.shape[-1]:

@@ -684,7 +684,8 @@ DSV2_API int dsv2_mla_decode_q4(const dsv2_mla_decode_q4_args* args, void* strea
  * with DSV2_EPI_STORE_F32).  y: y_dtype DSV2_BF16 (one rounding of the fp32 sum) or
  * DSV2_F32 (with n_base = 0 the adapters' part alone, e.g. one more partial of the projection).
  * low: fp32 work buffer [low_parts, tokens, rank] (low_parts >= 1 pieces of k run side by side);
- * order: int32 work buffer [3 * tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128.
+ * order: int32 work buffer [3 * tokens], may be NULL up to 16 tokens.  k % 8 == 0, n % 8 == 0, rank % 8 == 0, rank <= 128;
+ * with w and either more than 16 tokens or n_base > 1, k % 64 == 0 (DSV2_ERR_UNSUPPORTED otherwise).
  * xs, lists: work buffers, may be NULL: bf16 [tokens, k] and int32
  * [ceil(tokens / 256), 2 + 512 * ceil(rank / 16)].  With them and w, a long run of tokens (more than 256,
  * bf16 y, k % 64 == 0, the ranks that 256 of them use few beside k) is one GEMM over the tokens in adapter
