@@ -287,8 +287,9 @@ def lm_head_argmax(*, w: torch.Tensor, x: torch.Tensor, keys: torch.Tensor, next
         return
     if missed is None:
         raise ValueError("lm_head_argmax: served needs missed, which counts the other rows")
-    _lib.call("dsv2_lm_head_argmax_served", *args, _need(served, "served", torch.int64, n),
-              _need(missed, "missed", torch.int32, 1), family, stream())
+    dev = x.get_device()
+    _lib.call("dsv2_lm_head_argmax_served", *args, _need(served, "served", torch.int64, dev, n),
+              _need(missed, "missed", torch.int32, dev, 1), family, stream())
 
 
 def router(*, x: torch.Tensor, w: torch.Tensor, scaling: float, logits: torch.Tensor,
@@ -543,12 +544,17 @@ L4_BLOCK_TOKENS = 16     # tokens of a block of the 4-bit latent cache
 L4_BLOCK_BYTES = 6400    # its bytes (include/dsv2.h describes them)
 
 
-def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int | None = None) -> int:
-    """Address of a contiguous CUDA tensor of this dtype (and at least numel elements) on the
-    current device."""
-    if not (t.is_cuda and t.dtype is dtype and t.is_contiguous()):
-        if not t.is_cuda:
-            raise NotImplementedError(f"{name} must be a CUDA tensor")
+def _on(t: torch.Tensor, name: str, dev: int) -> None:
+    """t is a CUDA tensor of GPU dev."""
+    if t.get_device() != dev:
+        _cuda(t, name)
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{dev}")
+
+
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, numel: int | None = None) -> int:
+    """Address of a contiguous tensor of this dtype (and at least numel elements) on GPU dev."""
+    if not (t.get_device() == dev and t.dtype is dtype and t.is_contiguous()):
+        _on(t, name, dev)
         if t.dtype is not dtype:
             raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
         raise NotImplementedError(f"{name} must be contiguous")
@@ -557,11 +563,10 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int | None = No
     return t.data_ptr()
 
 
-def _here(t: torch.Tensor) -> int:
-    """The current stream, of the device that t lives on."""
-    dev = t.get_device()
+def _here(dev: int) -> int:
+    """The current stream, of the GPU that a call's tensors live on."""
     if dev != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        raise ValueError(f"tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
@@ -575,9 +580,9 @@ def latent4_cache(pages: int, page_size: int, device, layers: int | None = None)
     return torch.zeros(shape if layers is None else (layers, *shape), device=device, dtype=torch.uint8)
 
 
-def _l4_blocks(cache: torch.Tensor) -> tuple[int, int]:
-    """(address, 16-token blocks) of a 4-bit latent cache."""
-    ptr = _need(cache, "cache", torch.uint8)
+def _l4_blocks(cache: torch.Tensor, dev: int) -> tuple[int, int]:
+    """(address, 16-token blocks) of a 4-bit latent cache on GPU dev."""
+    ptr = _need(cache, "cache", torch.uint8, dev)
     n, rem = divmod(cache.numel(), L4_BLOCK_BYTES)
     if rem or not n:
         raise ValueError(f"the 4-bit cache must hold whole blocks of {L4_BLOCK_BYTES} bytes")
@@ -613,17 +618,17 @@ def page_plan(*, cached: torch.Tensor, new: torch.Tensor, block_table: torch.Ten
         raise ValueError("cached must be int32 or int64")
     if cached.numel() != R or new.numel() != R:
         raise ValueError(f"block_table has {R} rows, cached {cached.numel()} and new {new.numel()} entries")
-    cap = token_row.numel()
+    cap, dev = token_row.numel(), block_table.get_device()
     a = PagePlanArgs(
-        _need(cached, "cached", cached.dtype), _need(new, "new", torch.int32), block_table.data_ptr(),
-        _need(free_ring, "free_ring", torch.int32), _need(ring_in, "ring_in", torch.int64, 2),
-        _need(ring_out, "ring_out", torch.int64, 2), _need(token_row, "token_row", torch.int32),
-        _need(positions, "positions", torch.int64, cap), _need(slots, "slots", torch.int64, cap),
-        _need(cu_new, "cu_new", torch.int32, R + 1), _need(lens, "lens", torch.int32, R),
-        _need(counts, "counts", torch.int32, 4), _need(sync, "sync", torch.int32, 1),
+        _need(cached, "cached", cached.dtype, dev), _need(new, "new", torch.int32, dev), block_table.data_ptr(),
+        _need(free_ring, "free_ring", torch.int32, dev), _need(ring_in, "ring_in", torch.int64, dev, 2),
+        _need(ring_out, "ring_out", torch.int64, dev, 2), _need(token_row, "token_row", torch.int32, dev),
+        _need(positions, "positions", torch.int64, dev, cap), _need(slots, "slots", torch.int64, dev, cap),
+        _need(cu_new, "cu_new", torch.int32, dev, R + 1), _need(lens, "lens", torch.int32, dev, R),
+        _need(counts, "counts", torch.int32, dev, 4), _need(sync, "sync", torch.int32, dev, 1),
         block_table.stride(0) if R > 1 else max(width, 1), free_ring.numel(), R, width, page_size, cap,
         cached.dtype == torch.int64)
-    _lib.call("dsv2_page_plan", ctypes.byref(a), _here(block_table))
+    _lib.call("dsv2_page_plan", ctypes.byref(a), _here(dev))
 
 
 def _l4_rows(rows: torch.Tensor, slots: torch.Tensor, name: str) -> int:
@@ -638,18 +643,18 @@ def _l4_rows(rows: torch.Tensor, slots: torch.Tensor, name: str) -> int:
 def latent4_write(*, rows: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor) -> None:
     """Quantise bf16 latent rows [n, 576] into their slots (int64 [n], negative = skipped) of a
     4-bit latent cache."""
-    rs = _l4_rows(rows, slots, "rows")
-    ptr, blocks = _l4_blocks(cache)
-    _lib.call("dsv2_latent4_write", rows.data_ptr(), rs, _need(slots, "slots", torch.int64), rows.shape[0], ptr, blocks,
-              _here(rows))
+    rs, dev = _l4_rows(rows, slots, "rows"), rows.get_device()
+    ptr, blocks = _l4_blocks(cache, dev)
+    _lib.call("dsv2_latent4_write", rows.data_ptr(), rs, _need(slots, "slots", torch.int64, dev), rows.shape[0], ptr, blocks,
+              _here(dev))
 
 
 def latent4_read(*, cache: torch.Tensor, slots: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """The values that the slots hold (zeros for a negative slot) as bf16 rows [n, 576]."""
-    rs = _l4_rows(out, slots, "out")
-    ptr, blocks = _l4_blocks(cache)
-    _lib.call("dsv2_latent4_read", ptr, blocks, _need(slots, "slots", torch.int64), out.shape[0], out.data_ptr(), rs,
-              _here(out))
+    rs, dev = _l4_rows(out, slots, "out"), out.get_device()
+    ptr, blocks = _l4_blocks(cache, dev)
+    _lib.call("dsv2_latent4_read", ptr, blocks, _need(slots, "slots", torch.int64, dev), out.shape[0], out.data_ptr(), rs,
+              _here(dev))
     return out
 
 
@@ -659,8 +664,9 @@ def mla_prep_q4(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos:
     """mla_prep into slots (int64 [B], negative = no cache write) of a 4-bit latent cache; a
     negative position marks a padding row."""
     a = _mla_prep_args(qkva, kv_norm_w, eps, cos, sin, positions, q_pe_out, q_nope_out)
-    ptr, blocks = _l4_blocks(cache)
-    _lib.call("dsv2_mla_prep_q4", ctypes.byref(a), ptr, blocks, _need(slots, "slots", torch.int64, a.batch), _here(cache))
+    dev = qkva.get_device()
+    ptr, blocks = _l4_blocks(cache, dev)
+    _lib.call("dsv2_mla_prep_q4", ctypes.byref(a), ptr, blocks, _need(slots, "slots", torch.int64, dev, a.batch), _here(dev))
 
 
 def mla_q4_workspace(rows: int, device) -> dict:
@@ -687,17 +693,19 @@ def mla_decode_q4(*, q_abs: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tenso
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
         raise NotImplementedError("block_table must be int32 [sequences, width] with contiguous rows")
     _cuda(block_table, "block_table")
-    ptr, blocks = _l4_blocks(cache)
+    dev = block_table.get_device()
+    ptr, blocks = _l4_blocks(cache, dev)
     seqs, width = block_table.shape
     slots = o_part.shape[0]
     a = MlaDecodeQ4Args(
-        _need(q_abs, "q_abs", torch.bfloat16), _need(q_pe, "q_pe", torch.bfloat16), ptr, blocks,
+        _need(q_abs, "q_abs", torch.bfloat16, dev), _need(q_pe, "q_pe", torch.bfloat16, dev), ptr, blocks,
         block_table.data_ptr(), block_table.stride(0) if seqs > 1 else max(width, 1), width, seqs, page_size, rows,
-        _need(positions, "positions", torch.int64, rows),
-        None if seq_rows is None else _need(seq_rows, "seq_rows", torch.int32, rows), softmax_scale,
-        _need(o_lat, "o_lat", torch.bfloat16), _need(o_part, "o_part", torch.float32, slots * 16 * 512),
-        _need(ml_part, "ml_part", torch.float32, slots * 16 * 2), _need(cuts, "cuts", torch.int32, slots // 2 * 4), slots)
-    _lib.call("dsv2_mla_decode_q4", ctypes.byref(a), _here(q_abs))
+        _need(positions, "positions", torch.int64, dev, rows),
+        None if seq_rows is None else _need(seq_rows, "seq_rows", torch.int32, dev, rows), softmax_scale,
+        _need(o_lat, "o_lat", torch.bfloat16, dev), _need(o_part, "o_part", torch.float32, dev, slots * 16 * 512),
+        _need(ml_part, "ml_part", torch.float32, dev, slots * 16 * 2), _need(cuts, "cuts", torch.int32, dev, slots // 2 * 4),
+        slots)
+    _lib.call("dsv2_mla_decode_q4", ctypes.byref(a), _here(dev))
     return o_lat
 
 
@@ -711,8 +719,11 @@ def _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, base, token_row, x
     nb, N, rb = b.shape
     if ka != K or nb != n_ad or rb != rank:
         raise ValueError(f"a must be [adapters, rank, {K}] and b [adapters, n, rank]")
-    if y.shape != (T, N) or y.stride(1) != 1 or not y.is_cuda:
-        raise ValueError(f"y must be a CUDA tensor [{T}, {N}] with a contiguous last dimension")
+    dev = x.get_device()
+    if y.shape != (T, N) or y.stride(1) != 1 or y.get_device() != dev:
+        raise ValueError(f"y must be a tensor [{T}, {N}] on {x.device} with a contiguous last dimension")
+    if w is not None:
+        _on(w, "w", dev)
     y_dt = {torch.bfloat16: DSV2_BF16, torch.float32: DSV2_F32}.get(y.dtype)
     if y_dt is None:
         raise NotImplementedError(f"lora output dtype {y.dtype}")
@@ -720,21 +731,23 @@ def _lora_call(x, w, a, b, ids, ranks, scales, y, low, order, base, token_row, x
     if base is not None:
         if base.dim() != 3 or base.dtype != torch.float32 or base.shape[1:] != y.shape or base.stride(2) != 1:
             raise ValueError(f"base must be fp32 [parts, {T}, {N}] with a contiguous last dimension")
-        _cuda(base, "base")
+        _on(base, "base", dev)
         n_base, base_ps, base_rs = base.shape[0], base.stride(0), base.stride(1)
         base_ptr = base.data_ptr()
     args = LoraArgs(
-        x.data_ptr(), x.stride(0) if T > 1 else K, _need(a, "a", torch.bfloat16), _need(b, "b", torch.bfloat16),
-        _need(ids, "ids", torch.int32), None if token_row is None else _need(token_row, "token_row", torch.int32, T),
-        _need(ranks, "ranks", torch.int32, n_ad), _need(scales, "scales", torch.float32, n_ad),
+        x.data_ptr(), x.stride(0) if T > 1 else K, _need(a, "a", torch.bfloat16, dev), _need(b, "b", torch.bfloat16, dev),
+        _need(ids, "ids", torch.int32, dev), None if token_row is None else _need(token_row, "token_row", torch.int32, dev, T),
+        _need(ranks, "ranks", torch.int32, dev, n_ad), _need(scales, "scales", torch.float32, dev, n_ad),
         None if w is None else w.data_ptr(), 0 if w is None else w.stride(0), base_ptr, base_ps, base_rs,
-        _need(low, "low", torch.float32, T * rank), None if order is None else _need(order, "order", torch.int32, 3 * T),
+        _need(low, "low", torch.float32, dev, T * rank),
+        None if order is None else _need(order, "order", torch.int32, dev, 3 * T),
         y.data_ptr(), y.stride(0) if T > 1 else N, max(1, min(low.numel() // max(1, T * rank), 64)), y_dt, n_base,
         ids.numel(), n_ad, rank, T, K, N)
     if xs is not None and lists is not None:
         n_xs, n_lists = _lora_gemm_buffers(T, K, rank)
-        args.xs, args.lists = _need(xs, "xs", torch.bfloat16, n_xs[0] * n_xs[1]), _need(lists, "lists", torch.int32, n_lists[0] * n_lists[1])
-    _lib.call("dsv2_lora", ctypes.byref(args), _here(x))
+        args.xs = _need(xs, "xs", torch.bfloat16, dev, n_xs[0] * n_xs[1])
+        args.lists = _need(lists, "lists", torch.int32, dev, n_lists[0] * n_lists[1])
+    _lib.call("dsv2_lora", ctypes.byref(args), _here(dev))
 
 
 def lora(*, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, ranks: torch.Tensor,
