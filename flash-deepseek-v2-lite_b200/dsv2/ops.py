@@ -664,7 +664,18 @@ def mla_prep_q4(*, qkva: torch.Tensor, kv_norm_w: torch.Tensor, eps: float, cos:
     """mla_prep into slots (int64 [B], negative = no cache write) of a 4-bit latent cache; a
     negative position marks a padding row."""
     a = _mla_prep_args(qkva, kv_norm_w, eps, cos, sin, positions, q_pe_out, q_nope_out)
-    dev = qkva.get_device()
+    dev, B = qkva.get_device(), a.batch
+    if cos.dim() != 2 or sin.shape != cos.shape or sin.stride(0) != cos.stride(0) or cos.shape[1] < 32:
+        raise ValueError("cos and sin must be alike, [rows, 32 or more]")
+    if positions.numel() not in (1, B):
+        raise ValueError(f"{positions.numel()} positions for {B} rows")
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        _on(t, name, dev)
+    _need(kv_norm_w, "kv_norm_w", torch.bfloat16, dev, 512)
+    _need(positions, "positions", torch.int64, dev)
+    _need(q_pe_out, "q_pe_out", torch.bfloat16, dev, B * 16 * 64)
+    if q_nope_out is not None:
+        _need(q_nope_out, "q_nope_out", torch.bfloat16, dev, B * 16 * 128)
     ptr, blocks = _l4_blocks(cache, dev)
     _lib.call("dsv2_mla_prep_q4", ctypes.byref(a), ptr, blocks, _need(slots, "slots", torch.int64, dev, a.batch), _here(dev))
 

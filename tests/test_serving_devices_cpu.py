@@ -92,3 +92,32 @@ def test_operands_on_another_gpu_are_refused(calls, monkeypatch, make):
     with pytest.raises(ValueError):
         f(**kw)
     assert len(calls) == 1
+
+
+def prep():
+    return ops.mla_prep_q4, dict(qkva=f32(2, 3, 3648), kv_norm_w=z(512), eps=1e-6, cos=f32(9, 32), sin=f32(9, 32), positions=i64(3),
+                                 slots=i64(3), cache=z(2, 6400, dtype=torch.uint8), q_pe_out=z(3, 16, 64), q_nope_out=z(3, 16, 128))
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("positions", i32(3)), ("positions", i64(6)[::2]), ("positions", i64(4)), ("slots", i64(2)), ("slots", i32(3)),
+    ("kv_norm_w", f32(512)), ("kv_norm_w", z(511)), ("q_pe_out", f32(3, 16, 64)), ("q_pe_out", z(2, 16, 64)), ("q_nope_out", z(2, 16, 128)),
+    ("sin", f32(8, 32)), ("sin", f32(9, 64)[:, :32]), ("cos", f32(9, 31)), ("cache", z(6399, dtype=torch.uint8))])
+def test_prep_refuses_operands_that_the_kernel_would_read_past(calls, name, bad):
+    f, kw = prep()
+    f(**kw)
+    assert len(calls) == 1
+    if name == "cos":
+        kw["sin"] = bad
+    with pytest.raises((ValueError, NotImplementedError)):
+        f(**dict(kw, **{name: bad}))
+    assert len(calls) == 1
+
+
+def test_prep_refuses_operands_on_another_gpu(calls):
+    f, kw = prep()
+    for name, t in kw.items():
+        if isinstance(t, torch.Tensor):
+            with pytest.raises(ValueError):
+                f(**dict(kw, **{name: on(t.as_subclass(torch.Tensor), 1)}))
+    assert not calls
