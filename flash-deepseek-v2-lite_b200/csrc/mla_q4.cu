@@ -205,7 +205,7 @@ struct Q4Smem {
 static_assert(sizeof(Q4Smem) <= 232448, "4-bit latent attention: shared memory exceeds 227 KB");
 
 // One launch, persistent: the rows form one stream of units (kQ4SegUnits of per-row cost, then
-// the row's 16-token blocks), cut into equal ranges, one CTA (17 warps) per SM.  A row inside
+// the row's 16-token blocks), cut into equal ranges, one CTA (20 warps, of which 17 work) per SM.  A row inside
 // one range writes o_lat; a row cut by a boundary leaves (o, m, l) partials, two slots per CTA
 // (slot 0: a row that began before the range), which mla_q4_merge_kernel joins.
 //  - warps 0-7, scores: one block (16 positions) of a tile each, all dims; the row's query
@@ -215,8 +215,8 @@ static_assert(sizeof(Q4Smem) <= 232448, "4-bit latent attention: shared memory e
 // The maximum that P is taken against is kept until a score exceeds it by 2^kQ4Slack: the score
 // warps then agree on a new one and the P V warps rescale.
 //
-// With the merge launch: 64 rows of 8192 tokens 89 us (212 MB, 2.4 TB/s), 64 x 2048 36 us, 256 ragged rows
-// of 1 .. 1900 58 us, one row of 512 12 us.  The copies alone take 49 us of the 89, scores without P V 66,
+// With the merge launch: 64 rows of 8192 tokens 90 us (212 MB, 2.4 TB/s), 64 x 2048 36 us, 256 ragged rows
+// of 1 .. 1900 58 us, one row of 512 12 us.  The copies alone take 49 us of the 90, scores without P V 66,
 // P V without scores 56: about 33 us of products and as much of conversions on each side (34.8 kFLOP and
 // 1024 nibble conversions a token, for 400 bytes) overlap with each other and with the copies only in
 // part.  Tiles of 64 positions (7 stages) and conversions taken out on one side changed nothing.
@@ -760,8 +760,8 @@ __global__ __launch_bounds__(kQ4Threads, 1) void mla_q4_kernel(const MlaQ4Params
 
 // o_lat[r, h] = sum_k 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k over the partials of a row that was cut.
 // A CTA per cut and head: 4 groups of 64 threads take every fourth partial (a long row alone has one
-// per SM), then meet in shared memory.  A launch of its own:
-// with the merge in the last CTA of a row, 148 partials of 32 KB went through one SM (75 us).
+// per SM), then meet in shared memory.  A launch of its own: with the merge in the last CTA of a row, 148
+// partials of 32 KB went through one SM, and a row of 8192 took 88 us instead of 21.
 __global__ __launch_bounds__(256) void mla_q4_merge_kernel(const MlaQ4Params p) {
   pdl_enter();
   const int h = blockIdx.y, tid = threadIdx.x;

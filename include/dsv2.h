@@ -571,7 +571,8 @@ DSV2_API int dsv2_mla_decode_noalloc(const void* q_abs, const void* q_pe, const 
  * tokens (a multiple of 16) is page_size / 16 consecutive blocks, so page g holds slots
  * [g * page_size, (g + 1) * page_size).  An element is v * scale with v in -8 .. 7 and
  * scale = max |x| of its 32 / 7 rounded to 3 mantissa bits (0, 2^-17 .. 60: larger groups
- * saturate).  An infinity saturates and a NaN becomes 0; both set DSV2_DEVERR_NONFINITE.
+ * saturate).  Of the latent dims an infinity saturates and a NaN becomes 0; the roped dims are kept
+ * as given.  An infinity or NaN in either sets DSV2_DEVERR_NONFINITE.
  * Byte layout of a block:
  *   [0, 4096)     token p at 256 p, 16 bytes per group of 32 dims; group c at place
  *                 c ^ (2 (p & 1) + 4 ((p >> 1 ^ p >> 2) & 1)); of its 32-bit word w, dim
